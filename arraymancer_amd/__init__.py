@@ -19,6 +19,8 @@ from .tensor_hip import (OPERATORS, Graph, DigitPlanes, digits_prepare, HipStora
                          cbrt, sin, cos, tan, sinh, cosh, arcsin, arccos, arctan, arcsinh, arccosh, arctanh, erf, erfc,
                          gamma, lgamma, floor, ceil, trunc, reciprocal, tround as round, bc_eq, bc_ne, bc_lt, bc_le, bc_gt,
                          bc_ge, isNaN, isNotNaN, classify, FLOAT_CLASS, sgn, floorMod, copySign, mcopySign, degToRad, radToDeg, fac, sgd_update)
+from .sequence_hip import (rotary_frequencies, rotary, rotary_into, rotary_backward, decay_attention, decay_attention_backward,
+                           decay_attention_step, group_norm, group_norm_forward, group_norm_backward)
 
 __all__ = [
     "HipTensor", "HipStorage", "Graph", "DigitPlanes", "digits_prepare", "HipError", "HipAllocError", "Layout", "Step", "OPERATORS",
@@ -33,5 +35,7 @@ __all__ = [
     "trunc", "reciprocal", "round",
     "bc_eq", "bc_ne", "bc_lt", "bc_le", "bc_gt", "bc_ge", "isNaN", "isNotNaN", "classify", "FLOAT_CLASS", "sgn", "floorMod",
     "copySign", "mcopySign", "degToRad", "radToDeg", "fac", "sgd_update",
+    "rotary_frequencies", "rotary", "rotary_into", "rotary_backward", "decay_attention", "decay_attention_backward",
+    "decay_attention_step", "group_norm", "group_norm_forward", "group_norm_backward",
     "read_npy", "write_npy", "load_library",
 ]

@@ -24,6 +24,8 @@ UOP = dict(copy=0, neg=1, relu=2, sigmoid=3, tanh=4, exp=5, abs=6, sqrt=7, squar
            arccos=18, arctan=19, arcsinh=20, arccosh=21, arctanh=22, cbrt=23, erf=24, erfc=25, gamma=26,
            lgamma=27, floor=28, ceil=29, trunc=30, round=31, reciprocal=32, degtorad=33, radtodeg=34, fac=35)
 EPI = dict(none=0, bias=1, relu=2, bias_relu=3)
+ROTARY = dict(half=0, interleaved=1)
+ACT = dict(none=0, relu=1, silu=2)
 RED = dict(sum=0, product=1, min=2, max=3)
 
 SFX = {np.dtype(np.float32): "f32", np.dtype(np.float64): "f64",
@@ -117,6 +119,14 @@ def _signatures():
             sig[f"am_hip_sgd_update_{sfx}"] = (ci, [ci, vp, vp, vp, ct])
             sig[f"am_hip_gru_gates_{sfx}"] = (ci, [i64, i64, vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, i64])
             sig[f"am_hip_gru_gates_backward_{sfx}"] = (ci, [i64, i64, vp, vp, vp, vp, vp, vp, i64, vp, i64, vp, i64])
+            sig[f"am_hip_rotary_{sfx}"] = (ci, [i64] * 5 + [ci, ci, ct] + [vp, i64, i64] + [vp] + [vp, i64, i64, i64] * 2)
+            sig[f"am_hip_decay_attention_{sfx}"] = (ci, [i64] * 6 + [ct, vp, vp] + [vp, i64, i64, i64] * 3 + [vp, i64, i64] +
+                                                    [vp, i64, i64, i64] + [vp, i64, i64])
+            sig[f"am_hip_decay_attention_backward_{sfx}"] = (ci, [i64] * 6 + [ct, vp, vp] + [vp, i64, i64, i64] * 4 +
+                                                             [vp, i64, i64] * 2 + [vp, i64, i64, i64] * 3 + [vp, i64, i64])
+            sig[f"am_hip_decay_attention_step_{sfx}"] = (ci, [i64] * 5 + [ct, vp] + [vp, i64, i64] * 5)
+            sig[f"am_hip_group_norm_{sfx}"] = (ci, [i64] * 4 + [ct, ci] + [vp, i64, i64] + [vp, vp] + [vp, i64, i64] + [vp, vp])
+            sig[f"am_hip_group_norm_backward_{sfx}"] = (ci, [i64] * 4 + [ci] + [vp, i64, i64] * 2 + [vp] * 4 + [vp, i64, i64] + [vp, vp])
             sig[f"am_hip_softmax_cross_entropy_{sfx}"] = (ci, [i64, i64, vp, i64, i64, vp, i64, i64, ctypes.POINTER(ct)])
             sig[f"am_hip_sigmoid_cross_entropy_{sfx}"] = (ci, [i64, i64, vp, i64, i64, vp, i64, i64, ctypes.POINTER(ct)])
             sig[f"am_hip_sigmoid_cross_entropy_backward_{sfx}"] = (ci, [i64, i64, ct, vp, i64, i64, vp, i64, i64, vp, i64, i64])

@@ -21,6 +21,7 @@ SOURCES = [
     "runtime.hip", "diag.hip",
     "elementwise_f32.hip", "elementwise_f64.hip", "elementwise_i32.hip", "elementwise_i64.hip",
     "gemm_f32.hip", "gemm_f64.hip", "gemm_i32.hip", "gemm_i64.hip", "gemv.hip", "im2col.hip", "reduce.hip", "loss.hip", "gru.hip", "optim.hip",
+    "rotary.hip", "decay_attention.hip", "group_norm.hip",
 ]
 
 # -ffp-contract=off: every float operation of an epilogue / map body is rounded on its own, so

@@ -661,6 +661,101 @@ int am_hip_gru_gates_backward_f32(int64_t batch, int64_t H, const float* dnext, 
 int am_hip_gru_gates_backward_f64(int64_t batch, int64_t H, const double* dnext, const double* h, const double* r, const double* z,
                                   const double* n, const double* uh, int64_t ld_in, double* dw3x, int64_t ldw, double* du3h, int64_t ldu);
 
+/* ---------------------------------------------------------------- sequence mixing
+ * The reference's recurrent layer is the GRU above, one token after the other. The following operators make a layer of the
+ * same use - a state of fixed size per sequence, one step per new token - whose training and whose prompts run over all
+ * tokens at once: rotary positions on queries and keys, linear attention with a decay for each head, and a group norm of
+ * every head's output (which serves channels-last images as well). No counterpart in the reference. Strides are in elements;
+ * the last dimension of every operand has unit stride. Results must not overlap operands unless it is said.
+ *
+ * Rotary positions. x and out [batch, tokens, heads, dim] (strides _b, _t, _h): the first rot_dim elements of a head are
+ * rot_dim / 2 pairs, element i with i + rot_dim / 2 (AM_ROTARY_HALF) or 2 i with 2 i + 1 (AM_ROTARY_INTERLEAVED). Pair i of
+ * a token at position p turns by p * frequencies[i] and is multiplied by `scale`; the rest of the head is copied.
+ * inverse != 0 turns the other way: that is also the gradient. positions [batch, tokens] (strides pos_b, pos_t, 0 allowed;
+ * any sign) or NULL for the token's index. The angles are formed in double and reduced before the sines, so far positions
+ * lose nothing. out may be x itself with x's strides (in place). */
+#define AM_ROTARY_HALF        0
+#define AM_ROTARY_INTERLEAVED 1
+int am_hip_rotary_f32(int64_t batch, int64_t tokens, int64_t heads, int64_t dim, int64_t rot_dim, int layout, int inverse,
+                      float scale, const int64_t* positions, int64_t pos_b, int64_t pos_t, const double* frequencies,
+                      const float* x, int64_t x_b, int64_t x_t, int64_t x_h, float* out, int64_t out_b, int64_t out_t, int64_t out_h);
+int am_hip_rotary_f64(int64_t batch, int64_t tokens, int64_t heads, int64_t dim, int64_t rot_dim, int layout, int inverse,
+                      double scale, const int64_t* positions, int64_t pos_b, int64_t pos_t, const double* frequencies,
+                      const double* x, int64_t x_b, int64_t x_t, int64_t x_h, double* out, int64_t out_b, int64_t out_t, int64_t out_h);
+
+/* Linear attention with a decay for each head. A head keeps a state S [dk, dv]; token t of its sequence does
+ *   S <- e^g S + k_t^T v_t        out_t = scale * q_t S        g = log_decay[head] (<= 0; -infinity keeps the last token only)
+ * q [batch, tokens, heads, dk], k [batch, tokens, kv_heads, dk], v [batch, tokens, kv_heads, dv], out [batch, tokens, heads, dv];
+ * head h reads key / value head h / (heads / kv_heads). 1 <= dk, dv <= 256. state_in [batch, heads, dk, dv] (strides si_b,
+ * si_h; each head's [dk, dv] contiguous) is the state before the first token, NULL for zeros; state_out alike receives the
+ * state behind the last token, NULL when it is not wanted; it may be state_in. lengths [batch] (device, NULL: all tokens):
+ * sequence b has its first lengths[b] tokens (clamped to 0 .. tokens); what lies behind them is not read into any result,
+ * and out is 0 there. A NaN or an infinity in a token reaches the outputs of the tokens behind it, and may reach those of
+ * up to 63 tokens before it. */
+int am_hip_decay_attention_f32(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dk, int64_t dv, float scale,
+                               const float* log_decay, const int64_t* lengths,
+                               const float* q, int64_t q_b, int64_t q_t, int64_t q_h, const float* k, int64_t k_b, int64_t k_t, int64_t k_h,
+                               const float* v, int64_t v_b, int64_t v_t, int64_t v_h, const float* state_in, int64_t si_b, int64_t si_h,
+                               float* out, int64_t o_b, int64_t o_t, int64_t o_h, float* state_out, int64_t so_b, int64_t so_h);
+int am_hip_decay_attention_f64(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dk, int64_t dv, double scale,
+                               const double* log_decay, const int64_t* lengths,
+                               const double* q, int64_t q_b, int64_t q_t, int64_t q_h, const double* k, int64_t k_b, int64_t k_t, int64_t k_h,
+                               const double* v, int64_t v_b, int64_t v_t, int64_t v_h, const double* state_in, int64_t si_b, int64_t si_h,
+                               double* out, int64_t o_b, int64_t o_t, int64_t o_h, double* state_out, int64_t so_b, int64_t so_h);
+/* Its gradients: from grad_out [batch, tokens, heads, dv] and grad_state_out [batch, heads, dk, dv] (NULL: zeros) those of q,
+ * k, v (shapes of q, k, v; a shared key / value head's is the sum over the heads that read it, added in the heads' order)
+ * and of state_in (grad_state_in, NULL when not wanted; it may be grad_state_out). The decays are constants of the layer,
+ * no gradient of log_decay is formed. Behind lengths[b] the gradients are 0. */
+int am_hip_decay_attention_backward_f32(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dk, int64_t dv, float scale,
+                                        const float* log_decay, const int64_t* lengths,
+                                        const float* grad_out, int64_t g_b, int64_t g_t, int64_t g_h,
+                                        const float* q, int64_t q_b, int64_t q_t, int64_t q_h, const float* k, int64_t k_b, int64_t k_t, int64_t k_h,
+                                        const float* v, int64_t v_b, int64_t v_t, int64_t v_h, const float* state_in, int64_t si_b, int64_t si_h,
+                                        const float* grad_state_out, int64_t gso_b, int64_t gso_h,
+                                        float* grad_q, int64_t gq_b, int64_t gq_t, int64_t gq_h, float* grad_k, int64_t gk_b, int64_t gk_t, int64_t gk_h,
+                                        float* grad_v, int64_t gv_b, int64_t gv_t, int64_t gv_h, float* grad_state_in, int64_t gsi_b, int64_t gsi_h);
+int am_hip_decay_attention_backward_f64(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dk, int64_t dv, double scale,
+                                        const double* log_decay, const int64_t* lengths,
+                                        const double* grad_out, int64_t g_b, int64_t g_t, int64_t g_h,
+                                        const double* q, int64_t q_b, int64_t q_t, int64_t q_h, const double* k, int64_t k_b, int64_t k_t, int64_t k_h,
+                                        const double* v, int64_t v_b, int64_t v_t, int64_t v_h, const double* state_in, int64_t si_b, int64_t si_h,
+                                        const double* grad_state_out, int64_t gso_b, int64_t gso_h,
+                                        double* grad_q, int64_t gq_b, int64_t gq_t, int64_t gq_h, double* grad_k, int64_t gk_b, int64_t gk_t, int64_t gk_h,
+                                        double* grad_v, int64_t gv_b, int64_t gv_t, int64_t gv_h, double* grad_state_in, int64_t gsi_b, int64_t gsi_h);
+/* One token of every sequence: q [batch, heads, dk], k [batch, kv_heads, dk], v [batch, kv_heads, dv], out [batch, heads, dv];
+ * `state` [batch, heads, dk, dv] (strides s_b, s_h; each head's [dk, dv] contiguous) is updated in place. */
+int am_hip_decay_attention_step_f32(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dk, int64_t dv, float scale, const float* log_decay,
+                                    const float* q, int64_t q_b, int64_t q_h, const float* k, int64_t k_b, int64_t k_h,
+                                    const float* v, int64_t v_b, int64_t v_h, float* state, int64_t s_b, int64_t s_h, float* out, int64_t o_b, int64_t o_h);
+int am_hip_decay_attention_step_f64(int64_t batch, int64_t heads, int64_t kv_heads, int64_t dk, int64_t dv, double scale, const double* log_decay,
+                                    const double* q, int64_t q_b, int64_t q_h, const double* k, int64_t k_b, int64_t k_h,
+                                    const double* v, int64_t v_b, int64_t v_h, double* state, int64_t s_b, int64_t s_h, double* out, int64_t o_b, int64_t o_h);
+
+/* Group norm with an activation, channels last: x and y [batch, spatial, channels] (strides _n, _s); the channels form
+ * `groups` equal groups, and each (sample, group) is normalised over its spatial * channels / groups elements:
+ *   y = act((x - mean) / sqrt(variance + eps) * weight[c] + bias[c])
+ * weight and bias [channels] may be NULL (1 and 0). mean and rstd [batch, groups] (both or NULL) receive what the backward
+ * pass needs. */
+#define AM_ACT_NONE 0
+#define AM_ACT_RELU 1   /* (0 >= z) ? 0 : z            */
+#define AM_ACT_SILU 2   /* z / (1 + e^-z)              */
+int am_hip_group_norm_f32(int64_t batch, int64_t spatial, int64_t channels, int64_t groups, float eps, int activation,
+                          const float* x, int64_t x_n, int64_t x_s, const float* weight, const float* bias,
+                          float* y, int64_t y_n, int64_t y_s, float* mean, float* rstd);
+int am_hip_group_norm_f64(int64_t batch, int64_t spatial, int64_t channels, int64_t groups, double eps, int activation,
+                          const double* x, int64_t x_n, int64_t x_s, const double* weight, const double* bias,
+                          double* y, int64_t y_n, int64_t y_s, double* mean, double* rstd);
+/* Its gradients from dy, x and the mean and rstd that the forward pass kept: dx [batch, spatial, channels], and dweight and
+ * dbias [channels] (each may be NULL), summed over batch and spatial in a fixed order. */
+int am_hip_group_norm_backward_f32(int64_t batch, int64_t spatial, int64_t channels, int64_t groups, int activation,
+                                   const float* dy, int64_t dy_n, int64_t dy_s, const float* x, int64_t x_n, int64_t x_s,
+                                   const float* weight, const float* bias, const float* mean, const float* rstd,
+                                   float* dx, int64_t dx_n, int64_t dx_s, float* dweight, float* dbias);
+int am_hip_group_norm_backward_f64(int64_t batch, int64_t spatial, int64_t channels, int64_t groups, int activation,
+                                   const double* dy, int64_t dy_n, int64_t dy_s, const double* x, int64_t x_n, int64_t x_s,
+                                   const double* weight, const double* bias, const double* mean, const double* rstd,
+                                   double* dx, int64_t dx_n, int64_t dx_s, double* dweight, double* dbias);
+
 /* values[t][i] <- values[t][i] - learning_rate * grads[t][i] for `count` contiguous tensors of sizes[t] elements in ONE
  * launch (64 tensors per launch beyond that). Replaces the SGD optimizer's update, one apply2_inline per parameter
  * (src/arraymancer/nn/optimizers/optimizers.nim:35-51); same expression, the product rounded before the subtraction. */
