@@ -44,67 +44,441 @@ __device__ __forceinline__ double dev_exp(double v) { return exp(v); }
 // e^{g n}; e^0 also where g is -infinity
 template <typename T> __device__ __forceinline__ T power(T g, int64_t n) { return n == 0 ? (T)1 : dev_exp(g * (T)n); }
 
-// Token by token: a wavefront owns 16 columns of one head's state, a lane one column and R rows of it (rows
-// R * (lane / 16) ...), so a token's output is a sum over registers and two butterflies. Right for any size; its time is
-// the chain of tokens.
-template <typename T, int R, bool BACK>
-__global__ __launch_bounds__(64) void walk(Role<T> p) {
-  const int64_t b = blockIdx.z;
-  const int h = (int)blockIdx.y * p.out_group + p.out_member;
-  const int lane = (int)threadIdx.x, col = (int)blockIdx.x * 16 + (lane & 15), r0 = (lane >> 4) * R;
-  const bool live = col < p.dc;
-  const int c = live ? col : p.dc - 1;
-  int64_t n = p.tokens;
-  if (p.lengths) { const int64_t l = p.lengths[b]; n = l < 0 ? 0 : (l < n ? l : n); }
-  const T lam = dev_exp(p.log_decay[h]);
-  const T* qa = p.a.p + b * p.a.b + (h / p.a.group) * p.a.h;
-  const T* kb = p.b.p + b * p.b.b + (h / p.b.group) * p.b.h;
-  const T* vc = p.c.p + b * p.c.b + (h / p.c.group) * p.c.h + c;
-  T* out = p.out + b * p.o_b + (int64_t)blockIdx.y * p.o_h + c;
-  T s[R];
+template <typename T> struct Mma;
+template <> struct Mma<float> {
+  typedef float acc_t __attribute__((ext_vector_type(4)));
+  static __device__ __forceinline__ acc_t mma(float a, float b, acc_t c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+  // the operand row that lane % 16 = r brings, so that register i of lane group g holds row 4 g + i of the result
+  static __device__ __forceinline__ int row(int r) { return r; }
+};
+template <> struct Mma<double> {
+  typedef double acc_t __attribute__((ext_vector_type(4)));
+  static __device__ __forceinline__ acc_t mma(double a, double b, acc_t c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
+  // (this instruction's result has row 4 i + g there)
+  static __device__ __forceinline__ int row(int r) { return 4 * (r & 3) + (r >> 2); }
+};
+
+// ---- chunks of 32 tokens on the matrix cores ---------------------------------------------------------------------------
+//
+// For the tokens of a chunk, i and j counted within it, and the state S in front of it,
+//     o_i = sum_{j <= i} A_ij c_j + e^{g (i + after)} a_i S      A_ij = e^{g (i - j)} (a_i . b_j)
+//     S <- e^{g N} S + sum_j e^{g (N - after - j)} b_j^T c_j
+// so a chunk is four products: a b^T (32 x 32), A c, a S and b^T c. A workgroup of four wavefronts walks the chunks of one
+// head, a wavefront owning 16 columns of S and of o for all da rows, as accumulators that never leave its registers:
+//   - the 16 x 16 x 4 product leaves four consecutive rows of its result in a lane, and the sum over k may take its k in any
+//     order that both operands share: register i of S's tile is the right operand of the i-th of four instructions whose k
+//     are the rows 4 g + i. So S enters a S as it stands.
+//   - a b^T is computed transposed, so that a lane's four values lie next to each other in a row of A in LDS; the three
+//     tiles on and under the diagonal go to three wavefronts.
+//   - c is read straight into the layout of a right operand, which A c and b^T c share.
+// a and b go through LDS in rows padded by 16 bytes; the next chunk's are on their way in registers meanwhile.
+// All exponents of e^g are differences that the mask leaves >= 0, so nothing overflows however long the text.
+//
+// Where the heads alone do not fill the device, the tokens are cut into segments: `segment_sums` adds up each segment's
+// share of the state, `segment_states` carries them from segment to segment, and `chunks` starts every segment from its own.
+constexpr int kChunk = 32;
+constexpr int kCols = 64;      // columns of a workgroup
+
+template <typename T> struct Plan {
+  T* states;                   // [batch * heads / out_group][segments][da][dc]: the state in front of each segment; null: one segment
+  int segments, slices;
+  int64_t seg_tokens;          // a multiple of kChunk
+  int groups;                  // batch * heads / out_group
+  bool whole_a, whole_b;       // rows of a, b are whole 16-byte vectors
+};
+
+// Rows of `n` tokens (one after the other from local token i0 on) of an operand, as 16-byte vectors in registers.
+template <typename T, int DA> struct Tile {
+  static constexpr int V = 16 / (int)sizeof(T), PER_ROW = DA / V, NV = kChunk * PER_ROW / 256;
+  typedef T vec_t __attribute__((ext_vector_type(V)));
+  typedef T loose_t __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+  static constexpr int PITCH = DA + V;
+  vec_t v[NV];
+
+  // p: the first token's row; step: to the next token
+  __device__ __forceinline__ void load(const T* p, int64_t step, int n, int da, bool whole) {
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const int r = r0 + i;
-    s[i] = (p.s0 && r < p.da) ? p.s0[b * p.s0_b + h * p.s0_h + r * p.s0_r + c * p.s0_c] : (T)0;
-  }
-  for (int64_t i = 0; i < n; ++i) {
-    const int64_t t = BACK ? n - 1 - i : i;
-    const T v = vc[t * p.c.t];
-    T o = (T)0;
+    for (int u = 0; u < NV; ++u) {
+      const int f = (int)threadIdx.x + u * 256, row = f / PER_ROW, c = (f - row * PER_ROW) * V;
+      v[u] = (vec_t)((T)0);
+      if (row < n) {
+        const T* q = p + row * step + c;
+        if (whole) {
+          if (c < da) v[u] = *(const loose_t*)q;
+        } else {
 #pragma unroll
-    for (int e = 0; e < R; ++e) {
-      const int r = r0 + e;
-      if (r < p.da) {
-        const T kv = kb[t * p.b.t + r] * p.scale_b * v;
-        if constexpr (BACK) s[e] += kv;
-        else s[e] = s[e] * lam + kv;
-        o += qa[t * p.a.t + r] * p.scale_a * s[e];
-        if constexpr (BACK) s[e] *= lam;
+          for (int e = 0; e < V; ++e)
+            if (c + e < da) v[u][e] = q[e];
+        }
       }
     }
-    o += __shfl_xor(o, 16, 64);
-    o += __shfl_xor(o, 32, 64);
-    if (live && lane < 16) out[t * p.o_t] = p.add ? out[t * p.o_t] + o : o;
   }
-  if (live && lane < 16 && !p.add)
-    for (int64_t t = n; t < p.tokens; ++t) out[t * p.o_t] = (T)0;     // behind the sequence
-  if (p.s1 && live) {
+  __device__ __forceinline__ void store(T* lds, T scale) const {
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int r = r0 + i;
-      if (r < p.da) p.s1[b * p.s1_b + h * p.s1_h + r * p.s1_r + c * p.s1_c] = s[i];
+    for (int u = 0; u < NV; ++u) {
+      const int f = (int)threadIdx.x + u * 256, row = f / PER_ROW, c = (f - row * PER_ROW) * V;
+      *(vec_t*)(lds + row * PITCH + c) = v[u] * scale;
     }
   }
+};
+
+// Four neighbouring elements of LDS.
+template <typename T> __device__ __forceinline__ void four(const T* lds, T (&out)[4]) {
+  constexpr int V = 16 / (int)sizeof(T);
+  typedef T vec_t __attribute__((ext_vector_type(V)));
+#pragma unroll
+  for (int i = 0; i < 4; i += V) {
+    const vec_t w = *(const vec_t*)(lds + i);
+#pragma unroll
+    for (int e = 0; e < V; ++e) out[i + e] = w[e];
+  }
+}
+
+// What a workgroup works on. The slices of one (head, segment) read the same a and b: they get ids that are equal modulo
+// the eight dies, whose L2 they share.
+struct Work { int slice, segment, group; bool live; };
+template <typename T> __device__ __forceinline__ Work work_of(const Plan<T>& pl, int segments) {
+  const unsigned id = blockIdx.x, rest = id >> 3;
+  Work w;
+  w.slice = (int)(rest % (unsigned)pl.slices);
+  const unsigned item = (rest / (unsigned)pl.slices) * 8 + (id & 7);
+  w.segment = (int)(item % (unsigned)segments);
+  w.group = (int)(item / (unsigned)segments);
+  w.live = w.group < pl.groups;
+  return w;
+}
+
+template <typename T> __device__ __forceinline__ int64_t length_of(const Role<T>& p, int64_t b) {
+  if (!p.lengths) return p.tokens;
+  const int64_t l = p.lengths[b];
+  return l < 0 ? 0 : (l < p.tokens ? l : p.tokens);
+}
+
+// One wavefront's share of a chunk's sum over the tokens: S <- e^{g N} S + b^T (w c), c given weighted.
+template <typename T, int DA>
+__device__ __forceinline__ void add_tokens(typename Mma<T>::acc_t (&S)[DA / 16], const T* sB, const T (&wc)[2][4], T lam, int pr, int g) {
+  constexpr int PITCH = Tile<T, DA>::PITCH;
+#pragma unroll
+  for (int kt = 0; kt < DA / 16; ++kt) {
+    S[kt] *= lam;
+#pragma unroll
+    for (int jt = 0; jt < 2; ++jt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        S[kt] = Mma<T>::mma(sB[(16 * jt + 4 * g + r) * PITCH + 16 * kt + pr], wc[jt][r], S[kt]);
+  }
+}
+
+// c of a chunk, in the layout of a right operand: register r of tile jt is token 16 jt + 4 g + r.
+template <typename T>
+__device__ __forceinline__ void load_c(T (&c)[2][4], const T* p, int64_t step, int n, int g, bool live) {
+#pragma unroll
+  for (int jt = 0; jt < 2; ++jt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int j = 16 * jt + 4 * g + r;
+      c[jt][r] = (live && j < n) ? p[j * step] : (T)0;
+    }
+}
+
+// e^{g (n - after - j)} of this lane's tokens
+template <typename T>
+__device__ __forceinline__ void weights(T (&w)[2][4], T ld, int n, int after, int g) {
+#pragma unroll
+  for (int jt = 0; jt < 2; ++jt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int e = n - after - (16 * jt + 4 * g + r);
+      w[jt][r] = power(ld, (int64_t)(e > 0 ? e : 0));
+    }
+}
+
+template <typename T, int DA, bool BACK>
+__global__ __launch_bounds__(256) void chunks(Role<T> p, Plan<T> pl) {
+  typedef typename Mma<T>::acc_t acc_t;
+  typedef Tile<T, DA> tile_t;
+  constexpr int KT = DA / 16, V = tile_t::V, PITCH = tile_t::PITCH, APITCH = kChunk + V;
+  constexpr int after = BACK ? 0 : 1;
+  __shared__ __attribute__((aligned(16))) T sQ[kChunk * PITCH];
+  __shared__ __attribute__((aligned(16))) T sB[kChunk * PITCH];
+  __shared__ __attribute__((aligned(16))) T sA[kChunk * APITCH];
+  const Work w = work_of(pl, pl.segments);
+  if (!w.live) return;
+  const int heads = (int)(p.heads / p.out_group);
+  const int64_t b = w.group / heads;
+  const int oh = (int)(w.group - b * heads), h = oh * p.out_group + p.out_member;
+  const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63, g = lane >> 4, lr = lane & 15, pr = Mma<T>::row(lr);
+  const int col = w.slice * kCols + wave * 16 + lr;
+  const bool live = col < p.dc;
+  const int64_t n = length_of(p, b);
+  const int64_t lo = w.segment * pl.seg_tokens;
+  int64_t hi = lo + pl.seg_tokens;
+  if (hi > p.tokens) hi = p.tokens;
+  const int64_t end = hi < n ? hi : n;                      // local tokens lo .. end of the walk
+  // local token i is token i, or n - 1 - i
+  const int64_t first = BACK ? n - 1 - lo : lo, dir = BACK ? -1 : 1;
+  const T* pa = p.a.p + b * p.a.b + (h / p.a.group) * p.a.h + first * p.a.t;
+  const T* pb = p.b.p + b * p.b.b + (h / p.b.group) * p.b.h + first * p.b.t;
+  const T* pc = p.c.p + b * p.c.b + (h / p.c.group) * p.c.h + first * p.c.t + col;
+  T* po = p.out + b * p.o_b + oh * p.o_h + col;
+  const int64_t ta = dir * p.a.t, tb = dir * p.b.t, tc = dir * p.c.t;
+
+  acc_t S[KT];
+  const T* s0 = pl.states ? pl.states + ((int64_t)w.group * pl.segments + w.segment) * p.da * p.dc : (p.s0 ? p.s0 + b * p.s0_b + h * p.s0_h : nullptr);
+  const int64_t s0_r = pl.states ? p.dc : p.s0_r, s0_c = pl.states ? 1 : p.s0_c;
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int d = 16 * kt + 4 * g + r;
+      S[kt][r] = (s0 && live && d < p.da) ? s0[d * s0_r + col * s0_c] : (T)0;
+    }
+  const T ld = p.log_decay[h];
+  T reach[2][4], mask[2][4], wt[2][4];
+#pragma unroll
+  for (int it = 0; it < 2; ++it)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      reach[it][r] = power(ld, (int64_t)(16 * it + 4 * g + r + after));
+      const int apart = 16 * it + lr - 4 * g - r;          // i - j of tile distance `it`, transposed
+      mask[it][r] = apart >= 0 ? power(ld, (int64_t)apart) : (T)0;
+    }
+  weights(wt, ld, kChunk, after, g);
+  T lam = power(ld, (int64_t)kChunk);
+
+  tile_t a, k;
+  T c[2][4], cn[2][4];
+  const int64_t total = end - lo;
+  {
+    const int m = total < kChunk ? (int)(total < 0 ? 0 : total) : kChunk;
+    a.load(pa, ta, m, p.da, pl.whole_a);
+    k.load(pb, tb, m, p.da, pl.whole_b);
+    load_c(cn, pc, tc, m, g, live);
+  }
+  for (int64_t at = 0; at < total; at += kChunk) {
+    const int m = total - at < kChunk ? (int)(total - at) : kChunk;
+    a.store(sQ, p.scale_a);
+    k.store(sB, p.scale_b);
+#pragma unroll
+    for (int jt = 0; jt < 2; ++jt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) c[jt][r] = cn[jt][r];
+    __syncthreads();
+    if (at + kChunk < total) {
+      const int64_t next = at + kChunk;
+      const int mn = total - next < kChunk ? (int)(total - next) : kChunk;
+      a.load(pa + next * ta, ta, mn, p.da, pl.whole_a);
+      k.load(pb + next * tb, tb, mn, p.da, pl.whole_b);
+      load_c(cn, pc + next * tc, tc, mn, g, live);
+    }
+    if (wave < 3) {                                         // tiles (0, 0), (1, 0), (1, 1) of A
+      const int it = wave ? 1 : 0, jt = wave == 2 ? 1 : 0;
+      acc_t t = (acc_t)((T)0);
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+        T x[4], y[4];
+        four(sB + (16 * jt + pr) * PITCH + 16 * kt + 4 * g, x);
+        four(sQ + (16 * it + lr) * PITCH + 16 * kt + 4 * g, y);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) t = Mma<T>::mma(x[r], y[r], t);
+      }
+      T* q = sA + (16 * it + lr) * APITCH + 16 * jt + 4 * g;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const bool under = it > jt || lr >= 4 * g + r;
+        q[r] = under ? t[r] * (it > jt ? mask[1][r] : mask[0][r]) : (T)0;
+      }
+    }
+    acc_t o[2];
+#pragma unroll
+    for (int it = 0; it < 2; ++it) {
+      o[it] = (acc_t)((T)0);
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+        T x[4];
+        four(sQ + (16 * it + pr) * PITCH + 16 * kt + 4 * g, x);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[it] = Mma<T>::mma(x[r], S[kt][r], o[it]);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[it][r] *= reach[it][r];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int it = 0; it < 2; ++it)
+#pragma unroll
+      for (int jt = 0; jt <= it; ++jt) {
+        T x[4];
+        four(sA + (16 * it + pr) * APITCH + 16 * jt + 4 * g, x);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[it] = Mma<T>::mma(x[r], c[jt][r], o[it]);
+      }
+    if (m < kChunk) { weights(wt, ld, m, after, g); lam = power(ld, (int64_t)m); }
+#pragma unroll
+    for (int jt = 0; jt < 2; ++jt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) c[jt][r] *= wt[jt][r];
+    add_tokens<T, DA>(S, sB, c, lam, pr, g);
+#pragma unroll
+    for (int it = 0; it < 2; ++it)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = 16 * it + 4 * g + r;
+        if (live && i < m) {
+          T* q = po + (first + dir * (at + i)) * p.o_t;
+          *q = p.add ? *q + o[it][r] : o[it][r];
+        }
+      }
+    __syncthreads();
+  }
+  if (live && !p.add) {                                     // behind the sequence
+    for (int64_t t = (lo > n ? lo : n) + g; t < hi; t += 4) po[t * p.o_t] = (T)0;
+  }
+  if (p.s1 && w.segment == pl.segments - 1 && live) {
+    T* s1 = p.s1 + b * p.s1_b + h * p.s1_h + col * p.s1_c;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int d = 16 * kt + 4 * g + r;
+        if (d < p.da) s1[d * p.s1_r] = S[kt][r];
+      }
+  }
+}
+
+// The share of segment s (all but the last) in the state behind it, into the states' slot s + 1.
+template <typename T, int DA, bool BACK>
+__global__ __launch_bounds__(256) void segment_sums(Role<T> p, Plan<T> pl) {
+  typedef typename Mma<T>::acc_t acc_t;
+  typedef Tile<T, DA> tile_t;
+  constexpr int KT = DA / 16, PITCH = tile_t::PITCH;
+  constexpr int after = BACK ? 0 : 1;
+  __shared__ __attribute__((aligned(16))) T sB[2][kChunk * PITCH];
+  const Work w = work_of(pl, pl.segments - 1);
+  if (!w.live) return;
+  const int heads = (int)(p.heads / p.out_group);
+  const int64_t b = w.group / heads;
+  const int h = (int)(w.group - b * heads) * p.out_group + p.out_member;
+  const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63, g = lane >> 4, lr = lane & 15, pr = Mma<T>::row(lr);
+  const int col = w.slice * kCols + wave * 16 + lr;
+  const bool live = col < p.dc;
+  const int64_t n = length_of(p, b);
+  const int64_t lo = w.segment * pl.seg_tokens;
+  const int64_t end = lo + pl.seg_tokens < n ? lo + pl.seg_tokens : n;
+  const int64_t first = BACK ? n - 1 - lo : lo, dir = BACK ? -1 : 1;
+  const T* pb = p.b.p + b * p.b.b + (h / p.b.group) * p.b.h + first * p.b.t;
+  const T* pc = p.c.p + b * p.c.b + (h / p.c.group) * p.c.h + first * p.c.t + col;
+  const int64_t tb = dir * p.b.t, tc = dir * p.c.t;
+  acc_t S[KT];
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt) S[kt] = (acc_t)((T)0);
+  const T ld = p.log_decay[h];
+  T wt[2][4];
+  weights(wt, ld, kChunk, after, g);
+  T lam = power(ld, (int64_t)kChunk);
+  tile_t k;
+  T c[2][4], cn[2][4];
+  const int64_t total = end - lo;
+  {
+    const int m = total < kChunk ? (int)(total < 0 ? 0 : total) : kChunk;
+    k.load(pb, tb, m, p.da, pl.whole_b);
+    load_c(cn, pc, tc, m, g, live);
+  }
+  int turn = 0;
+  for (int64_t at = 0; at < total; at += kChunk, turn ^= 1) {
+    const int m = total - at < kChunk ? (int)(total - at) : kChunk;
+    k.store(sB[turn], p.scale_b);                           // (two buffers: one barrier a chunk)
+    if (m < kChunk) { weights(wt, ld, m, after, g); lam = power(ld, (int64_t)m); }
+#pragma unroll
+    for (int jt = 0; jt < 2; ++jt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) c[jt][r] = cn[jt][r] * wt[jt][r];
+    __syncthreads();
+    if (at + kChunk < total) {
+      const int64_t next = at + kChunk;
+      const int mn = total - next < kChunk ? (int)(total - next) : kChunk;
+      k.load(pb + next * tb, tb, mn, p.da, pl.whole_b);
+      load_c(cn, pc + next * tc, tc, mn, g, live);
+    }
+    add_tokens<T, DA>(S, sB[turn], c, lam, pr, g);
+  }
+  if (!live) return;
+  T* s1 = pl.states + ((int64_t)w.group * pl.segments + w.segment + 1) * p.da * p.dc + col;
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int d = 16 * kt + 4 * g + r;
+      if (d < p.da) s1[(int64_t)d * p.dc] = S[kt][r];
+    }
+}
+
+// From the segments' shares to the state in front of each: one lane per element of a head's state.
+template <typename T>
+__global__ __launch_bounds__(256) void segment_states(Role<T> p, Plan<T> pl) {
+  const int per = p.da * p.dc;
+  const int blocks = (per + 255) / 256;
+  const int group = (int)(blockIdx.x / (unsigned)blocks);
+  const int i = (int)(blockIdx.x - (unsigned)group * (unsigned)blocks) * 256 + (int)threadIdx.x;
+  if (i >= per) return;
+  const int heads = (int)(p.heads / p.out_group);
+  const int64_t b = group / heads;
+  const int h = (int)(group - b * heads) * p.out_group + p.out_member;
+  const int64_t n = length_of(p, b);
+  const T ld = p.log_decay[h];
+  const int r = i / p.dc, c = i - r * p.dc;
+  T* at = pl.states + (int64_t)group * pl.segments * per + i;
+  T s = p.s0 ? p.s0[b * p.s0_b + h * p.s0_h + r * p.s0_r + c * p.s0_c] : (T)0;
+  at[0] = s;
+#pragma unroll 4
+  for (int k = 1; k < pl.segments; ++k) {
+    int64_t len = n - (k - 1) * pl.seg_tokens;
+    len = len < 0 ? 0 : (len < pl.seg_tokens ? len : pl.seg_tokens);
+    s = s * power(ld, len) + at[(int64_t)k * per];
+    at[(int64_t)k * per] = s;
+  }
+}
+
+template <typename T, int DA, bool BACK>
+static int run_chunks(const Role<T>& p) {
+  Plan<T> pl = {};
+  pl.slices = (p.dc + kCols - 1) / kCols;
+  pl.groups = (int)(p.batch * (p.heads / p.out_group));
+  pl.segments = 1;
+  constexpr int V = 16 / (int)sizeof(T);
+  pl.whole_a = pl.whole_b = p.da % V == 0;
+  const int64_t wgs = (int64_t)pl.groups * pl.slices;
+  const int64_t n_chunks = (p.tokens + kChunk - 1) / kChunk;
+  // Two workgroups for every CU; a segment has four chunks at least.
+  int64_t segments = (2 * num_cus() + wgs - 1) / wgs;
+  if (segments > n_chunks / 4) segments = n_chunks / 4;
+  if (segments < 1) segments = 1;
+  const int64_t per_segment = n_chunks ? (n_chunks + segments - 1) / segments : 1;
+  pl.seg_tokens = per_segment * kChunk;
+  pl.segments = (int)(n_chunks ? (n_chunks + per_segment - 1) / per_segment : 1);
+  Scratch states;
+  if (pl.segments > 1) {
+    AM_TRY(states.take((size_t)pl.groups * pl.segments * p.da * p.dc * sizeof(T)));
+    pl.states = (T*)states.p;
+    const int64_t ids = ((int64_t)pl.groups * (pl.segments - 1) + 7) / 8 * 8 * pl.slices;
+    hipLaunchKernelGGL((segment_sums<T, DA, BACK>), dim3((unsigned)ids), dim3(256), 0, stream(), p, pl);
+    AM_TRY(check_launch("segment_sums"));
+    hipLaunchKernelGGL((segment_states<T>), dim3((unsigned)(pl.groups * ((p.da * p.dc + 255) / 256))), dim3(256), 0, stream(), p, pl);
+    AM_TRY(check_launch("segment_states"));
+  }
+  const int64_t ids = ((int64_t)pl.groups * pl.segments + 7) / 8 * 8 * pl.slices;
+  hipLaunchKernelGGL((chunks<T, DA, BACK>), dim3((unsigned)ids), dim3(256), 0, stream(), p, pl);
+  return check_launch("chunks");
 }
 
 template <typename T, bool BACK>
 static int run_role(const Role<T>& p) {
-  const int64_t heads = p.heads / p.out_group;
-  const dim3 grid((unsigned)((p.dc + 15) / 16), (unsigned)heads, (unsigned)p.batch), block(64);
-  if (p.da <= 64) hipLaunchKernelGGL((walk<T, 16, BACK>), grid, block, 0, stream(), p);
-  else if (p.da <= 128) hipLaunchKernelGGL((walk<T, 32, BACK>), grid, block, 0, stream(), p);
-  else hipLaunchKernelGGL((walk<T, 64, BACK>), grid, block, 0, stream(), p);
-  return check_launch("walk");
+  if (p.da <= 32) return run_chunks<T, 32, BACK>(p);
+  if (p.da <= 64) return run_chunks<T, 64, BACK>(p);
+  if (p.da <= 96) return run_chunks<T, 96, BACK>(p);
+  if (p.da <= 128) return run_chunks<T, 128, BACK>(p);
+  if (p.da <= 192) return run_chunks<T, 192, BACK>(p);
+  return run_chunks<T, 256, BACK>(p);
 }
 
 // One token: the state is read and written once. A workgroup takes one head's state in rows of 16-byte vectors: `lanes`
@@ -166,7 +540,7 @@ static int check_sizes(const char* fn, int64_t batch, int64_t tokens, int64_t he
   if (dk < 1 || dv < 1 || dk > kMostDim || dv > kMostDim)
     return fail(AM_E_SHAPE, "%s: heads of %lld and %lld elements (1 .. %lld are supported)", fn, (long long)dk, (long long)dv, (long long)kMostDim);
   if (heads && (kv_heads < 1 || heads % kv_heads)) return fail(AM_E_SHAPE, "%s: %lld heads cannot share %lld key / value heads evenly", fn, (long long)heads, (long long)kv_heads);
-  if (heads > 65535 || batch > 65535) return fail(AM_E_SHAPE, "%s: more than 65535 heads or batch entries", fn);
+  if (heads && batch > ((int64_t)1 << 20) / heads) return fail(AM_E_SHAPE, "%s: more than 2^20 heads of all sequences together", fn);
   return AM_OK;
 }
 
@@ -235,17 +609,19 @@ static int backward(const char* fn, int64_t batch, int64_t tokens, int64_t heads
   for (int m = 0; m < group; ++m) {
     p.out_member = m;
     p.add = m > 0;
-    p.a = K; p.b = Q; p.c = G;
-    p.out = dval.p; p.o_b = dval.b; p.o_t = dval.t; p.o_h = dval.h;
-    p.s0 = gs; p.s0_b = gs_b; p.s0_h = gs_h; p.s0_r = dv; p.s0_c = 1;
-    p.s1 = gs0; p.s1_b = gs0_b; p.s1_h = gs0_h; p.s1_r = dv; p.s1_c = 1;
-    p.da = (int)dk; p.dc = (int)dv;
-    AM_TRY((run_role<T, true>(p)));
+    // dk first: dv's walk writes the first state's gradient, which may lie over the last state's
+    p.s0 = gs; p.s0_b = gs_b; p.s0_h = gs_h;
     p.a = W; p.b = G; p.c = Q;
     p.out = dkey.p; p.o_b = dkey.b; p.o_t = dkey.t; p.o_h = dkey.h;
     p.s0_r = 1; p.s0_c = dv;
     p.s1 = nullptr;
     p.da = (int)dv; p.dc = (int)dk;
+    AM_TRY((run_role<T, true>(p)));
+    p.a = K; p.b = Q; p.c = G;
+    p.out = dval.p; p.o_b = dval.b; p.o_t = dval.t; p.o_h = dval.h;
+    p.s0_r = dv; p.s0_c = 1;
+    p.s1 = gs0; p.s1_b = gs0_b; p.s1_h = gs0_h; p.s1_r = dv; p.s1_c = 1;
+    p.da = (int)dk; p.dc = (int)dv;
     AM_TRY((run_role<T, true>(p)));
   }
   return AM_OK;
