@@ -28,11 +28,9 @@ template <typename T> struct Operand { const T* p; int64_t b, t, h; int group; }
 template <typename T> struct Role {
   Operand<T> a, b, c;
   T* out; int64_t o_b, o_t, o_h;
-  int out_group, out_member;         // > 1: only heads h with h % group == member run, and out has heads / group of them
-  bool add;                          // out is added to
   const T* s0; int64_t s0_b, s0_h, s0_r, s0_c;     // first state [da, dc], null: zeros
   T* s1; int64_t s1_b, s1_h, s1_r, s1_c;           // last state, null: not wanted
-  T scale_a, scale_b;
+  T scale_a, scale_b;                // of the queries, of the keys
   int da, dc;
   const T* log_decay;
   const int64_t* lengths;
@@ -76,48 +74,93 @@ template <> struct Mma<double> {
 //
 // Where the heads alone do not fill the device, the tokens are cut into segments: `segment_sums` adds up each segment's
 // share of the state, `segment_states` carries them from segment to segment, and `chunks` starts every segment from its own.
+constexpr int64_t kMostDim = 256;
 constexpr int kChunk = 32;
 constexpr int kCols = 64;      // columns of a workgroup
+constexpr int kLds = 160 * 1024;
 
 template <typename T> struct Plan {
-  T* states;                   // [batch * heads / out_group][segments][da][dc]: the state in front of each segment; null: one segment
+  T* states;                   // [batch * heads][slots][da][dc]: the state in front of each part; null: one segment
   int segments, slices;
-  int64_t seg_tokens;          // a multiple of kChunk
-  int groups;                  // batch * heads / out_group
-  bool whole_a, whole_b;       // rows of a, b are whole 16-byte vectors
+  int parts, slots;            // parts of a segment; slots = parts * (segments - 1) + 1, one in front of every part but the last segment's later ones
+  int64_t seg_tokens, part_tokens;   // multiples of kChunk, seg_tokens = parts * part_tokens
+  int groups;                  // batch * heads
 };
 
-// Rows of `n` tokens (one after the other from local token i0 on) of an operand, as 16-byte vectors in registers.
-template <typename T, int DA> struct Tile {
+// The n <= 32 tokens of a chunk as a buffer: the hardware adds a lane's 32-bit offset to a uniform base, and what lies outside
+// the buffer reads as 0 and is not written, so a short chunk needs neither branches nor clamped addresses. Token `row` lies
+// `row * step` elements behind the chunk's first one; with a negative step the base is the last token's address, and tokens
+// behind the last get offsets that wrap around, out of the buffer. Needs 32 steps to lie within 2^31 bytes.
+struct Chunk { __amdgpu_buffer_rsrc_t rsrc; uint32_t first; };    // first: offset of the chunk's first token
+template <typename T> __device__ __forceinline__ Chunk chunk_of(const T* p, int64_t step, int n, int width) {
+  const T* base = step < 0 ? p + (n - 1) * step : p;
+  const int reach = (n - 1) * (int)(step < 0 ? -step : step);
+  Chunk c;
+  c.rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (reach + width) * (int)sizeof(T), 0x00020000);
+  c.first = step < 0 ? (uint32_t)(reach * (int)sizeof(T)) : 0u;
+  return c;
+}
+__device__ __forceinline__ void get(const Chunk& c, uint32_t off, float& v) { v = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(c.rsrc, (int)off, 0, 0)); }
+__device__ __forceinline__ void get(const Chunk& c, uint32_t off, double& v) { v = __builtin_bit_cast(double, __builtin_amdgcn_raw_buffer_load_b64(c.rsrc, (int)off, 0, 0)); }
+__device__ __forceinline__ void put(const Chunk& c, uint32_t off, float v) { __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), c.rsrc, (int)off, 0, 0); }
+__device__ __forceinline__ void put(const Chunk& c, uint32_t off, double v) {
+  typedef unsigned u2 __attribute__((ext_vector_type(2)));
+  __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u2, v), c.rsrc, (int)off, 0, 0);
+}
+
+// The rows of up to 32 tokens of an operand, as 16-byte vectors in registers on their way to LDS. Every lane always loads (a
+// load under a branch would have to be waited for before the next one). FAST: rows are whole vectors and the chunks buffers;
+// else element by element from clamped addresses. What lies outside becomes 0 on the way into LDS.
+template <typename T, int DA, bool FAST> struct Tile {
   static constexpr int V = 16 / (int)sizeof(T), PER_ROW = DA / V, NV = kChunk * PER_ROW / 256;
+  static constexpr bool EVEN = 256 % PER_ROW == 0;       // vector u of a lane lies whole rows behind its first
+  static constexpr int NO = EVEN ? 1 : NV;
   typedef T vec_t __attribute__((ext_vector_type(V)));
-  typedef T loose_t __attribute__((ext_vector_type(V), aligned(sizeof(T))));
   static constexpr int PITCH = DA + V;
   vec_t v[NV];
+  uint32_t off[NO];                                      // of a lane's vectors behind the chunk's first token
 
-  // p: the first token's row; step: to the next token
-  __device__ __forceinline__ void load(const T* p, int64_t step, int n, int da, bool whole) {
+  __device__ __forceinline__ void prepare(int64_t step, int da) {
+    if constexpr (FAST) {
 #pragma unroll
-    for (int u = 0; u < NV; ++u) {
-      const int f = (int)threadIdx.x + u * 256, row = f / PER_ROW, c = (f - row * PER_ROW) * V;
-      v[u] = (vec_t)((T)0);
-      if (row < n) {
-        const T* q = p + row * step + c;
-        if (whole) {
-          if (c < da) v[u] = *(const loose_t*)q;
-        } else {
-#pragma unroll
-          for (int e = 0; e < V; ++e)
-            if (c + e < da) v[u][e] = q[e];
-        }
+      for (int u = 0; u < NO; ++u) {
+        const int f = (int)threadIdx.x + u * 256, row = f / PER_ROW, c = (f - row * PER_ROW) * V;
+        off[u] = (uint32_t)((row * (int)step + c) * (int)sizeof(T));
       }
     }
   }
-  __device__ __forceinline__ void store(T* lds, T scale) const {
+  // p: the first token's row; step: to the next token; n >= 1 tokens
+  __device__ __forceinline__ void load(const T* p, int64_t step, int n, int da) {
+    if constexpr (FAST) {
+      const Chunk k = chunk_of(p, step, n, da);
+#pragma unroll
+      for (int u = 0; u < NV; ++u) {
+        const uint32_t o = EVEN ? off[0] + (k.first + (uint32_t)(u * (256 / PER_ROW) * (int)step * (int)sizeof(T))) : off[u % NO] + k.first;
+        v[u] = __builtin_bit_cast(vec_t, __builtin_amdgcn_raw_buffer_load_b128(k.rsrc, (int)o, 0, 0));
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < NV; ++u) {
+        const int f = (int)threadIdx.x + u * 256;
+        int row = f / PER_ROW, c = (f - row * PER_ROW) * V;
+        row = row < n ? row : n - 1;
+        const T* q = p + row * step;
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[u][e] = q[c + e < da ? c + e : da - 1];
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* lds, int n, int da) const {
+    const bool all = n == kChunk && da == DA;
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
       const int f = (int)threadIdx.x + u * 256, row = f / PER_ROW, c = (f - row * PER_ROW) * V;
-      *(vec_t*)(lds + row * PITCH + c) = v[u] * scale;
+      vec_t w = v[u];
+      if (!all) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) w[e] = (row < n && c + (FAST ? 0 : e) < da) ? w[e] : (T)0;
+      }
+      *(vec_t*)(lds + row * PITCH + c) = w;
     }
   }
 };
@@ -133,6 +176,10 @@ template <typename T> __device__ __forceinline__ void four(const T* lds, T (&out
     for (int e = 0; e < V; ++e) out[i + e] = w[e];
   }
 }
+
+// Nothing moves across here: the LDS reads of the next step stay in front of the matrix instructions of this one. Left alone,
+// the scheduler puts every read right in front of its use, and the wavefront waits for LDS in every step.
+__device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0); }
 
 // What a workgroup works on. The slices of one (head, segment) read the same a and b: they get ids that are equal modulo
 // the eight dies, whose L2 they share.
@@ -157,7 +204,7 @@ template <typename T> __device__ __forceinline__ int64_t length_of(const Role<T>
 // One wavefront's share of a chunk's sum over the tokens: S <- e^{g N} S + b^T (w c), c given weighted.
 template <typename T, int DA>
 __device__ __forceinline__ void add_tokens(typename Mma<T>::acc_t (&S)[DA / 16], const T* sB, const T (&wc)[2][4], T lam, int pr, int g) {
-  constexpr int PITCH = Tile<T, DA>::PITCH;
+  constexpr int PITCH = DA + 16 / (int)sizeof(T);
 #pragma unroll
   for (int kt = 0; kt < DA / 16; ++kt) {
     S[kt] *= lam;
@@ -169,44 +216,70 @@ __device__ __forceinline__ void add_tokens(typename Mma<T>::acc_t (&S)[DA / 16],
   }
 }
 
-// c of a chunk, in the layout of a right operand: register r of tile jt is token 16 jt + 4 g + r.
+// c of a chunk of n >= 1 tokens, in the layout of a right operand: register r of tile jt is token 16 jt + 4 g + r, in column
+// `col`. `take` makes tokens behind the n-th 0.
+template <typename T, bool FAST>
+__device__ __forceinline__ void load_c(T (&c)[2][4], const T* p, int64_t step, int n, int g, int col, int width) {
+  if constexpr (FAST) {
+    const Chunk k = chunk_of(p, step, n, width);
+    const uint32_t off = (uint32_t)((4 * g * (int)step + col) * (int)sizeof(T));
+#pragma unroll
+    for (int jt = 0; jt < 2; ++jt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) get(k, off + (k.first + (uint32_t)((16 * jt + r) * (int)step * (int)sizeof(T))), c[jt][r]);
+  } else {
+#pragma unroll
+    for (int jt = 0; jt < 2; ++jt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int j = 16 * jt + 4 * g + r;
+        c[jt][r] = p[(j < n ? j : n - 1) * step + col];
+      }
+  }
+}
 template <typename T>
-__device__ __forceinline__ void load_c(T (&c)[2][4], const T* p, int64_t step, int n, int g, bool live) {
+__device__ __forceinline__ void take(T (&c)[2][4], const T (&from)[2][4], int n, int g) {
+  if (n == kChunk) {
+#pragma unroll
+    for (int jt = 0; jt < 2; ++jt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) c[jt][r] = from[jt][r];
+    return;
+  }
 #pragma unroll
   for (int jt = 0; jt < 2; ++jt)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int j = 16 * jt + 4 * g + r;
-      c[jt][r] = (live && j < n) ? p[j * step] : (T)0;
-    }
+    for (int r = 0; r < 4; ++r) c[jt][r] = 16 * jt + 4 * g + r < n ? from[jt][r] : (T)0;
 }
 
-// e^{g (n - after - j)} of this lane's tokens
+// scale * e^{g (n - after - j)} of this lane's tokens
 template <typename T>
-__device__ __forceinline__ void weights(T (&w)[2][4], T ld, int n, int after, int g) {
+__device__ __forceinline__ void weights(T (&w)[2][4], T scale, T ld, int n, int after, int g) {
 #pragma unroll
   for (int jt = 0; jt < 2; ++jt)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int e = n - after - (16 * jt + 4 * g + r);
-      w[jt][r] = power(ld, (int64_t)(e > 0 ? e : 0));
+      w[jt][r] = scale * power(ld, (int64_t)(e > 0 ? e : 0));
     }
 }
 
-template <typename T, int DA, bool BACK>
-__global__ __launch_bounds__(256) void chunks(Role<T> p, Plan<T> pl) {
+#ifndef WPE
+#define WPE 2
+#endif
+template <typename T, int DA, bool BACK, bool FAST>
+__global__ __launch_bounds__(256, sizeof(T) == 4 ? WPE : 1) void chunks(Role<T> p, Plan<T> pl) {
   typedef typename Mma<T>::acc_t acc_t;
-  typedef Tile<T, DA> tile_t;
+  typedef Tile<T, DA, FAST> tile_t;
   constexpr int KT = DA / 16, V = tile_t::V, PITCH = tile_t::PITCH, APITCH = kChunk + V;
   constexpr int after = BACK ? 0 : 1;
-  __shared__ __attribute__((aligned(16))) T sQ[kChunk * PITCH];
-  __shared__ __attribute__((aligned(16))) T sB[kChunk * PITCH];
+  constexpr int BUFS = (4 * kChunk * PITCH + kChunk * APITCH) * (int)sizeof(T) <= kLds ? 2 : 1;
+  __shared__ __attribute__((aligned(16))) T bufs[BUFS][2][kChunk * PITCH];
   __shared__ __attribute__((aligned(16))) T sA[kChunk * APITCH];
   const Work w = work_of(pl, pl.segments);
   if (!w.live) return;
-  const int heads = (int)(p.heads / p.out_group);
-  const int64_t b = w.group / heads;
-  const int oh = (int)(w.group - b * heads), h = oh * p.out_group + p.out_member;
+  const int64_t b = w.group / (int)p.heads;
+  const int h = (int)(w.group - b * p.heads);
   const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63, g = lane >> 4, lr = lane & 15, pr = Mma<T>::row(lr);
   const int col = w.slice * kCols + wave * 16 + lr;
   const bool live = col < p.dc;
@@ -219,12 +292,13 @@ __global__ __launch_bounds__(256) void chunks(Role<T> p, Plan<T> pl) {
   const int64_t first = BACK ? n - 1 - lo : lo, dir = BACK ? -1 : 1;
   const T* pa = p.a.p + b * p.a.b + (h / p.a.group) * p.a.h + first * p.a.t;
   const T* pb = p.b.p + b * p.b.b + (h / p.b.group) * p.b.h + first * p.b.t;
-  const T* pc = p.c.p + b * p.c.b + (h / p.c.group) * p.c.h + first * p.c.t + col;
-  T* po = p.out + b * p.o_b + oh * p.o_h + col;
+  const T* pc = p.c.p + b * p.c.b + (h / p.c.group) * p.c.h + first * p.c.t;
+  const int ccol = live ? col : p.dc - 1;
+  T* po = p.out + b * p.o_b + h * p.o_h;
   const int64_t ta = dir * p.a.t, tb = dir * p.b.t, tc = dir * p.c.t;
 
   acc_t S[KT];
-  const T* s0 = pl.states ? pl.states + ((int64_t)w.group * pl.segments + w.segment) * p.da * p.dc : (p.s0 ? p.s0 + b * p.s0_b + h * p.s0_h : nullptr);
+  const T* s0 = pl.states ? pl.states + ((int64_t)w.group * pl.slots + w.segment * pl.parts) * p.da * p.dc : (p.s0 ? p.s0 + b * p.s0_b + h * p.s0_h : nullptr);
   const int64_t s0_r = pl.states ? p.dc : p.s0_r, s0_c = pl.states ? 1 : p.s0_c;
 #pragma unroll
   for (int kt = 0; kt < KT; ++kt)
@@ -239,48 +313,59 @@ __global__ __launch_bounds__(256) void chunks(Role<T> p, Plan<T> pl) {
   for (int it = 0; it < 2; ++it)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      reach[it][r] = power(ld, (int64_t)(16 * it + 4 * g + r + after));
+      reach[it][r] = p.scale_a * power(ld, (int64_t)(16 * it + 4 * g + r + after));
       const int apart = 16 * it + lr - 4 * g - r;          // i - j of tile distance `it`, transposed
-      mask[it][r] = apart >= 0 ? power(ld, (int64_t)apart) : (T)0;
+      mask[it][r] = apart >= 0 ? p.scale_a * p.scale_b * power(ld, (int64_t)apart) : (T)0;
     }
-  weights(wt, ld, kChunk, after, g);
+  weights(wt, p.scale_b, ld, kChunk, after, g);
   T lam = power(ld, (int64_t)kChunk);
 
   tile_t a, k;
   T c[2][4], cn[2][4];
+  a.prepare(ta, p.da);
+  k.prepare(tb, p.da);
+  const int64_t to = dir * p.o_t;
   const int64_t total = end - lo;
-  {
-    const int m = total < kChunk ? (int)(total < 0 ? 0 : total) : kChunk;
-    a.load(pa, ta, m, p.da, pl.whole_a);
-    k.load(pb, tb, m, p.da, pl.whole_b);
-    load_c(cn, pc, tc, m, g, live);
+  if (total > 0) {
+    const int m = total < kChunk ? (int)total : kChunk;
+    a.load(pa, ta, m, p.da);
+    k.load(pb, tb, m, p.da);
+    load_c<T, FAST>(cn, pc, tc, m, g, ccol, p.dc);
+    a.store(bufs[0][0], m, p.da);
+    k.store(bufs[0][1], m, p.da);
   }
+  int turn = 0;
   for (int64_t at = 0; at < total; at += kChunk) {
+    const int64_t next = at + kChunk;
     const int m = total - at < kChunk ? (int)(total - at) : kChunk;
-    a.store(sQ, p.scale_a);
-    k.store(sB, p.scale_b);
-#pragma unroll
-    for (int jt = 0; jt < 2; ++jt)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) c[jt][r] = cn[jt][r];
+    const int mn = total - next < kChunk ? (int)(total - next) : kChunk;
+    const T* sQ = bufs[turn][0];
+    const T* sB = bufs[turn][1];
+    take(c, cn, m, g);
     __syncthreads();
-    if (at + kChunk < total) {
-      const int64_t next = at + kChunk;
-      const int mn = total - next < kChunk ? (int)(total - next) : kChunk;
-      a.load(pa + next * ta, ta, mn, p.da, pl.whole_a);
-      k.load(pb + next * tb, tb, mn, p.da, pl.whole_b);
-      load_c(cn, pc + next * tc, tc, mn, g, live);
+    if (next < total) {
+      a.load(pa + next * ta, ta, mn, p.da);
+      k.load(pb + next * tb, tb, mn, p.da);
+      load_c<T, FAST>(cn, pc + next * tc, tc, mn, g, ccol, p.dc);
     }
     if (wave < 3) {                                         // tiles (0, 0), (1, 0), (1, 1) of A
       const int it = wave ? 1 : 0, jt = wave == 2 ? 1 : 0;
       acc_t t = (acc_t)((T)0);
+      const T* px = sB + (16 * jt + pr) * PITCH + 4 * g;
+      const T* py = sQ + (16 * it + lr) * PITCH + 4 * g;
+      T x[2][4], y[2][4];
+      four(px, x[0]);
+      four(py, y[0]);
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
-        T x[4], y[4];
-        four(sB + (16 * jt + pr) * PITCH + 16 * kt + 4 * g, x);
-        four(sQ + (16 * it + lr) * PITCH + 16 * kt + 4 * g, y);
+        if (kt + 1 < KT) {
+          four(px + 16 * (kt + 1), x[(kt + 1) & 1]);
+          four(py + 16 * (kt + 1), y[(kt + 1) & 1]);
+        }
+        pin();
 #pragma unroll
-        for (int r = 0; r < 4; ++r) t = Mma<T>::mma(x[r], y[r], t);
+        for (int r = 0; r < 4; ++r) t = Mma<T>::mma(x[kt & 1][r], y[kt & 1][r], t);
+        pin();
       }
       T* q = sA + (16 * it + lr) * APITCH + 16 * jt + 4 * g;
 #pragma unroll
@@ -290,49 +375,82 @@ __global__ __launch_bounds__(256) void chunks(Role<T> p, Plan<T> pl) {
       }
     }
     acc_t o[2];
-#pragma unroll
-    for (int it = 0; it < 2; ++it) {
-      o[it] = (acc_t)((T)0);
+    {
+      const T* px = sQ + pr * PITCH + 4 * g;
+      T x[2][2][4];
+      o[0] = o[1] = (acc_t)((T)0);
+      four(px, x[0][0]);
+      four(px + 16 * PITCH, x[0][1]);
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
-        T x[4];
-        four(sQ + (16 * it + pr) * PITCH + 16 * kt + 4 * g, x);
+        if (kt + 1 < KT) {
+          four(px + 16 * (kt + 1), x[(kt + 1) & 1][0]);
+          four(px + 16 * PITCH + 16 * (kt + 1), x[(kt + 1) & 1][1]);
+        }
+        pin();
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[it] = Mma<T>::mma(x[r], S[kt][r], o[it]);
+        for (int r = 0; r < 4; ++r) {
+          o[0] = Mma<T>::mma(x[kt & 1][0][r], S[kt][r], o[0]);
+          o[1] = Mma<T>::mma(x[kt & 1][1][r], S[kt][r], o[1]);
+        }
+        pin();
       }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) o[it][r] *= reach[it][r];
     }
-    __syncthreads();
 #pragma unroll
     for (int it = 0; it < 2; ++it)
 #pragma unroll
-      for (int jt = 0; jt <= it; ++jt) {
-        T x[4];
-        four(sA + (16 * it + pr) * APITCH + 16 * jt + 4 * g, x);
+      for (int r = 0; r < 4; ++r) o[it][r] *= reach[it][r];
+    __syncthreads();
+    {
+      const T* px = sA + pr * APITCH + 4 * g;
+      T x[3][4];
+      four(px, x[0]);
+      four(px + 16 * APITCH, x[1]);
+      four(px + 16 * APITCH + 16, x[2]);
+      pin();
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[it] = Mma<T>::mma(x[r], c[jt][r], o[it]);
+      for (int r = 0; r < 4; ++r) {
+        o[0] = Mma<T>::mma(x[0][r], c[0][r], o[0]);
+        o[1] = Mma<T>::mma(x[1][r], c[0][r], o[1]);
       }
-    if (m < kChunk) { weights(wt, ld, m, after, g); lam = power(ld, (int64_t)m); }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[1] = Mma<T>::mma(x[2][r], c[1][r], o[1]);
+    }
+    if (m < kChunk) { weights(wt, p.scale_b, ld, m, after, g); lam = power(ld, (int64_t)m); }
 #pragma unroll
     for (int jt = 0; jt < 2; ++jt)
 #pragma unroll
       for (int r = 0; r < 4; ++r) c[jt][r] *= wt[jt][r];
     add_tokens<T, DA>(S, sB, c, lam, pr, g);
+    if (live) {
+      T* q = po + (first + dir * at) * p.o_t;
+      if constexpr (FAST) {
+        const Chunk k = chunk_of(q, to, m, p.dc);
+        const uint32_t off = (uint32_t)((4 * g * (int)to + col) * (int)sizeof(T));
 #pragma unroll
-    for (int it = 0; it < 2; ++it)
+        for (int it = 0; it < 2; ++it)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = 16 * it + 4 * g + r;
-        if (live && i < m) {
-          T* q = po + (first + dir * (at + i)) * p.o_t;
-          *q = p.add ? *q + o[it][r] : o[it][r];
-        }
+          for (int r = 0; r < 4; ++r) put(k, off + (k.first + (uint32_t)((16 * it + r) * (int)to * (int)sizeof(T))), o[it][r]);
+      } else {
+#pragma unroll
+        for (int it = 0; it < 2; ++it)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int i = 16 * it + 4 * g + r;
+            if (i < m) q[i * to + col] = o[it][r];
+          }
       }
-    __syncthreads();
+    }
+    // the next chunk into LDS: into the other buffer, or (where two do not fit) behind a barrier
+    if constexpr (BUFS == 2) turn ^= 1;
+    else __syncthreads();
+    if (next < total) {
+      a.store(bufs[turn][0], mn, p.da);
+      k.store(bufs[turn][1], mn, p.da);
+    }
   }
-  if (live && !p.add) {                                     // behind the sequence
-    for (int64_t t = (lo > n ? lo : n) + g; t < hi; t += 4) po[t * p.o_t] = (T)0;
+  if (live) {                                               // behind the sequence
+    for (int64_t t = (lo > n ? lo : n) + g; t < hi; t += 4) po[t * p.o_t + col] = (T)0;
   }
   if (p.s1 && w.segment == pl.segments - 1 && live) {
     T* s1 = p.s1 + b * p.s1_b + h * p.s1_h + col * p.s1_c;
@@ -346,64 +464,66 @@ __global__ __launch_bounds__(256) void chunks(Role<T> p, Plan<T> pl) {
   }
 }
 
-// The share of segment s (all but the last) in the state behind it, into the states' slot s + 1.
-template <typename T, int DA, bool BACK>
+// The share of a part (of all segments but the last) in the state behind it, into the slot behind the part's own.
+template <typename T, int DA, bool BACK, bool FAST>
 __global__ __launch_bounds__(256) void segment_sums(Role<T> p, Plan<T> pl) {
   typedef typename Mma<T>::acc_t acc_t;
-  typedef Tile<T, DA> tile_t;
+  typedef Tile<T, DA, FAST> tile_t;
   constexpr int KT = DA / 16, PITCH = tile_t::PITCH;
   constexpr int after = BACK ? 0 : 1;
   __shared__ __attribute__((aligned(16))) T sB[2][kChunk * PITCH];
-  const Work w = work_of(pl, pl.segments - 1);
+  const Work w = work_of(pl, pl.slots - 1);
   if (!w.live) return;
-  const int heads = (int)(p.heads / p.out_group);
-  const int64_t b = w.group / heads;
-  const int h = (int)(w.group - b * heads) * p.out_group + p.out_member;
+  const int64_t b = w.group / (int)p.heads;
+  const int h = (int)(w.group - b * p.heads);
   const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63, g = lane >> 4, lr = lane & 15, pr = Mma<T>::row(lr);
   const int col = w.slice * kCols + wave * 16 + lr;
   const bool live = col < p.dc;
   const int64_t n = length_of(p, b);
-  const int64_t lo = w.segment * pl.seg_tokens;
-  const int64_t end = lo + pl.seg_tokens < n ? lo + pl.seg_tokens : n;
+  const int64_t lo = w.segment * pl.part_tokens;
+  const int64_t end = lo + pl.part_tokens < n ? lo + pl.part_tokens : n;
   const int64_t first = BACK ? n - 1 - lo : lo, dir = BACK ? -1 : 1;
   const T* pb = p.b.p + b * p.b.b + (h / p.b.group) * p.b.h + first * p.b.t;
-  const T* pc = p.c.p + b * p.c.b + (h / p.c.group) * p.c.h + first * p.c.t + col;
+  const T* pc = p.c.p + b * p.c.b + (h / p.c.group) * p.c.h + first * p.c.t;
+  const int ccol = live ? col : p.dc - 1;
   const int64_t tb = dir * p.b.t, tc = dir * p.c.t;
   acc_t S[KT];
 #pragma unroll
   for (int kt = 0; kt < KT; ++kt) S[kt] = (acc_t)((T)0);
   const T ld = p.log_decay[h];
   T wt[2][4];
-  weights(wt, ld, kChunk, after, g);
+  weights(wt, p.scale_b, ld, kChunk, after, g);
   T lam = power(ld, (int64_t)kChunk);
   tile_t k;
   T c[2][4], cn[2][4];
+  k.prepare(tb, p.da);
   const int64_t total = end - lo;
-  {
-    const int m = total < kChunk ? (int)(total < 0 ? 0 : total) : kChunk;
-    k.load(pb, tb, m, p.da, pl.whole_b);
-    load_c(cn, pc, tc, m, g, live);
+  if (total > 0) {
+    const int m = total < kChunk ? (int)total : kChunk;
+    k.load(pb, tb, m, p.da);
+    load_c<T, FAST>(cn, pc, tc, m, g, ccol, p.dc);
   }
   int turn = 0;
   for (int64_t at = 0; at < total; at += kChunk, turn ^= 1) {
     const int m = total - at < kChunk ? (int)(total - at) : kChunk;
-    k.store(sB[turn], p.scale_b);                           // (two buffers: one barrier a chunk)
-    if (m < kChunk) { weights(wt, ld, m, after, g); lam = power(ld, (int64_t)m); }
+    k.store(sB[turn], m, p.da);                             // (two buffers: one barrier a chunk)
+    if (m < kChunk) { weights(wt, p.scale_b, ld, m, after, g); lam = power(ld, (int64_t)m); }
+    take(c, cn, m, g);
 #pragma unroll
     for (int jt = 0; jt < 2; ++jt)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) c[jt][r] = cn[jt][r] * wt[jt][r];
+      for (int r = 0; r < 4; ++r) c[jt][r] *= wt[jt][r];
     __syncthreads();
     if (at + kChunk < total) {
       const int64_t next = at + kChunk;
       const int mn = total - next < kChunk ? (int)(total - next) : kChunk;
-      k.load(pb + next * tb, tb, mn, p.da, pl.whole_b);
-      load_c(cn, pc + next * tc, tc, mn, g, live);
+      k.load(pb + next * tb, tb, mn, p.da);
+      load_c<T, FAST>(cn, pc + next * tc, tc, mn, g, ccol, p.dc);
     }
     add_tokens<T, DA>(S, sB[turn], c, lam, pr, g);
   }
   if (!live) return;
-  T* s1 = pl.states + ((int64_t)w.group * pl.segments + w.segment + 1) * p.da * p.dc + col;
+  T* s1 = pl.states + ((int64_t)w.group * pl.slots + w.segment + 1) * p.da * p.dc + col;
 #pragma unroll
   for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -413,7 +533,24 @@ __global__ __launch_bounds__(256) void segment_sums(Role<T> p, Plan<T> pl) {
     }
 }
 
-// From the segments' shares to the state in front of each: one lane per element of a head's state.
+// From the parts' shares to the states in front of the segments (the slots at multiples of `parts`): one lane per element of
+// a head's state, BATCH slots on their way at a time (no load may pass the stores of the batch before).
+template <typename T, int BATCH>
+__device__ __forceinline__ void carry(T* at, int64_t per, int& k, T& s, T ld, int64_t n, const Plan<T>& pl) {
+  for (; k + BATCH <= pl.slots; k += BATCH) {
+    T v[BATCH];
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) v[u] = at[(int64_t)(k + u) * per];
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+      int64_t len = n - (k + u - 1) * pl.part_tokens;
+      len = len < 0 ? 0 : (len < pl.part_tokens ? len : pl.part_tokens);
+      s = s * power(ld, len) + v[u];
+      if ((k + u) % pl.parts == 0) at[(int64_t)(k + u) * per] = s;
+    }
+  }
+}
+
 template <typename T>
 __global__ __launch_bounds__(256) void segment_states(Role<T> p, Plan<T> pl) {
   const int per = p.da * p.dc;
@@ -421,64 +558,89 @@ __global__ __launch_bounds__(256) void segment_states(Role<T> p, Plan<T> pl) {
   const int group = (int)(blockIdx.x / (unsigned)blocks);
   const int i = (int)(blockIdx.x - (unsigned)group * (unsigned)blocks) * 256 + (int)threadIdx.x;
   if (i >= per) return;
-  const int heads = (int)(p.heads / p.out_group);
-  const int64_t b = group / heads;
-  const int h = (int)(group - b * heads) * p.out_group + p.out_member;
+  const int64_t b = group / (int)p.heads;
+  const int h = (int)(group - b * p.heads);
   const int64_t n = length_of(p, b);
   const T ld = p.log_decay[h];
   const int r = i / p.dc, c = i - r * p.dc;
-  T* at = pl.states + (int64_t)group * pl.segments * per + i;
+  T* at = pl.states + (int64_t)group * pl.slots * per + i;
   T s = p.s0 ? p.s0[b * p.s0_b + h * p.s0_h + r * p.s0_r + c * p.s0_c] : (T)0;
   at[0] = s;
-#pragma unroll 4
-  for (int k = 1; k < pl.segments; ++k) {
-    int64_t len = n - (k - 1) * pl.seg_tokens;
-    len = len < 0 ? 0 : (len < pl.seg_tokens ? len : pl.seg_tokens);
-    s = s * power(ld, len) + at[(int64_t)k * per];
-    at[(int64_t)k * per] = s;
-  }
+  int k = 1;
+  carry<T, 32>(at, per, k, s, ld, n, pl);
+  carry<T, 8>(at, per, k, s, ld, n, pl);
+  carry<T, 2>(at, per, k, s, ld, n, pl);
+  carry<T, 1>(at, per, k, s, ld, n, pl);
 }
 
-template <typename T, int DA, bool BACK>
+static int workgroups_per_cu(const void* kernel) {
+  int n = 0;
+  if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, 256, 0) != hipSuccess || n < 1) { (void)hipGetLastError(); n = 1; }
+  return n;
+}
+
+#ifndef MINSEG
+#define MINSEG 2
+#endif
+template <typename T, int DA, bool BACK, bool FAST>
 static int run_chunks(const Role<T>& p) {
   Plan<T> pl = {};
   pl.slices = (p.dc + kCols - 1) / kCols;
-  pl.groups = (int)(p.batch * (p.heads / p.out_group));
+  pl.groups = (int)(p.batch * p.heads);
   pl.segments = 1;
-  constexpr int V = 16 / (int)sizeof(T);
-  pl.whole_a = pl.whole_b = p.da % V == 0;
   const int64_t wgs = (int64_t)pl.groups * pl.slices;
   const int64_t n_chunks = (p.tokens + kChunk - 1) / kChunk;
-  // Two workgroups for every CU; a segment has four chunks at least.
-  int64_t segments = (2 * num_cus() + wgs - 1) / wgs;
-  if (segments > n_chunks / 4) segments = n_chunks / 4;
+  // As many segments as the device has room for workgroups, of MINSEG chunks at least.
+  static const int room = workgroups_per_cu((const void*)chunks<T, DA, BACK, FAST>), sums_room = workgroups_per_cu((const void*)segment_sums<T, DA, BACK, FAST>);
+  int64_t segments = (int64_t)room * num_cus() / wgs;
+  if (segments > n_chunks / MINSEG) segments = n_chunks / MINSEG;
   if (segments < 1) segments = 1;
-  const int64_t per_segment = n_chunks ? (n_chunks + segments - 1) / segments : 1;
+  int64_t per_segment = n_chunks ? (n_chunks + segments - 1) / segments : 1;
+  int64_t parts = 1;
+  if (segments > 1) {
+    // the sums run in parts of a segment, so that they too fill the device
+    parts = (int64_t)sums_room * num_cus() / (wgs * (segments - 1));
+    if (parts > per_segment / 2) parts = per_segment / 2;
+    if (parts < 1) parts = 1;
+    per_segment = (per_segment + parts - 1) / parts * parts;
+  }
+  pl.parts = (int)parts;
+  pl.part_tokens = per_segment / parts * kChunk;
   pl.seg_tokens = per_segment * kChunk;
   pl.segments = (int)(n_chunks ? (n_chunks + per_segment - 1) / per_segment : 1);
+  pl.slots = pl.parts * (pl.segments - 1) + 1;
   Scratch states;
   if (pl.segments > 1) {
-    AM_TRY(states.take((size_t)pl.groups * pl.segments * p.da * p.dc * sizeof(T)));
+    AM_TRY(states.take((size_t)pl.groups * pl.slots * p.da * p.dc * sizeof(T)));
     pl.states = (T*)states.p;
-    const int64_t ids = ((int64_t)pl.groups * (pl.segments - 1) + 7) / 8 * 8 * pl.slices;
-    hipLaunchKernelGGL((segment_sums<T, DA, BACK>), dim3((unsigned)ids), dim3(256), 0, stream(), p, pl);
+    const int64_t ids = ((int64_t)pl.groups * (pl.slots - 1) + 7) / 8 * 8 * pl.slices;
+    hipLaunchKernelGGL((segment_sums<T, DA, BACK, FAST>), dim3((unsigned)ids), dim3(256), 0, stream(), p, pl);
     AM_TRY(check_launch("segment_sums"));
     hipLaunchKernelGGL((segment_states<T>), dim3((unsigned)(pl.groups * ((p.da * p.dc + 255) / 256))), dim3(256), 0, stream(), p, pl);
     AM_TRY(check_launch("segment_states"));
   }
   const int64_t ids = ((int64_t)pl.groups * pl.segments + 7) / 8 * 8 * pl.slices;
-  hipLaunchKernelGGL((chunks<T, DA, BACK>), dim3((unsigned)ids), dim3(256), 0, stream(), p, pl);
+  hipLaunchKernelGGL((chunks<T, DA, BACK, FAST>), dim3((unsigned)ids), dim3(256), 0, stream(), p, pl);
   return check_launch("chunks");
+}
+
+template <typename T, int DA, bool BACK>
+static int run_sized(const Role<T>& p) {
+  // FAST: rows of whole vectors, and 32 tokens of every operand within 2^31 bytes
+  const int64_t most = ((int64_t)1 << 31) / (kChunk * (int64_t)sizeof(T)) - kMostDim;
+  auto near = [&](int64_t t) { return t < most && -t < most; };
+  const bool fast = p.da % (16 / (int)sizeof(T)) == 0 && near(p.a.t) && near(p.b.t) && near(p.c.t) && near(p.o_t);
+  return fast ? run_chunks<T, DA, BACK, true>(p) : run_chunks<T, DA, BACK, false>(p);
 }
 
 template <typename T, bool BACK>
 static int run_role(const Role<T>& p) {
-  if (p.da <= 32) return run_chunks<T, 32, BACK>(p);
-  if (p.da <= 64) return run_chunks<T, 64, BACK>(p);
-  if (p.da <= 96) return run_chunks<T, 96, BACK>(p);
-  if (p.da <= 128) return run_chunks<T, 128, BACK>(p);
-  if (p.da <= 192) return run_chunks<T, 192, BACK>(p);
-  return run_chunks<T, 256, BACK>(p);
+  if (p.da <= 32) return run_sized<T, 32, BACK>(p);
+  if (p.da <= 64) return run_sized<T, 64, BACK>(p);
+  if (p.da <= 96) return run_sized<T, 96, BACK>(p);
+  if (p.da <= 128) return run_sized<T, 128, BACK>(p);
+  if (p.da <= 192) return run_sized<T, 192, BACK>(p);
+  return run_sized<T, 256, BACK>(p);
 }
 
 // One token: the state is read and written once. A workgroup takes one head's state in rows of 16-byte vectors: `lanes`
@@ -533,8 +695,6 @@ __global__ __launch_bounds__(256) void step(StepArgs<T> p, int lanes, int tiles)
   }
 }
 
-constexpr int64_t kMostDim = 256;
-
 static int check_sizes(const char* fn, int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dk, int64_t dv) {
   if (batch < 0 || tokens < 0 || heads < 0 || kv_heads < 0) return fail(AM_E_SHAPE, "%s: negative extent", fn);
   if (dk < 1 || dv < 1 || dk > kMostDim || dv > kMostDim)
@@ -566,7 +726,6 @@ static int forward(const char* fn, int64_t batch, int64_t tokens, int64_t heads,
   p.b = {k.p, k.b, k.t, k.h, group};
   p.c = {v.p, v.b, v.t, v.h, group};
   p.out = out.p; p.o_b = out.b; p.o_t = out.t; p.o_h = out.h;
-  p.out_group = 1;
   p.s0 = s0; p.s0_b = s0_b; p.s0_h = s0_h; p.s0_r = dv; p.s0_c = 1;
   p.s1 = s1; p.s1_b = s1_b; p.s1_h = s1_h; p.s1_r = dv; p.s1_c = 1;
   p.scale_a = scale; p.scale_b = (T)1;
@@ -574,6 +733,35 @@ static int forward(const char* fn, int64_t batch, int64_t tokens, int64_t heads,
   p.log_decay = log_decay; p.lengths = lengths;
   p.batch = batch; p.tokens = tokens; p.heads = heads;
   return run_role<T, false>(p);
+}
+
+// out[b, t, head, :] = the sum of the `group` heads' shares that follow each other, in the heads' order
+template <typename T, int V>
+__global__ __launch_bounds__(256) void fold(const T* shares, Result<T> out, int64_t rows, int tokens, int kv_heads, int group, int d) {
+  typedef T vec_t __attribute__((ext_vector_type(V)));
+  const int per = d / V;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = i / per;                             // (batch, token, head)
+  if (row >= rows) return;
+  const int c = (int)(i - row * per) * V;
+  const T* q = shares + row * group * d + c;
+  vec_t sum = *(const vec_t*)q;
+  for (int m = 1; m < group; ++m) sum += *(const vec_t*)(q + (int64_t)m * d);
+  const int64_t bt = row / kv_heads, b = bt / tokens;
+  *(vec_t*)(out.p + b * out.b + (bt - b * tokens) * out.t + (row - bt * kv_heads) * out.h + c) = sum;
+}
+
+template <typename T>
+static int fold_heads(const T* shares, const Result<T>& out, int64_t batch, int64_t tokens, int64_t kv_heads, int group, int d) {
+  constexpr int W = 16 / (int)sizeof(T);
+  const int64_t rows = batch * tokens * kv_heads;
+  if (rows == 0) return AM_OK;
+  const bool vec = d % W == 0 && (uintptr_t)out.p % 16 == 0 && out.b % W == 0 && out.t % W == 0 && out.h % W == 0;
+  const int64_t wgs = (rows * (vec ? d / W : d) + 255) / 256;
+  if (wgs >= ((int64_t)1 << 31) || tokens >= ((int64_t)1 << 31)) return fail(AM_E_SHAPE, "decay attention: too many tokens for shared heads");
+  if (vec) hipLaunchKernelGGL((fold<T, W>), dim3((unsigned)wgs), dim3(256), 0, stream(), shares, out, rows, (int)tokens, (int)kv_heads, group, d);
+  else hipLaunchKernelGGL((fold<T, 1>), dim3((unsigned)wgs), dim3(256), 0, stream(), shares, out, rows, (int)tokens, (int)kv_heads, group, d);
+  return check_launch("fold");
 }
 
 template <typename T>
@@ -597,33 +785,33 @@ static int backward(const char* fn, int64_t batch, int64_t tokens, int64_t heads
   // dq: forwards over (do, v, k) from the transposed first state
   p.a = G; p.b = W; p.c = K;
   p.out = dq.p; p.o_b = dq.b; p.o_t = dq.t; p.o_h = dq.h;
-  p.out_group = 1;
   p.s0 = s0; p.s0_b = s0_b; p.s0_h = s0_h; p.s0_r = 1; p.s0_c = dv;
   p.scale_a = scale; p.scale_b = (T)1;
   p.da = (int)dv; p.dc = (int)dk;
   AM_TRY((run_role<T, false>(p)));
-  // dv and dk: backwards; key / value heads that several heads share add up their shares one head after the other, in
-  // the heads' order
-  p.out_group = group;
+  // dk and dv: backwards. Where heads share a key / value head each writes its own share, and `fold_heads` adds them up.
+  // dk first: dv's walk writes the first state's gradient, which may lie over the last state's.
   p.scale_a = (T)1; p.scale_b = scale;
-  for (int m = 0; m < group; ++m) {
-    p.out_member = m;
-    p.add = m > 0;
-    // dk first: dv's walk writes the first state's gradient, which may lie over the last state's
-    p.s0 = gs; p.s0_b = gs_b; p.s0_h = gs_h;
-    p.a = W; p.b = G; p.c = Q;
-    p.out = dkey.p; p.o_b = dkey.b; p.o_t = dkey.t; p.o_h = dkey.h;
-    p.s0_r = 1; p.s0_c = dv;
-    p.s1 = nullptr;
-    p.da = (int)dv; p.dc = (int)dk;
-    AM_TRY((run_role<T, true>(p)));
-    p.a = K; p.b = Q; p.c = G;
-    p.out = dval.p; p.o_b = dval.b; p.o_t = dval.t; p.o_h = dval.h;
-    p.s0_r = dv; p.s0_c = 1;
-    p.s1 = gs0; p.s1_b = gs0_b; p.s1_h = gs0_h; p.s1_r = dv; p.s1_c = 1;
-    p.da = (int)dk; p.dc = (int)dv;
-    AM_TRY((run_role<T, true>(p)));
-  }
+  p.s0 = gs; p.s0_b = gs_b; p.s0_h = gs_h;
+  Scratch shares;
+  if (group > 1 && tokens) AM_TRY(shares.take((size_t)batch * tokens * heads * (dk > dv ? dk : dv) * sizeof(T)));
+  auto into = [&](const Result<T>& r, int64_t d) {
+    if (group == 1) { p.out = r.p; p.o_b = r.b; p.o_t = r.t; p.o_h = r.h; }
+    else { p.out = (T*)shares.p; p.o_b = tokens * heads * d; p.o_t = heads * d; p.o_h = d; }
+  };
+  p.a = W; p.b = G; p.c = Q;
+  into(dkey, dk);
+  p.s0_r = 1; p.s0_c = dv;
+  p.da = (int)dv; p.dc = (int)dk;
+  AM_TRY((run_role<T, true>(p)));
+  if (group > 1) AM_TRY(fold_heads((const T*)shares.p, dkey, batch, tokens, kv_heads, group, (int)dk));
+  p.a = K; p.b = Q; p.c = G;
+  into(dval, dv);
+  p.s0_r = dv; p.s0_c = 1;
+  p.s1 = gs0; p.s1_b = gs0_b; p.s1_h = gs0_h; p.s1_r = dv; p.s1_c = 1;
+  p.da = (int)dk; p.dc = (int)dv;
+  AM_TRY((run_role<T, true>(p)));
+  if (group > 1) AM_TRY(fold_heads((const T*)shares.p, dval, batch, tokens, kv_heads, group, (int)dv));
   return AM_OK;
 }
 

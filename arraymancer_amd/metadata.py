@@ -34,17 +34,16 @@ class Layout:
 
 
 def shape_to_strides(shape: Sequence[int], order: str = "C") -> Tuple[int, ...]:
-    strides = [0] * len(shape)
+    strides = []
     acc = 1
-    idx = range(len(shape) - 1, -1, -1) if order == "C" else range(len(shape))
-    for i in idx:
-        strides[i] = acc
-        acc *= shape[i]
-    return tuple(strides)
+    for s in (reversed(shape) if order == "C" else shape):
+        strides.append(acc)
+        acc *= s
+    return tuple(strides[::-1] if order == "C" else strides)
 
 
 def contiguous(shape: Sequence[int], order: str = "C") -> Layout:
-    shape = tuple(int(s) for s in shape)
+    shape = tuple(map(int, shape))
     if len(shape) > MAXRANK:
         raise ValueError(f"rank {len(shape)} exceeds the maximum rank {MAXRANK}")
     return Layout(shape, shape_to_strides(shape, order), 0)

@@ -31,17 +31,24 @@ _FLOAT64 = np.dtype(np.float64)
 ROTARY_SCALINGS = ("none", "linear", "base", "parts")
 
 
+_ENTRIES: dict = {}
+
+
 def _entry(name: str, t: HipTensor):
-    """The entry point of `t`'s element type and its scalar type."""
-    sfx = t.sfx
-    if t.dtype.kind != "f":
-        raise TypeError(f"{name} is defined for float tensors, not {t.dtype}")
-    return getattr(_lib.load(), f"am_hip_{name}_{sfx}"), _lib.CTYPE[sfx]
+    """The entry point of `t`'s element type."""
+    fn = _ENTRIES.get((name, t.dtype))
+    if fn is None:
+        sfx = t.sfx
+        if t.dtype.kind != "f":
+            raise TypeError(f"{name} is defined for float tensors, not {t.dtype}")
+        fn = _ENTRIES[name, t.dtype] = getattr(_lib.load(), f"am_hip_{name}_{sfx}")
+    return fn
 
 
 def _unit_rows(t: HipTensor) -> HipTensor:
     """`t`, or a copy of it, with unit stride in the last dimension."""
-    return t if t.strides[-1] == 1 or t.shape[-1] == 1 else t.clone()
+    lay = t.layout
+    return t if lay.strides[-1] == 1 or lay.shape[-1] == 1 else t.clone()
 
 
 def _shape(name: str, what: str, t: HipTensor, shape):
@@ -82,7 +89,7 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: str = "none
 
 
 def _rotate(name, out: HipTensor | None, x: HipTensor, positions: HipTensor | None, frequencies: HipTensor, layout: str, scale: float, inverse: int):
-    fn, ct = _entry("rotary", x)
+    fn = _entry("rotary", x)
     if x.rank != 4:
         raise ValueError(f"{name}: a tensor [batch, tokens, heads, dim] is needed, not one of rank {x.rank}")
     B, T, H, D = x.shape
@@ -113,7 +120,7 @@ def _rotate(name, out: HipTensor | None, x: HipTensor, positions: HipTensor | No
         out = empty(x.shape, x.dtype)
     src = x if x is out else _unit_rows(x)
     xs, os = src.strides, out.strides
-    check(fn(B, T, H, D, R, ROTARY[layout], inverse, ct(scale), pp, pb, pt, frequencies.data_ptr(), src.data_ptr(), xs[0], xs[1], xs[2],
+    check(fn(B, T, H, D, R, ROTARY[layout], inverse, scale, pp, pb, pt, frequencies.data_ptr(), src.data_ptr(), xs[0], xs[1], xs[2],
              out.data_ptr(), os[0], os[1], os[2]))
     return out
 
@@ -174,7 +181,7 @@ def _lengths(name, lengths: HipTensor | None, batch: int):
 
 
 def _rows(t: HipTensor):
-    return (t.data_ptr(),) + t.strides[:-1]
+    return (t.data_ptr(),) + t.layout.strides[:-1]
 
 
 def decay_attention(q: HipTensor, k: HipTensor, v: HipTensor, log_decay: HipTensor, state: HipTensor | None = None,
@@ -185,13 +192,13 @@ def decay_attention(q: HipTensor, k: HipTensor, v: HipTensor, log_decay: HipTens
     states [batch, heads, dk, dv]; head h reads key / value head h // (heads / kv_heads). lengths: int64 [batch], the tokens
     of each sequence; behind them out is 0. `state` is not changed."""
     name = "decay_attention"
-    fn, ct = _entry(name, q)
+    fn = _entry(name, q)
     (B, T), H, KH, dk, dv = _attention_sizes(name, q, k, v, log_decay, 2)
     s0 = _head_state(name, state, (B, H, dk, dv), q) if state is not None else (None, 0, 0)
     n = _lengths(name, lengths, B)
     q, k, v, g = _unit_rows(q), _unit_rows(k), _unit_rows(v), log_decay.asContiguous()
     out, end = empty((B, T, H, dv), q.dtype), empty((B, H, dk, dv), q.dtype)
-    check(fn(B, T, H, KH, dk, dv, ct(scale), g.data_ptr(), n, *_rows(q), *_rows(k), *_rows(v), *s0,
+    check(fn(B, T, H, KH, dk, dv, scale, g.data_ptr(), n, *_rows(q), *_rows(k), *_rows(v), *s0,
              *_rows(out), *_rows(end)[:3]))
     return out, end
 
@@ -203,7 +210,7 @@ def decay_attention_backward(gradOutput: HipTensor, q: HipTensor, k: HipTensor, 
     state it returned (None: zeros). dk and dv of a shared key / value head are sums over the heads that read it; dstate is
     None where no state went in. The decays are constants of the layer and get no gradient."""
     name = "decay_attention_backward"
-    fn, ct = _entry(name, q)
+    fn = _entry(name, q)
     (B, T), H, KH, dk, dv = _attention_sizes(name, q, k, v, log_decay, 2)
     _same_dtype(q, gradOutput)
     _shape(name, "the output's gradient", gradOutput, (B, T, H, dv))
@@ -213,7 +220,7 @@ def decay_attention_backward(gradOutput: HipTensor, q: HipTensor, k: HipTensor, 
     q, k, v, do, g = _unit_rows(q), _unit_rows(k), _unit_rows(v), _unit_rows(gradOutput), log_decay.asContiguous()
     dq, dkey, dval = empty((B, T, H, dk), q.dtype), empty((B, T, KH, dk), q.dtype), empty((B, T, KH, dv), q.dtype)
     dstate = empty((B, H, dk, dv), q.dtype) if state is not None else None
-    check(fn(B, T, H, KH, dk, dv, ct(scale), g.data_ptr(), n, *_rows(do), *_rows(q), *_rows(k), *_rows(v),
+    check(fn(B, T, H, KH, dk, dv, scale, g.data_ptr(), n, *_rows(do), *_rows(q), *_rows(k), *_rows(v),
              *s0, *gs, *_rows(dq), *_rows(dkey), *_rows(dval), *(_rows(dstate)[:3] if dstate is not None else (None, 0, 0))))
     return dq, dkey, dval, dstate
 
@@ -222,12 +229,12 @@ def decay_attention_step(q: HipTensor, k: HipTensor, v: HipTensor, log_decay: Hi
     """One new token of every sequence: `state` [batch, heads, dk, dv] is updated in place and the outputs [batch, heads, dv]
     are returned. q [batch, heads, dk], k [batch, kv_heads, dk], v [batch, kv_heads, dv]."""
     name = "decay_attention_step"
-    fn, ct = _entry(name, q)
+    fn = _entry(name, q)
     (B,), H, KH, dk, dv = _attention_sizes(name, q, k, v, log_decay, 1)
     s = _head_state(name, state, (B, H, dk, dv), q)
     q, k, v, g = _unit_rows(q), _unit_rows(k), _unit_rows(v), log_decay.asContiguous()
     out = empty((B, H, dv), q.dtype)
-    check(fn(B, H, KH, dk, dv, ct(scale), g.data_ptr(), *_rows(q), *_rows(k), *_rows(v), *s, *_rows(out)))
+    check(fn(B, H, KH, dk, dv, scale, g.data_ptr(), *_rows(q), *_rows(k), *_rows(v), *s, *_rows(out)))
     return out
 
 
@@ -280,7 +287,7 @@ def _ptr(t: HipTensor | None):
 
 
 def _normalise(name, x, weight, bias, groups, eps, activation, keep):
-    fn, ct = _entry("group_norm", x)
+    fn = _entry("group_norm", x)
     B, S, C = _norm_sizes(name, x, weight, bias, groups, activation)
     src, sn, ss = _channels_last(x)
     w, b = _vector(weight), _vector(bias)
@@ -289,7 +296,7 @@ def _normalise(name, x, weight, bias, groups, eps, activation, keep):
     if keep:
         make = empty if S * C else zeros
         mean, rstd = make((B, groups), x.dtype), make((B, groups), x.dtype)
-    check(fn(B, S, C, groups, ct(eps), ACT[activation], src.data_ptr(), sn, ss, _ptr(w), _ptr(b), y.data_ptr(), S * C, C, _ptr(mean), _ptr(rstd)))
+    check(fn(B, S, C, groups, eps, ACT[activation], src.data_ptr(), sn, ss, _ptr(w), _ptr(b), y.data_ptr(), S * C, C, _ptr(mean), _ptr(rstd)))
     return y, mean, rstd
 
 
@@ -313,7 +320,7 @@ def group_norm_backward(gradOutput: HipTensor, x: HipTensor, weight: HipTensor |
     """(dx, dweight, dbias) from the gradient of the output, the inputs of `group_norm_forward` and the mean and rstd that it
     returned; dweight and dbias have the shapes of weight and bias and are None where those are."""
     name = "group_norm_backward"
-    fn, ct = _entry(name, x)
+    fn = _entry(name, x)
     B, S, C = _norm_sizes(name, x, weight, bias, groups, activation)
     _same_dtype(x, gradOutput, mean, rstd)
     _shape(name, "the output's gradient", gradOutput, x.shape)
