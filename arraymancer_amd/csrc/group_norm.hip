@@ -9,13 +9,14 @@
 //
 // Two ways through it:
 //  - `team_*`: the elements of a group fit the registers of a team of lanes (8 .. 64, or a workgroup of 256). One launch,
-//    x is read once, mean and squared deviations are two folds over registers.
+//    x is read once, mean and squared deviations are two folds over registers. A team keeps its group and walks over samples,
+//    with the group's parameters in registers; backwards it also adds up its lanes' shares of dweight and dbias on the way.
 //  - slabs: a workgroup takes a slab of rows of one sample and reads them whole, channels next to each other, whatever the
 //    group's width; a lane owns V channels and keeps two sums for each. The slabs' sums per channel go to scratch memory
 //    and a small kernel folds them in a fixed order, per group (mean, rstd, or the two averages of the backward pass) and,
-//    backwards, per channel (dweight, dbias); then a second pass over the slabs writes the result. The sums of the forward
-//    pass are of x - pivot, with the group's first element as pivot, in double: no cancellation where the mean is large
-//    against the deviation.
+//    backwards, per channel; then a second pass over the slabs writes the result. The sums of the forward pass are of
+//    x - pivot, with the group's first element as pivot, in double: no cancellation where the mean is large against the
+//    deviation.
 #include "common.h"
 #include "fastdiv.h"
 #include "scratch.h"
@@ -30,7 +31,9 @@ template <typename T> struct Args {
   T* y; int64_t y_n, y_s;            // forward: the result; backward: dx
   T* mean; T* rstd;                  // [batch, groups]
   T* dweight; T* dbias;
-  double* part;                      // [n][slab][channel][2]
+  double* part;                      // slabs: [n][slab][channel][2]
+  double* chan;                      // slabs, backward: [n][channel][2], null when no parameter's gradient is wanted
+  T* share;                          // teams, backward: [slot][group][row][channel of the group][2] (workgroups: rows summed), null likewise
   T* coef;                           // backward: [n][group][2], the two averages
   T eps;
   int64_t batch, spatial;
@@ -39,24 +42,32 @@ template <typename T> struct Args {
   int slabs; int64_t rows_per_slab;
   int tiles, lanes, rows_at_once;    // channel tiles; lanes per row of a tile; rows a workgroup reads at once
   FastDiv per_div, tiles_div, slabs_div, groups_div, units_div;
-  int add;                           // backward: dweight / dbias are added to
 };
 
-__device__ __forceinline__ float dev_exp(float v) { return expf(v); }
-__device__ __forceinline__ double dev_exp(double v) { return exp(v); }
 __device__ __forceinline__ float dev_rsqrt(float v) { return 1.0f / sqrtf(v); }
 __device__ __forceinline__ double dev_rsqrt(double v) { return 1.0 / sqrt(v); }
 
+// 1 / (1 + e^-z). In float from the hardware's exp2 and reciprocal, one step each: -z log2(e) is split into the product
+// and what its rounding lost, so that the error does not grow with z (3 steps in all). The backward pass over a large image
+// spends most of its instructions here; expf and a division take three times as many.
+__device__ __forceinline__ float sigmoid(float z) {
+  const float hi = z * -1.44269504f;
+  const float lo = fmaf(z, -1.44269504f, -hi) + z * -1.92596299e-8f;
+  const float e = __builtin_amdgcn_exp2f(hi);
+  return __builtin_amdgcn_rcpf(1.0f + (e + e * (lo * 0.693147181f)));
+}
+__device__ __forceinline__ double sigmoid(double z) { return 1.0 / (1.0 + exp(-z)); }
+
 template <typename T, int ACT> __device__ __forceinline__ T activate(T z) {
   if constexpr (ACT == AM_ACT_RELU) return ((T)0 >= z) ? (T)0 : z;
-  else if constexpr (ACT == AM_ACT_SILU) return z / ((T)1 + dev_exp(-z));
+  else if constexpr (ACT == AM_ACT_SILU) return z * sigmoid(z);
   else return z;
 }
 // dy * act'(z)
 template <typename T, int ACT> __device__ __forceinline__ T through(T dy, T z) {
   if constexpr (ACT == AM_ACT_RELU) return ((T)0 >= z) ? (T)0 : dy;
   else if constexpr (ACT == AM_ACT_SILU) {
-    const T s = (T)1 / ((T)1 + dev_exp(-z));
+    const T s = sigmoid(z);
     return dy * (s * ((T)1 + z * ((T)1 - s)));
   } else return dy;
 }
@@ -77,113 +88,169 @@ template <typename T, bool WIDE> __device__ __forceinline__ T team_sum(T v, int 
 
 constexpr int kUnits = 8;   // units (vectors) a lane of a team holds at most
 
-// Unit q of a group (sample base pointers given): row q / units-per-row, channels V * (q % units-per-row) ...
-template <typename T, int V, bool WIDE, int ACT>
-__global__ __launch_bounds__(256) void team_forward(Args<T> p, int lanes, int units) {
-  typedef typename Vec<T, V>::type vec_t;
-  __shared__ T lds[4];
-  const int teams = WIDE ? 1 : 256 / lanes;
-  const int64_t team = (int64_t)blockIdx.x * teams + (WIDE ? 0 : (int)threadIdx.x / lanes);
-  const int j0 = WIDE ? (int)threadIdx.x : (int)threadIdx.x & (lanes - 1);
-  const int step = WIDE ? 256 : lanes;
-  if (!WIDE && team >= p.nc * p.groups) return;       // whole teams leave together, and teams never straddle a wavefront
-  const int64_t n = team / p.groups;
-  const int g = (int)(team - n * p.groups);
-  const T* x = p.x + n * p.x_n + (int64_t)g * p.per;
-  vec_t v[kUnits];
-  uint32_t row[kUnits], col[kUnits];
-  T sum = (T)0;
+// A team's place: its group, the first sample it takes, and its lanes' units (q = lane + k * lanes): row q / units-per-row of
+// the sample, channels V * (q % units-per-row) ... of the group. Units behind the last repeat it, so that every load is
+// unconditional; they count for nothing and are not written.
+template <typename T, int V, int U, bool WIDE> struct Team {
+  int j0, step, g;
+  int64_t slot;
+  bool there, live[U];
+  uint32_t row[U], col[U];
+  __device__ __forceinline__ Team(const Args<T>& p, int lanes, int units, int64_t slots) {
+    const int teams = WIDE ? 1 : 256 / lanes;
+    const int64_t team = (int64_t)blockIdx.x * teams + (WIDE ? 0 : (int)threadIdx.x / lanes);
+    j0 = WIDE ? (int)threadIdx.x : (int)threadIdx.x & (lanes - 1);
+    step = WIDE ? 256 : lanes;
+    slot = team / p.groups;
+    g = (int)(team - slot * p.groups);
+    there = slot < slots;
 #pragma unroll
-  for (int k = 0; k < kUnits; ++k) {
-    const int q = j0 + k * step;
-    if (q < units) {
+    for (int k = 0; k < U; ++k) {
+      int q = j0 + k * step;
+      live[k] = q < units;
+      q = live[k] ? q : units - 1;
       row[k] = p.units_div.divmod((uint32_t)q, col[k]);
-      v[k] = *(const vec_t*)(x + row[k] * p.x_s + col[k] * V);
+      col[k] *= V;
     }
   }
+};
+
+template <typename T, int V, int U, bool WIDE, int ACT>
+__global__ __launch_bounds__(256) void team_forward(Args<T> p, int lanes, int units, int64_t slots) {
+  typedef typename Vec<T, V>::type vec_t;
+  __shared__ T lds[4];
+  const Team<T, V, U, WIDE> t(p, lanes, units, slots);
+  if (!t.there) return;       // whole teams leave together, and teams never straddle a wavefront
+  const int c0 = t.g * p.per;
+  vec_t w[U], b[U];
 #pragma unroll
-  for (int k = 0; k < kUnits; ++k)
-    if (j0 + k * step < units)
-#pragma unroll
-      for (int e = 0; e < V; ++e) sum += v[k][e];
-  const T count = (T)((T)p.spatial * (T)p.per);
-  const T mean = team_sum<T, WIDE>(sum, lanes, lds) / count;
-  T sq = (T)0;
-#pragma unroll
-  for (int k = 0; k < kUnits; ++k)
-    if (j0 + k * step < units)
-#pragma unroll
-      for (int e = 0; e < V; ++e) { const T d = v[k][e] - mean; sq += d * d; }
-  const T rstd = dev_rsqrt(team_sum<T, WIDE>(sq, lanes, lds) / count + p.eps);
-  if (j0 == 0 && p.mean) { p.mean[team] = mean; p.rstd[team] = rstd; }
-  T* y = p.y + n * p.y_n + (int64_t)g * p.per;
-#pragma unroll
-  for (int k = 0; k < kUnits; ++k) {
-    if (j0 + k * step >= units) continue;
-    const int c = g * p.per + (int)col[k] * V;
-    vec_t out;
+  for (int k = 0; k < U; ++k)
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      T z = (v[k][e] - mean) * rstd;
-      if (p.weight) z *= p.weight[c + e];
-      if (p.bias) z += p.bias[c + e];
-      out[e] = activate<T, ACT>(z);
+      w[k][e] = p.weight ? p.weight[c0 + t.col[k] + e] : (T)1;
+      b[k][e] = p.bias ? p.bias[c0 + t.col[k] + e] : (T)0;
     }
-    *(vec_t*)(y + row[k] * p.y_s + col[k] * V) = out;
+  const T count = (T)((T)p.spatial * (T)p.per);
+  for (int64_t n = t.slot; n < p.batch; n += slots) {
+    const T* x = p.x + n * p.x_n + c0;
+    vec_t v[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) v[k] = *(const vec_t*)(x + t.row[k] * p.x_s + t.col[k]);
+    T sum = (T)0;
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+#pragma unroll
+      for (int e = 0; e < V; ++e) sum += t.live[k] ? v[k][e] : (T)0;
+    const T mean = team_sum<T, WIDE>(sum, lanes, lds) / count;
+    T sq = (T)0;
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        v[k][e] -= mean;
+        sq += t.live[k] ? v[k][e] * v[k][e] : (T)0;
+      }
+    const T rstd = dev_rsqrt(team_sum<T, WIDE>(sq, lanes, lds) / count + p.eps);
+    if (t.j0 == 0 && p.mean) { p.mean[n * p.groups + t.g] = mean; p.rstd[n * p.groups + t.g] = rstd; }
+    T* y = p.y + n * p.y_n + c0;
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      vec_t out;
+#pragma unroll
+      for (int e = 0; e < V; ++e) out[e] = activate<T, ACT>(v[k][e] * rstd * w[k][e] + b[k][e]);
+      if (t.live[k]) *(vec_t*)(y + t.row[k] * p.y_s + t.col[k]) = out;
+    }
   }
 }
 
-template <typename T, int V, bool WIDE, int ACT>
-__global__ __launch_bounds__(256) void team_backward(Args<T> p, int lanes, int units) {
+template <typename T, int V, int U, bool WIDE, int ACT>
+__global__ __launch_bounds__(256) void team_backward(Args<T> p, int lanes, int units, int64_t slots) {
   typedef typename Vec<T, V>::type vec_t;
   __shared__ T lds[4];
-  const int teams = WIDE ? 1 : 256 / lanes;
-  const int64_t team = (int64_t)blockIdx.x * teams + (WIDE ? 0 : (int)threadIdx.x / lanes);
-  const int j0 = WIDE ? (int)threadIdx.x : (int)threadIdx.x & (lanes - 1);
-  const int step = WIDE ? 256 : lanes;
-  if (!WIDE && team >= p.nc * p.groups) return;
-  const int64_t n = team / p.groups;
-  const int g = (int)(team - n * p.groups);
-  const T* x = p.x + n * p.x_n + (int64_t)g * p.per;
-  const T* dy = p.dy + n * p.dy_n + (int64_t)g * p.per;
-  const T mean = p.mean[team], rstd = p.rstd[team];
-  vec_t h[kUnits], d[kUnits];     // xhat and weight * dz
-  uint32_t row[kUnits], col[kUnits];
+  const Team<T, V, U, WIDE> t(p, lanes, units, slots);
+  if (!t.there) return;
+  const int c0 = t.g * p.per;
+  vec_t w[U], b[U], dw[U], db[U];
 #pragma unroll
-  for (int k = 0; k < kUnits; ++k) {
-    const int q = j0 + k * step;
-    if (q < units) {
-      row[k] = p.units_div.divmod((uint32_t)q, col[k]);
-      h[k] = *(const vec_t*)(x + row[k] * p.x_s + col[k] * V);
-      d[k] = *(const vec_t*)(dy + row[k] * p.dy_s + col[k] * V);
-    }
-  }
-  T s1 = (T)0, s2 = (T)0;
-#pragma unroll
-  for (int k = 0; k < kUnits; ++k) {
-    if (j0 + k * step >= units) continue;
-    const int c = g * p.per + (int)col[k] * V;
+  for (int k = 0; k < U; ++k)
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      h[k][e] = (h[k][e] - mean) * rstd;
-      const T w = p.weight ? p.weight[c + e] : (T)1;
-      const T z = h[k][e] * w + (p.bias ? p.bias[c + e] : (T)0);
-      d[k][e] = through<T, ACT>(d[k][e], z) * w;
-      s1 += d[k][e];
-      s2 += d[k][e] * h[k][e];
+      w[k][e] = p.weight ? p.weight[c0 + t.col[k] + e] : (T)1;
+      b[k][e] = p.bias ? p.bias[c0 + t.col[k] + e] : (T)0;
+      dw[k][e] = db[k][e] = (T)0;
+    }
+  const T count = (T)((T)p.spatial * (T)p.per);
+  for (int64_t n = t.slot; n < p.batch; n += slots) {
+    const T* x = p.x + n * p.x_n + c0;
+    const T* dy = p.dy + n * p.dy_n + c0;
+    const T mean = p.mean[n * p.groups + t.g], rstd = p.rstd[n * p.groups + t.g];
+    vec_t h[U], d[U];     // xhat and weight * dz
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      h[k] = *(const vec_t*)(x + t.row[k] * p.x_s + t.col[k]);
+      d[k] = *(const vec_t*)(dy + t.row[k] * p.dy_s + t.col[k]);
+    }
+    T s1 = (T)0, s2 = (T)0;
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        h[k][e] = (h[k][e] - mean) * rstd;
+        const T dz = through<T, ACT>(d[k][e], h[k][e] * w[k][e] + b[k][e]);
+        dw[k][e] += dz * h[k][e];
+        db[k][e] += dz;
+        d[k][e] = dz * w[k][e];
+        s1 += t.live[k] ? d[k][e] : (T)0;
+        s2 += t.live[k] ? d[k][e] * h[k][e] : (T)0;
+      }
+    s1 = team_sum<T, WIDE>(s1, lanes, lds) / count;
+    s2 = team_sum<T, WIDE>(s2, lanes, lds) / count;
+    T* dx = p.y + n * p.y_n + c0;
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      vec_t out;
+#pragma unroll
+      for (int e = 0; e < V; ++e) out[e] = rstd * (d[k][e] - s1 - h[k][e] * s2);
+      if (t.live[k]) *(vec_t*)(dx + t.row[k] * p.y_s + t.col[k]) = out;
     }
   }
-  const T count = (T)((T)p.spatial * (T)p.per);
-  s1 = team_sum<T, WIDE>(s1, lanes, lds) / count;
-  s2 = team_sum<T, WIDE>(s2, lanes, lds) / count;
-  T* dx = p.y + n * p.y_n + (int64_t)g * p.per;
+  if (!p.share) return;
+  if constexpr (WIDE) {
+    // a workgroup adds up the rows of its group first, a lane staying with one channel
+    __shared__ T rows[256 * U * V];
+    __shared__ T part[256];
+    const int wide = p.per < 256 ? p.per : 256, over = 256 / wide, k0 = (int)threadIdx.x / wide, cl = (int)threadIdx.x - k0 * wide;
+    for (int which = 0; which < 2; ++which) {
+      __syncthreads();
 #pragma unroll
-  for (int k = 0; k < kUnits; ++k) {
-    if (j0 + k * step >= units) continue;
-    vec_t out;
+      for (int k = 0; k < U; ++k)
+        if (t.live[k])
 #pragma unroll
-    for (int e = 0; e < V; ++e) out[e] = rstd * (d[k][e] - s1 - h[k][e] * s2);
-    *(vec_t*)(dx + row[k] * p.y_s + col[k] * V) = out;
+          for (int e = 0; e < V; ++e) rows[(t.j0 + k * 256) * V + e] = which ? db[k][e] : dw[k][e];
+      __syncthreads();
+      for (int b0 = 0; b0 < p.per; b0 += wide) {
+        const int c = b0 + cl;
+        const bool mine = k0 < over && c < p.per;
+        T sum = (T)0;
+        if (mine)
+          for (int r = k0; r < (int)p.spatial; r += over) sum += rows[r * p.per + c];
+        __syncthreads();
+        part[threadIdx.x] = sum;
+        __syncthreads();
+        if (mine && k0 == 0) {
+          for (int r = 1; r < over; ++r) sum += part[threadIdx.x + r * wide];
+          p.share[((t.slot * p.groups + t.g) * p.per + c) * 2 + which] = sum;
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      if (!t.live[k]) continue;
+      T* at = p.share + (((t.slot * p.groups + t.g) * p.spatial + t.row[k]) * p.per + t.col[k]) * 2;
+#pragma unroll
+      for (int e = 0; e < V; ++e) { at[2 * e] = dw[k][e]; at[2 * e + 1] = db[k][e]; }
+    }
   }
 }
 
@@ -201,9 +268,8 @@ template <typename T, int V> __device__ __forceinline__ Place place(const Args<T
   return w;
 }
 
-// Per slab and channel: the sums of x - pivot and of its square; BWD: the sums of dz and dz * xhat. FLAT (BWD): the slabs
-// cut the rows of all samples together (their sums are wanted per channel only), and a row's sample is its index / spatial.
-template <typename T, int V, bool BWD, bool FLAT, int ACT>
+// Per slab and channel: the sums of x - pivot and of its square; BWD: the sums of dz * xhat and dz.
+template <typename T, int V, bool BWD, int ACT>
 __global__ __launch_bounds__(256) void slab_sums(Args<T> p) {
   typedef typename Vec<T, V>::type vec_t;
   __shared__ double lds[256 * V * 2];
@@ -211,43 +277,68 @@ __global__ __launch_bounds__(256) void slab_sums(Args<T> p) {
   double a[V], b[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) a[e] = b[e] = 0.0;
-  const int64_t rows = FLAT ? p.nc * p.spatial : p.spatial;
   const int64_t lo = (int64_t)w.slab * p.rows_per_slab;
-  const int64_t hi = lo + p.rows_per_slab < rows ? lo + p.rows_per_slab : rows;
+  const int64_t hi = lo + p.rows_per_slab < p.spatial ? lo + p.rows_per_slab : p.spatial;
   if (w.live) {
     T pivot[V], mean[V], rstd[V], wt[V], bs[V];
-    int g[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      g[e] = (int)p.per_div.div((uint32_t)(w.c + e));
+      const int g = (int)p.per_div.div((uint32_t)(w.c + e));
       if constexpr (BWD) {
         wt[e] = p.weight ? p.weight[w.c + e] : (T)1;
         bs[e] = p.bias ? p.bias[w.c + e] : (T)0;
-        if constexpr (!FLAT) { mean[e] = p.mean[w.n * p.groups + g[e]]; rstd[e] = p.rstd[w.n * p.groups + g[e]]; }
+        mean[e] = p.mean[w.n * p.groups + g];
+        rstd[e] = p.rstd[w.n * p.groups + g];
       } else {
-        pivot[e] = p.x[w.n * p.x_n + (int64_t)g[e] * p.per];
+        pivot[e] = p.x[w.n * p.x_n + (int64_t)g * p.per];
       }
     }
-#pragma unroll 4
-    for (int64_t r = lo + w.row0; r < hi; r += p.rows_at_once) {
-      int64_t n = w.n, s = r;
-      if constexpr (FLAT) { n = p.spatial == 1 ? r : r / p.spatial; s = r - n * p.spatial; }
-      const vec_t xv = *(const vec_t*)(p.x + n * p.x_n + s * p.x_s + w.c);
-      if constexpr (BWD) {
-        const vec_t dv = *(const vec_t*)(p.dy + n * p.dy_n + s * p.dy_s + w.c);
+    const T* x = p.x + w.n * p.x_n + w.c;
+    const T* dy = BWD ? p.dy + w.n * p.dy_n + w.c : nullptr;
+    constexpr int R = 4;                         // rows on their way at once
+    int64_t s = lo + w.row0;
+    for (; s + (R - 1) * p.rows_at_once < hi; s += R * p.rows_at_once) {
+      vec_t xv[R], dv[R];
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          T m, q;
-          if constexpr (FLAT) { m = p.mean[n * p.groups + g[e]]; q = p.rstd[n * p.groups + g[e]]; }
-          else { m = mean[e]; q = rstd[e]; }
-          const T h = (xv[e] - m) * q;
-          const T dz = through<T, ACT>(dv[e], h * wt[e] + bs[e]);
-          a[e] += (double)dz;
-          b[e] += (double)dz * (double)h;
+      for (int r = 0; r < R; ++r) {
+        xv[r] = *(const vec_t*)(x + (s + r * p.rows_at_once) * p.x_s);
+        if constexpr (BWD) dv[r] = *(const vec_t*)(dy + (s + r * p.rows_at_once) * p.dy_s);
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        if constexpr (BWD) {                     // four rows in T, then on in double
+          T ha = (T)0, hb = (T)0;
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const T h = (xv[r][e] - mean[e]) * rstd[e];
+            const T dz = through<T, ACT>(dv[r][e], h * wt[e] + bs[e]);
+            ha += dz * h;
+            hb += dz;
+          }
+          a[e] += (double)ha;
+          b[e] += (double)hb;
+        } else {
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const double d = (double)xv[r][e] - (double)pivot[e];
+            a[e] += d;
+            b[e] += d * d;
+          }
         }
-      } else {
+      }
+    }
+    for (; s < hi; s += p.rows_at_once) {
+      const vec_t xv = *(const vec_t*)(x + s * p.x_s);
+      vec_t dv;
+      if constexpr (BWD) dv = *(const vec_t*)(dy + s * p.dy_s);
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
+      for (int e = 0; e < V; ++e) {
+        if constexpr (BWD) {
+          const T h = (xv[e] - mean[e]) * rstd[e];
+          const T dz = through<T, ACT>(dv[e], h * wt[e] + bs[e]);
+          a[e] += (double)(dz * h);
+          b[e] += (double)dz;
+        } else {
           const double d = (double)xv[e] - (double)pivot[e];
           a[e] += d;
           b[e] += d * d;
@@ -274,59 +365,101 @@ __global__ __launch_bounds__(256) void slab_sums(Args<T> p) {
   }
 }
 
-// The slabs' sums of one group, in a fixed order: mean and rstd, or (BWD) the two averages of the backward pass.
+// The slabs' sums of one group, in a fixed order: mean and rstd, or (BWD) the two averages of the backward pass and, where
+// they are wanted, each channel's sums over the sample. A lane stays with one channel (of up to 256 at a time) and takes
+// every so many-th slab.
 template <typename T, bool BWD>
-__global__ __launch_bounds__(64) void group_fold(Args<T> p) {
+__global__ __launch_bounds__(256) void group_fold(Args<T> p) {
+  typedef Vec<double, 2>::type pair_t;
+  __shared__ pair_t lds[256];
   uint32_t g;
   const int64_t n = p.groups_div.divmod(blockIdx.x, g);
-  double a = 0.0, b = 0.0;
-  const double* part = p.part + (n * p.slabs * (int64_t)p.channels + (int64_t)g * p.per) * 2;
-  const uint32_t total = (uint32_t)p.slabs * (uint32_t)p.per;
-  for (uint32_t i = threadIdx.x; i < total; i += 64) {
-    uint32_t c;
-    const uint32_t slab = p.per_div.divmod(i, c);
-    const double* at = part + ((int64_t)slab * p.channels + c) * 2;
-    const double w = (BWD && p.weight) ? (double)p.weight[g * p.per + c] : 1.0;
-    a += at[0] * w;
-    b += at[1] * w;
+  const pair_t* part = (const pair_t*)p.part + n * p.slabs * (int64_t)p.channels + (int64_t)g * p.per;
+  const int wide = p.per < 256 ? p.per : 256, rows = 256 / wide;
+  const int k = (int)threadIdx.x / wide, cl = (int)threadIdx.x - k * wide;
+  pair_t all = (pair_t)(0.0);                              // lanes of row 0: their channels' sums
+  for (int c0 = 0; c0 < p.per; c0 += wide) {
+    const int c = c0 + cl;
+    const bool live = k < rows && c < p.per;
+    pair_t s = (pair_t)(0.0);
+    if (live) {
+      int i = k;
+      for (; i + 7 * rows < p.slabs; i += 8 * rows) {
+        pair_t v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = part[(int64_t)(i + u * rows) * p.channels + c];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) s += v[u];
+      }
+      for (; i < p.slabs; i += rows) s += part[(int64_t)i * p.channels + c];
+    }
+    __syncthreads();
+    lds[threadIdx.x] = s;
+    __syncthreads();
+    if (live && k == 0) {
+      for (int r = 1; r < rows; ++r) s += lds[threadIdx.x + r * wide];
+      if constexpr (BWD) {
+        if (p.chan) ((pair_t*)p.chan)[n * p.channels + (int64_t)g * p.per + c] = s;
+        all += s * (p.weight ? (double)p.weight[g * p.per + c] : 1.0);
+      } else {
+        all += s;
+      }
+    }
   }
-  for (int d = 32; d >= 1; d >>= 1) { a += __shfl_xor(a, d, 64); b += __shfl_xor(b, d, 64); }
+  __syncthreads();
+  lds[threadIdx.x] = all;
+  __syncthreads();
+  for (int d = 128; d >= 1; d >>= 1) {
+    if ((int)threadIdx.x < d) lds[threadIdx.x] += lds[threadIdx.x + d];
+    __syncthreads();
+  }
   if (threadIdx.x) return;
+  all = lds[0];
   const double count = (double)p.spatial * (double)p.per;
   const int64_t at = n * p.groups + g;
   if constexpr (BWD) {
-    p.coef[2 * at] = (T)(a / count);
-    p.coef[2 * at + 1] = (T)(b / count);
+    p.coef[2 * at] = (T)(all[1] / count);
+    p.coef[2 * at + 1] = (T)(all[0] / count);
   } else {
-    const double m = a / count;
-    double var = b / count - m * m;
+    const double m = all[0] / count;
+    double var = all[1] / count - m * m;
     if (var < 0.0) var = 0.0;
     p.mean[at] = (T)((double)p.x[n * p.x_n + (int64_t)g * p.per] + m);
     p.rstd[at] = (T)(1.0 / sqrt(var + (double)p.eps));
   }
 }
 
-// dweight and dbias of 16 channels: 16 lanes side by side, 16 of them over the slabs, folded through LDS.
-template <typename T>
-__global__ __launch_bounds__(256) void channel_fold(Args<T> p, int64_t parts) {
+// dweight and dbias of 8 channels: 8 lanes side by side, 32 of them over the parts, folded through LDS. Part i (slot, row) of
+// channel c (group, channel of it) lies at ((slot * groups + group) * rows + row) * per + channel; rows = 1: at i * channels + c.
+template <typename T, typename P>
+__global__ __launch_bounds__(256) void channel_fold(Args<T> p, const P* part, int64_t slots, int rows, bool add) {
+  typedef typename Vec<P, 2>::type pair_t;
   __shared__ double lds[256][2];
-  const int c = (int)blockIdx.x * 16 + ((int)threadIdx.x & 15), k = (int)threadIdx.x >> 4;
+  const int c = (int)blockIdx.x * 8 + ((int)threadIdx.x & 7), k = (int)threadIdx.x >> 3;
   double a = 0.0, b = 0.0;
   if (c < p.channels) {
-#pragma unroll 4
-    for (int64_t i = k; i < parts; i += 16) {
-      const double* at = p.part + (i * p.channels + c) * 2;
-      a += at[0];
-      b += at[1];
+    uint32_t cg;
+    const uint32_t g = p.per_div.divmod((uint32_t)c, cg);
+    const pair_t* at = (const pair_t*)part + (int64_t)g * rows * p.per + cg;
+    const int64_t pitch = (int64_t)p.channels * rows, parts = slots * rows;
+    auto where = [&](int64_t i) { const int64_t slot = rows == 1 ? i : i / rows; return slot * pitch + (i - slot * rows) * p.per; };
+    int64_t i = k;
+    for (; i + 7 * 32 < parts; i += 8 * 32) {
+      pair_t v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = at[where(i + u * 32)];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) { a += (double)v[u][0]; b += (double)v[u][1]; }
     }
+    for (; i < parts; i += 32) { const pair_t v = at[where(i)]; a += (double)v[0]; b += (double)v[1]; }
   }
   lds[threadIdx.x][0] = a;
   lds[threadIdx.x][1] = b;
   __syncthreads();
   if (k != 0 || c >= p.channels) return;
-  for (int r = 1; r < 16; ++r) { a += lds[threadIdx.x + 16 * r][0]; b += lds[threadIdx.x + 16 * r][1]; }
-  if (p.dweight) p.dweight[c] = (T)(p.add ? (double)p.dweight[c] + b : b);
-  if (p.dbias) p.dbias[c] = (T)(p.add ? (double)p.dbias[c] + a : a);
+  for (int r = 1; r < 32; ++r) { a += lds[threadIdx.x + 8 * r][0]; b += lds[threadIdx.x + 8 * r][1]; }
+  if (p.dweight) p.dweight[c] = (T)(add ? (double)p.dweight[c] + a : a);
+  if (p.dbias) p.dbias[c] = (T)(add ? (double)p.dbias[c] + b : b);
 }
 
 // Second pass over the slabs: y from mean and rstd, or (BWD) dx from the averages too.
@@ -375,12 +508,12 @@ __global__ __launch_bounds__(256) void clear(T* a, T* b, int n) {
   if (b) b[i] = (T)0;
 }
 
-// How a team covers a group of `units` vectors; 0 when it does not fit.
+// How a team covers a group of `units` vectors: the narrowest team that holds four vectors a lane, or a workgroup with up to
+// eight; 0 when it does not fit.
 static int team_lanes(int64_t units) {
   for (int l = 8; l <= 64; l *= 2)
-    if (units <= (int64_t)l * 4) return l;      // four vectors in flight for a lane
-  if (units <= 256 * kUnits) return 256;
-  return 0;
+    if (units <= (int64_t)l * 4) return l;
+  return units <= 256 * kUnits ? 256 : 0;
 }
 
 template <typename T> static void set_slabs(Args<T>& p, int V, int64_t rows, int64_t samples) {
@@ -389,7 +522,7 @@ template <typename T> static void set_slabs(Args<T>& p, int V, int64_t rows, int
   p.lanes = cv < 256 ? cv : 256;
   p.rows_at_once = 256 / p.lanes;
   // a few workgroups for every CU, of at least eight rows for each lane
-  int64_t slabs = ((int64_t)num_cus() * 8 + samples * p.tiles - 1) / (samples * p.tiles);
+  int64_t slabs = ((int64_t)num_cus() * 4 + samples * p.tiles - 1) / (samples * p.tiles);
   const int64_t most = (rows + p.rows_at_once * 8 - 1) / (p.rows_at_once * 8);
   if (slabs > most) slabs = most;
   if (slabs < 1) slabs = 1;
@@ -422,55 +555,73 @@ static int check_args(const char* fn, int64_t batch, int64_t spatial, int64_t ch
   return AM_OK;
 }
 
-template <typename T, int ACT, bool BWD>
-static int team_pass(Args<T> p, int V, int lanes, int units) {
-  constexpr int W = 16 / (int)sizeof(T);
-  const int64_t teams_per_wg = 256 / lanes;
-  // at most 2^30 workgroups a launch
-  const int64_t per_launch = (((int64_t)1 << 30) * teams_per_wg) / p.groups;
-  const Args<T> all = p;
-  for (int64_t n = 0; n < all.batch; n += per_launch) {
-    p.nc = all.batch - n < per_launch ? all.batch - n : per_launch;
-    p.x = all.x + n * p.x_n;
-    p.y = all.y + n * p.y_n;
-    if (BWD) p.dy = all.dy + n * p.dy_n;
-    if (all.mean) { p.mean = all.mean + n * p.groups; p.rstd = all.rstd + n * p.groups; }
-    const dim3 grid((unsigned)((p.nc * p.groups + teams_per_wg - 1) / teams_per_wg)), block(256);
-    if (lanes == 256) {
-      if constexpr (BWD) {
-        if (V > 1) hipLaunchKernelGGL((team_backward<T, W, true, ACT>), grid, block, 0, stream(), p, lanes, units);
-        else hipLaunchKernelGGL((team_backward<T, 1, true, ACT>), grid, block, 0, stream(), p, lanes, units);
-      } else {
-        if (V > 1) hipLaunchKernelGGL((team_forward<T, W, true, ACT>), grid, block, 0, stream(), p, lanes, units);
-        else hipLaunchKernelGGL((team_forward<T, 1, true, ACT>), grid, block, 0, stream(), p, lanes, units);
-      }
-    } else {
-      if constexpr (BWD) {
-        if (V > 1) hipLaunchKernelGGL((team_backward<T, W, false, ACT>), grid, block, 0, stream(), p, lanes, units);
-        else hipLaunchKernelGGL((team_backward<T, 1, false, ACT>), grid, block, 0, stream(), p, lanes, units);
-      } else {
-        if (V > 1) hipLaunchKernelGGL((team_forward<T, W, false, ACT>), grid, block, 0, stream(), p, lanes, units);
-        else hipLaunchKernelGGL((team_forward<T, 1, false, ACT>), grid, block, 0, stream(), p, lanes, units);
-      }
-    }
-    AM_TRY(check_launch("group norm of teams"));
+template <typename T, int V, int U, bool WIDE, int ACT, bool BWD>
+static void launch_team(const Args<T>& p, int lanes, int units, int64_t slots, int64_t wgs) {
+  if constexpr (BWD) hipLaunchKernelGGL((team_backward<T, V, U, WIDE, ACT>), dim3((unsigned)wgs), dim3(256), 0, stream(), p, lanes, units, slots);
+  else hipLaunchKernelGGL((team_forward<T, V, U, WIDE, ACT>), dim3((unsigned)wgs), dim3(256), 0, stream(), p, lanes, units, slots);
+}
+
+#ifndef GNW
+#define GNW 2
+#endif
+template <typename T, int V, int ACT, bool BWD>
+static int team_pass(Args<T> p, int lanes, int units) {
+  // Samples per team: as many as leave eight workgroups for every CU (backwards GNW, whose shares of the parameters'
+  // gradients have to be written and read again), and at most 64, so that a lane's shares are short sums.
+  const int64_t at_once = 256 / lanes;
+  int64_t slots = (int64_t)num_cus() * (BWD ? GNW : 8) * at_once / p.groups;
+  if (slots < (p.batch + 63) / 64) slots = (p.batch + 63) / 64;
+  if (slots < 1) slots = 1;
+  if (slots > p.batch) slots = p.batch;
+  const int64_t each = (p.batch + slots - 1) / slots;
+  slots = (p.batch + each - 1) / each;
+  const int64_t wgs = (slots * p.groups + at_once - 1) / at_once;
+  if (wgs >= ((int64_t)1 << 31)) return fail(AM_E_SHAPE, "group norm: too many groups for one launch");
+  const int64_t rows = lanes == 256 ? 1 : p.spatial;      // of a slot's shares
+  Scratch share;
+  if (BWD && (p.dweight || p.dbias)) {
+    AM_TRY(share.take((size_t)slots * p.channels * (size_t)rows * 2 * sizeof(T)));
+    p.share = (T*)share.p;
+  }
+  const int per_lane = (units + lanes - 1) / lanes;
+  if (lanes == 256) {
+    if (per_lane <= 2) launch_team<T, V, 2, true, ACT, BWD>(p, lanes, units, slots, wgs);
+    else if (per_lane <= 4) launch_team<T, V, 4, true, ACT, BWD>(p, lanes, units, slots, wgs);
+    else launch_team<T, V, 8, true, ACT, BWD>(p, lanes, units, slots, wgs);
+  } else {
+    if (per_lane == 1) launch_team<T, V, 1, false, ACT, BWD>(p, lanes, units, slots, wgs);
+    else if (per_lane == 2) launch_team<T, V, 2, false, ACT, BWD>(p, lanes, units, slots, wgs);
+    else launch_team<T, V, 4, false, ACT, BWD>(p, lanes, units, slots, wgs);
+  }
+  AM_TRY(check_launch("group norm of teams"));
+  if (p.share) {
+    hipLaunchKernelGGL((channel_fold<T, T>), dim3((unsigned)((p.channels + 7) / 8)), dim3(256), 0, stream(), p, (const T*)p.share, slots, (int)rows, false);
+    AM_TRY(check_launch("channel_fold"));
   }
   return AM_OK;
+}
+
+// The team's way, if the groups fit it: AM_OK + taken.
+template <typename T, int ACT, bool BWD>
+static int try_teams(Args<T>& p, bool aligned, bool& taken) {
+  constexpr int W = 16 / (int)sizeof(T);
+  const int V = aligned && p.per % W == 0 ? W : 1;
+  const int64_t upr = p.per / V;
+  const int lanes = p.spatial <= 256 * kUnits ? team_lanes(p.spatial * upr) : 0;
+  taken = lanes > 0;
+  if (!taken) return AM_OK;
+  p.units_div = FastDiv((uint32_t)upr);
+  const int units = (int)(p.spatial * upr);
+  return V > 1 ? team_pass<T, W, ACT, BWD>(p, lanes, units) : team_pass<T, 1, ACT, BWD>(p, lanes, units);
 }
 
 template <typename T, int ACT>
 static int forward(Args<T> p) {
   constexpr int W = 16 / (int)sizeof(T);
   const bool aligned = fits<T>(p.x, p.x_n, p.x_s, p.batch, p.spatial) && fits<T>(p.y, p.y_n, p.y_s, p.batch, p.spatial);
-  {
-    const int V = aligned && p.per % W == 0 ? W : 1;
-    const int64_t upr = p.per / V;
-    const int lanes = p.spatial <= 256 * kUnits ? team_lanes(p.spatial * upr) : 0;
-    if (lanes) {
-      p.units_div = FastDiv((uint32_t)upr);
-      return team_pass<T, ACT, false>(p, V, lanes, (int)(p.spatial * upr));
-    }
-  }
+  bool taken;
+  AM_TRY((try_teams<T, ACT, false>(p, aligned, taken)));
+  if (taken) return AM_OK;
   const int V = aligned && p.channels % W == 0 ? W : 1;
   const Args<T> all = p;
   Scratch stats;
@@ -496,9 +647,9 @@ static int forward(Args<T> p) {
     p.mean = mean + n * p.groups;
     p.rstd = rstd + n * p.groups;
     const int64_t wgs = p.nc * p.slabs * p.tiles;
-    AM_GN_LAUNCH(slab_sums, V, wgs, false, false, ACT);
+    AM_GN_LAUNCH(slab_sums, V, wgs, false, ACT);
     AM_TRY(check_launch("slab_sums"));
-    hipLaunchKernelGGL((group_fold<T, false>), dim3((unsigned)(p.nc * p.groups)), dim3(64), 0, stream(), p);
+    hipLaunchKernelGGL((group_fold<T, false>), dim3((unsigned)(p.nc * p.groups)), dim3(256), 0, stream(), p);
     AM_TRY(check_launch("group_fold"));
     AM_GN_LAUNCH(slab_apply, V, wgs, false, ACT);
     AM_TRY(check_launch("slab_apply"));
@@ -517,35 +668,23 @@ static int backward(Args<T> p) {
   }
   const bool aligned = fits<T>(p.x, p.x_n, p.x_s, p.batch, p.spatial) && fits<T>(p.y, p.y_n, p.y_s, p.batch, p.spatial) &&
                        fits<T>(p.dy, p.dy_n, p.dy_s, p.batch, p.spatial);
+  bool taken;
+  AM_TRY((try_teams<T, ACT, true>(p, aligned, taken)));
+  if (taken) return AM_OK;
   const int V = aligned && p.channels % W == 0 ? W : 1;
   const Args<T> all = p;
   Scratch part;
-  const int TV = aligned && p.per % W == 0 ? W : 1;
-  const int64_t upr = p.per / TV;
-  const int lanes = p.spatial <= 256 * kUnits ? team_lanes(p.spatial * upr) : 0;
-  if (lanes) {
-    p.units_div = FastDiv((uint32_t)upr);
-    AM_TRY((team_pass<T, ACT, true>(p, TV, lanes, (int)(p.spatial * upr))));
-    if (!params) return AM_OK;
-    p.nc = p.batch;
-    set_slabs(p, V, p.batch * p.spatial, 1);
-    AM_TRY(part.take((size_t)p.slabs * p.channels * 2 * sizeof(double)));
-    p.part = (double*)part.p;
-    AM_GN_LAUNCH(slab_sums, V, (int64_t)p.slabs * p.tiles, true, true, ACT);
-    AM_TRY(check_launch("slab_sums"));
-    hipLaunchKernelGGL((channel_fold<T>), dim3((unsigned)((p.channels + 15) / 16)), dim3(256), 0, stream(), p, (int64_t)p.slabs);
-    return check_launch("channel_fold");
-  }
   set_slabs(p, V, p.spatial, p.batch);
   const size_t per_sample = (size_t)p.slabs * p.channels * 2 * sizeof(double);
   int64_t nc = (int64_t)(kMostScratch / per_sample);
   if (nc < 1) nc = 1;
   if (nc > p.batch) nc = p.batch;
   const size_t coef_bytes = (size_t)nc * p.groups * 2 * sizeof(T);
-  const size_t part_bytes = per_sample * (size_t)nc;
-  AM_TRY(part.take(part_bytes + coef_bytes));
+  const size_t part_bytes = per_sample * (size_t)nc, chan_bytes = params ? (size_t)nc * p.channels * 2 * sizeof(double) : 0;
+  AM_TRY(part.take(part_bytes + chan_bytes + coef_bytes));
   p.part = (double*)part.p;
-  p.coef = (T*)((char*)part.p + part_bytes);
+  p.chan = params ? (double*)((char*)part.p + part_bytes) : nullptr;
+  p.coef = (T*)((char*)part.p + part_bytes + chan_bytes);
   for (int64_t n = 0; n < all.batch; n += nc) {
     p.nc = all.batch - n < nc ? all.batch - n : nc;
     p.x = all.x + n * p.x_n;
@@ -554,13 +693,12 @@ static int backward(Args<T> p) {
     p.mean = all.mean + n * p.groups;
     p.rstd = all.rstd + n * p.groups;
     const int64_t wgs = p.nc * p.slabs * p.tiles;
-    AM_GN_LAUNCH(slab_sums, V, wgs, true, false, ACT);
+    AM_GN_LAUNCH(slab_sums, V, wgs, true, ACT);
     AM_TRY(check_launch("slab_sums"));
-    hipLaunchKernelGGL((group_fold<T, true>), dim3((unsigned)(p.nc * p.groups)), dim3(64), 0, stream(), p);
+    hipLaunchKernelGGL((group_fold<T, true>), dim3((unsigned)(p.nc * p.groups)), dim3(256), 0, stream(), p);
     AM_TRY(check_launch("group_fold"));
     if (params) {
-      p.add = n > 0;
-      hipLaunchKernelGGL((channel_fold<T>), dim3((unsigned)((p.channels + 15) / 16)), dim3(256), 0, stream(), p, p.nc * p.slabs);
+      hipLaunchKernelGGL((channel_fold<T, double>), dim3((unsigned)((p.channels + 7) / 8)), dim3(256), 0, stream(), p, (const double*)p.chan, p.nc, 1, n > 0);
       AM_TRY(check_launch("channel_fold"));
     }
     AM_GN_LAUNCH(slab_apply, V, wgs, true, ACT);
