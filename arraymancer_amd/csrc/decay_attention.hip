@@ -42,41 +42,31 @@ __device__ __forceinline__ double dev_exp(double v) { return exp(v); }
 // e^{g n}; e^0 also where g is -infinity
 template <typename T> __device__ __forceinline__ T power(T g, int64_t n) { return n == 0 ? (T)1 : dev_exp(g * (T)n); }
 
-template <typename T> struct Mma;
-template <> struct Mma<float> {
-  typedef float acc_t __attribute__((ext_vector_type(4)));
-  static __device__ __forceinline__ acc_t mma(float a, float b, acc_t c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
-  // the operand row that lane % 16 = r brings, so that register i of lane group g holds row 4 g + i of the result
-  static __device__ __forceinline__ int row(int r) { return r; }
-};
-template <> struct Mma<double> {
-  typedef double acc_t __attribute__((ext_vector_type(4)));
-  static __device__ __forceinline__ acc_t mma(double a, double b, acc_t c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
-  // (this instruction's result has row 4 i + g there)
-  static __device__ __forceinline__ int row(int r) { return 4 * (r & 3) + (r >> 2); }
-};
-
 // ---- chunks of 32 tokens on the matrix cores ---------------------------------------------------------------------------
 //
 // For the tokens of a chunk, i and j counted within it, and the state S in front of it,
 //     o_i = sum_{j <= i} A_ij c_j + e^{g (i + after)} a_i S      A_ij = e^{g (i - j)} (a_i . b_j)
 //     S <- e^{g N} S + sum_j e^{g (N - after - j)} b_j^T c_j
 // so a chunk is four products: a b^T (32 x 32), A c, a S and b^T c. A workgroup of four wavefronts walks the chunks of one
-// head, a wavefront owning 16 columns of S and of o for all da rows, as accumulators that never leave its registers:
-//   - the 16 x 16 x 4 product leaves four consecutive rows of its result in a lane, and the sum over k may take its k in any
-//     order that both operands share: register i of S's tile is the right operand of the i-th of four instructions whose k
-//     are the rows 4 g + i. So S enters a S as it stands.
+// head, a wavefront owning columns of S and of o for all da rows, as accumulators that never leave its registers: the product
+// instructions leave neighbouring rows of a result in a lane, and the sum over k may take its k in any order that both
+// operands share, so the rows of S a lane holds are k of the next product's right operand as they stand.
 //   - a b^T is computed transposed, so that a lane's four values lie next to each other in a row of A in LDS; the three
 //     tiles on and under the diagonal go to three wavefronts.
 //   - c is read straight into the layout of a right operand, which A c and b^T c share.
-// a and b go through LDS in rows padded by 16 bytes; the next chunk's are on their way in registers meanwhile.
-// All exponents of e^g are differences that the mask leaves >= 0, so nothing overflows however long the text.
+// a and b go through LDS; the next chunk's are on their way in registers meanwhile. All exponents of e^g are differences that
+// the mask leaves >= 0, so nothing overflows however long the text.
 //
-// Where the heads alone do not fill the device, the tokens are cut into segments: `segment_sums` adds up each segment's
-// share of the state, `segment_states` carries them from segment to segment, and `chunks` starts every segment from its own.
+// float64 runs on the 16 x 16 x 4 product of doubles (`chunks_f64`). float32 does not run on its float counterpart, which has
+// a sixteenth of the bfloat16 rate: every operand is the sum of three bfloat16 (8 bits each, 24 in all: `split`), and a
+// product takes the six pairs of pieces down to 2^-16 (the three that are left out are below 2^-24 of the term, a float's
+// half step), with float32 sums inside the instruction: `chunks_f32`. Measured on 4 x 4096 tokens, 16 heads of 128 x 128:
+// 291 us with the float instruction, FILLIN us in pieces.
+//
+// Where the heads alone do not fill the device, the tokens are cut into segments: `sums_*` add up each segment's share of the
+// state, `segment_states` carries them from segment to segment, and the chunk kernels start every segment from its own.
 constexpr int64_t kMostDim = 256;
 constexpr int kChunk = 32;
-constexpr int kCols = 64;      // columns of a workgroup
 constexpr int kLds = 160 * 1024;
 
 template <typename T> struct Plan {
@@ -85,6 +75,52 @@ template <typename T> struct Plan {
   int parts, slots;            // parts of a segment; slots = parts * (segments - 1) + 1, one in front of every part but the last segment's later ones
   int64_t seg_tokens, part_tokens;   // multiples of kChunk, seg_tokens = parts * part_tokens
   int groups;                  // batch * heads
+};
+
+// What a workgroup works on. The slices of one (head, segment) read the same a and b: they get ids that are equal modulo
+// the eight dies, whose L2 they share.
+struct Work { int slice, segment, group; bool live; };
+template <typename T> __device__ __forceinline__ Work work_of(const Plan<T>& pl, int segments) {
+  const unsigned id = blockIdx.x, rest = id >> 3;
+  Work w;
+  w.slice = (int)(rest % (unsigned)pl.slices);
+  const unsigned item = (rest / (unsigned)pl.slices) * 8 + (id & 7);
+  w.segment = (int)(item % (unsigned)segments);
+  w.group = (int)(item / (unsigned)segments);
+  w.live = w.group < pl.groups;
+  return w;
+}
+
+template <typename T> __device__ __forceinline__ int64_t length_of(const Role<T>& p, int64_t b) {
+  if (!p.lengths) return p.tokens;
+  const int64_t l = p.lengths[b];
+  return l < 0 ? 0 : (l < p.tokens ? l : p.tokens);
+}
+
+// The stretch of a head's walk that a workgroup takes: local tokens lo .. lo + total, local token i being token i or, walking
+// back, n - 1 - i. The pointers are those of the first one, t_* the steps to the next.
+template <typename T, bool BACK> struct Path {
+  int64_t b, n, lo, hi, total;
+  int h;
+  const T *a, *k, *c;
+  T* o;
+  int64_t ta, tk, tc, to;
+  __device__ __forceinline__ Path(const Role<T>& p, int group, int64_t lo_, int64_t tokens) {
+    b = group / (int)p.heads;
+    h = (int)(group - b * p.heads);
+    n = length_of(p, b);
+    lo = lo_;
+    hi = lo + tokens < p.tokens ? lo + tokens : p.tokens;
+    total = (hi < n ? hi : n) - lo;
+    const int64_t first = BACK ? n - 1 - lo : lo, dir = BACK ? -1 : 1;
+    a = p.a.p + b * p.a.b + (h / p.a.group) * p.a.h + first * p.a.t;
+    k = p.b.p + b * p.b.b + (h / p.b.group) * p.b.h + first * p.b.t;
+    c = p.c.p + b * p.c.b + (h / p.c.group) * p.c.h + first * p.c.t;
+    o = p.out + b * p.o_b + h * p.o_h + first * p.o_t;
+    ta = dir * p.a.t; tk = dir * p.b.t; tc = dir * p.c.t; to = dir * p.o_t;
+  }
+  // tokens of the chunk at local token `at`, 1 .. 32
+  __device__ __forceinline__ int tokens(int64_t at) const { return total - at < kChunk ? (int)(total - at) : kChunk; }
 };
 
 // The n <= 32 tokens of a chunk as a buffer: the hardware adds a lane's 32-bit offset to a uniform base, and what lies outside
@@ -116,11 +152,10 @@ template <typename T, int DA, bool FAST> struct Tile {
   static constexpr bool EVEN = 256 % PER_ROW == 0;       // vector u of a lane lies whole rows behind its first
   static constexpr int NO = EVEN ? 1 : NV;
   typedef T vec_t __attribute__((ext_vector_type(V)));
-  static constexpr int PITCH = DA + V;
   vec_t v[NV];
   uint32_t off[NO];                                      // of a lane's vectors behind the chunk's first token
 
-  __device__ __forceinline__ void prepare(int64_t step, int da) {
+  __device__ __forceinline__ void prepare(int64_t step) {
     if constexpr (FAST) {
 #pragma unroll
       for (int u = 0; u < NO; ++u) {
@@ -150,7 +185,8 @@ template <typename T, int DA, bool FAST> struct Tile {
       }
     }
   }
-  __device__ __forceinline__ void store(T* lds, int n, int da) const {
+  // write(row, column, vector) for every vector of the lane
+  template <typename F> __device__ __forceinline__ void store(int n, int da, F write) const {
     const bool all = n == kChunk && da == DA;
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
@@ -160,61 +196,14 @@ template <typename T, int DA, bool FAST> struct Tile {
 #pragma unroll
         for (int e = 0; e < V; ++e) w[e] = (row < n && c + (FAST ? 0 : e) < da) ? w[e] : (T)0;
       }
-      *(vec_t*)(lds + row * PITCH + c) = w;
+      write(row, c, w);
     }
   }
 };
 
-// Four neighbouring elements of LDS.
-template <typename T> __device__ __forceinline__ void four(const T* lds, T (&out)[4]) {
-  constexpr int V = 16 / (int)sizeof(T);
-  typedef T vec_t __attribute__((ext_vector_type(V)));
-#pragma unroll
-  for (int i = 0; i < 4; i += V) {
-    const vec_t w = *(const vec_t*)(lds + i);
-#pragma unroll
-    for (int e = 0; e < V; ++e) out[i + e] = w[e];
-  }
-}
-
 // Nothing moves across here: the LDS reads of the next step stay in front of the matrix instructions of this one. Left alone,
 // the scheduler puts every read right in front of its use, and the wavefront waits for LDS in every step.
 __device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0); }
-
-// What a workgroup works on. The slices of one (head, segment) read the same a and b: they get ids that are equal modulo
-// the eight dies, whose L2 they share.
-struct Work { int slice, segment, group; bool live; };
-template <typename T> __device__ __forceinline__ Work work_of(const Plan<T>& pl, int segments) {
-  const unsigned id = blockIdx.x, rest = id >> 3;
-  Work w;
-  w.slice = (int)(rest % (unsigned)pl.slices);
-  const unsigned item = (rest / (unsigned)pl.slices) * 8 + (id & 7);
-  w.segment = (int)(item % (unsigned)segments);
-  w.group = (int)(item / (unsigned)segments);
-  w.live = w.group < pl.groups;
-  return w;
-}
-
-template <typename T> __device__ __forceinline__ int64_t length_of(const Role<T>& p, int64_t b) {
-  if (!p.lengths) return p.tokens;
-  const int64_t l = p.lengths[b];
-  return l < 0 ? 0 : (l < p.tokens ? l : p.tokens);
-}
-
-// One wavefront's share of a chunk's sum over the tokens: S <- e^{g N} S + b^T (w c), c given weighted.
-template <typename T, int DA>
-__device__ __forceinline__ void add_tokens(typename Mma<T>::acc_t (&S)[DA / 16], const T* sB, const T (&wc)[2][4], T lam, int pr, int g) {
-  constexpr int PITCH = DA + 16 / (int)sizeof(T);
-#pragma unroll
-  for (int kt = 0; kt < DA / 16; ++kt) {
-    S[kt] *= lam;
-#pragma unroll
-    for (int jt = 0; jt < 2; ++jt)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        S[kt] = Mma<T>::mma(sB[(16 * jt + 4 * g + r) * PITCH + 16 * kt + pr], wc[jt][r], S[kt]);
-  }
-}
 
 // c of a chunk of n >= 1 tokens, in the layout of a right operand: register r of tile jt is token 16 jt + 4 g + r, in column
 // `col`. `take` makes tokens behind the n-th 0.
@@ -252,6 +241,34 @@ __device__ __forceinline__ void take(T (&c)[2][4], const T (&from)[2][4], int n,
     for (int r = 0; r < 4; ++r) c[jt][r] = 16 * jt + 4 * g + r < n ? from[jt][r] : (T)0;
 }
 
+// The lane's column of a chunk's result: register r of tile it is token 16 it + 4 g + r.
+template <typename T, typename A, bool FAST>
+__device__ __forceinline__ void put_o(const A (&o)[2], T* p, int64_t step, int n, int g, int col, int width) {
+  if constexpr (FAST) {
+    const Chunk k = chunk_of(p, step, n, width);
+    const uint32_t off = (uint32_t)((4 * g * (int)step + col) * (int)sizeof(T));
+#pragma unroll
+    for (int it = 0; it < 2; ++it)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) put(k, off + (k.first + (uint32_t)((16 * it + r) * (int)step * (int)sizeof(T))), o[it][r]);
+  } else {
+#pragma unroll
+    for (int it = 0; it < 2; ++it)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = 16 * it + 4 * g + r;
+        if (i < n) p[i * step + col] = o[it][r];
+      }
+  }
+}
+
+// Zeros into the lane's column behind the sequence, as far as the stretch goes.
+template <typename T, bool BACK>
+__device__ __forceinline__ void zero_tail(const Role<T>& p, const Path<T, BACK>& path, int g, int col) {
+  T* o = p.out + path.b * p.o_b + path.h * p.o_h + col;
+  for (int64_t t = (path.lo > path.n ? path.lo : path.n) + g; t < path.hi; t += 4) o[t * p.o_t] = (T)0;
+}
+
 // scale * e^{g (n - after - j)} of this lane's tokens
 template <typename T>
 __device__ __forceinline__ void weights(T (&w)[2][4], T scale, T ld, int n, int after, int g) {
@@ -264,96 +281,116 @@ __device__ __forceinline__ void weights(T (&w)[2][4], T scale, T ld, int n, int 
     }
 }
 
-#ifndef WPE
-#define WPE 2
-#endif
-template <typename T, int DA, bool BACK, bool FAST>
-__global__ __launch_bounds__(256, sizeof(T) == 4 ? WPE : 1) void chunks(Role<T> p, Plan<T> pl) {
-  typedef typename Mma<T>::acc_t acc_t;
-  typedef Tile<T, DA, FAST> tile_t;
-  constexpr int KT = DA / 16, V = tile_t::V, PITCH = tile_t::PITCH, APITCH = kChunk + V;
-  constexpr int after = BACK ? 0 : 1;
-  constexpr int BUFS = (4 * kChunk * PITCH + kChunk * APITCH) * (int)sizeof(T) <= kLds ? 2 : 1;
-  __shared__ __attribute__((aligned(16))) T bufs[BUFS][2][kChunk * PITCH];
-  __shared__ __attribute__((aligned(16))) T sA[kChunk * APITCH];
-  const Work w = work_of(pl, pl.segments);
-  if (!w.live) return;
-  const int64_t b = w.group / (int)p.heads;
-  const int h = (int)(w.group - b * p.heads);
-  const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63, g = lane >> 4, lr = lane & 15, pr = Mma<T>::row(lr);
-  const int col = w.slice * kCols + wave * 16 + lr;
-  const bool live = col < p.dc;
-  const int64_t n = length_of(p, b);
-  const int64_t lo = w.segment * pl.seg_tokens;
-  int64_t hi = lo + pl.seg_tokens;
-  if (hi > p.tokens) hi = p.tokens;
-  const int64_t end = hi < n ? hi : n;                      // local tokens lo .. end of the walk
-  // local token i is token i, or n - 1 - i
-  const int64_t first = BACK ? n - 1 - lo : lo, dir = BACK ? -1 : 1;
-  const T* pa = p.a.p + b * p.a.b + (h / p.a.group) * p.a.h + first * p.a.t;
-  const T* pb = p.b.p + b * p.b.b + (h / p.b.group) * p.b.h + first * p.b.t;
-  const T* pc = p.c.p + b * p.c.b + (h / p.c.group) * p.c.h + first * p.c.t;
-  const int ccol = live ? col : p.dc - 1;
-  T* po = p.out + b * p.o_b + h * p.o_h;
-  const int64_t ta = dir * p.a.t, tb = dir * p.b.t, tc = dir * p.c.t;
-
-  acc_t S[KT];
-  const T* s0 = pl.states ? pl.states + ((int64_t)w.group * pl.slots + w.segment * pl.parts) * p.da * p.dc : (p.s0 ? p.s0 + b * p.s0_b + h * p.s0_h : nullptr);
-  const int64_t s0_r = pl.states ? p.dc : p.s0_r, s0_c = pl.states ? 1 : p.s0_c;
-#pragma unroll
-  for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int d = 16 * kt + 4 * g + r;
-      S[kt][r] = (s0 && live && d < p.da) ? s0[d * s0_r + col * s0_c] : (T)0;
-    }
-  const T ld = p.log_decay[h];
-  T reach[2][4], mask[2][4], wt[2][4];
+// The factors of a lane's rows: reach, e^{g (i + after)} of its rows of o; mask, e^{g (i - j)} or 0 of its row j, column i of a
+// transposed tile of A at distance 0 and 1; both with the scales in.
+template <typename T>
+__device__ __forceinline__ void row_factors(T (&reach)[2][4], T (&mask)[2][4], const Role<T>& p, T ld, int after, int g, int lr) {
 #pragma unroll
   for (int it = 0; it < 2; ++it)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       reach[it][r] = p.scale_a * power(ld, (int64_t)(16 * it + 4 * g + r + after));
-      const int apart = 16 * it + lr - 4 * g - r;          // i - j of tile distance `it`, transposed
+      const int apart = 16 * it + lr - 4 * g - r;
       mask[it][r] = apart >= 0 ? p.scale_a * p.scale_b * power(ld, (int64_t)apart) : (T)0;
     }
-  weights(wt, p.scale_b, ld, kChunk, after, g);
-  T lam = power(ld, (int64_t)kChunk);
+}
 
-  tile_t a, k;
-  T c[2][4], cn[2][4];
-  a.prepare(ta, p.da);
-  k.prepare(tb, p.da);
-  const int64_t to = dir * p.o_t;
-  const int64_t total = end - lo;
-  if (total > 0) {
-    const int m = total < kChunk ? (int)total : kChunk;
-    a.load(pa, ta, m, p.da);
-    k.load(pb, tb, m, p.da);
-    load_c<T, FAST>(cn, pc, tc, m, g, ccol, p.dc);
-    a.store(bufs[0][0], m, p.da);
-    k.store(bufs[0][1], m, p.da);
+// Where the first state of a segment is read, and its strides.
+template <typename T> struct First { const T* p; int64_t r, c; };
+template <typename T> __device__ __forceinline__ First<T> first_state(const Role<T>& p, const Plan<T>& pl, const Work& w, int64_t b, int h) {
+  if (pl.states) return {pl.states + ((int64_t)w.group * pl.slots + w.segment * pl.parts) * p.da * p.dc, p.dc, 1};
+  return {p.s0 ? p.s0 + b * p.s0_b + h * p.s0_h : nullptr, p.s0_r, p.s0_c};
+}
+
+// ---- float64 ----
+// A lane's four registers of a 16 x 16 result are rows 4 i + g there (i the register, g = lane / 16). The rows that lanes bring
+// as left operand are ordered so that they are rows 4 g + i all the same, and a left operand's four k lie side by side in LDS.
+typedef double acc64 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ acc64 mma64(double a, double b, acc64 c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ int row64(int r) { return 4 * (r & 3) + (r >> 2); }
+constexpr int kCols64 = 64;    // columns of a workgroup
+
+__device__ __forceinline__ void four(const double* lds, double (&out)[4]) {
+  typedef double d2 __attribute__((ext_vector_type(2)));
+  const d2 a = *(const d2*)lds, b = *(const d2*)(lds + 2);
+  out[0] = a[0]; out[1] = a[1]; out[2] = b[0]; out[3] = b[1];
+}
+
+// One wavefront's share of a chunk's sum over the tokens: S <- e^{g N} S + b^T (w c), c given weighted.
+template <int DA>
+__device__ __forceinline__ void add_tokens64(acc64 (&S)[DA / 16], const double* sB, const double (&wc)[2][4], double lam, int pr, int g) {
+  constexpr int PITCH = DA + 2;
+#pragma unroll
+  for (int kt = 0; kt < DA / 16; ++kt) {
+    S[kt] *= lam;
+#pragma unroll
+    for (int jt = 0; jt < 2; ++jt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        S[kt] = mma64(sB[(16 * jt + 4 * g + r) * PITCH + 16 * kt + pr], wc[jt][r], S[kt]);
   }
+}
+
+template <int DA, bool BACK, bool FAST>
+__global__ __launch_bounds__(256) void chunks_f64(Role<double> p, Plan<double> pl) {
+  constexpr int KT = DA / 16, PITCH = DA + 2, APITCH = kChunk + 2;
+  constexpr int after = BACK ? 0 : 1;
+  constexpr int BUFS = (4 * kChunk * PITCH + kChunk * APITCH) * 8 <= kLds ? 2 : 1;
+  __shared__ __attribute__((aligned(16))) double bufs[BUFS][2][kChunk * PITCH];
+  __shared__ __attribute__((aligned(16))) double sA[kChunk * APITCH];
+  const Work w = work_of(pl, pl.segments);
+  if (!w.live) return;
+  const Path<double, BACK> path(p, w.group, w.segment * pl.seg_tokens, pl.seg_tokens);
+  const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63, g = lane >> 4, lr = lane & 15, pr = row64(lr);
+  const int col = w.slice * kCols64 + wave * 16 + lr;
+  const bool live = col < p.dc;
+  const int ccol = live ? col : p.dc - 1;
+  acc64 S[KT];
+  const First<double> s0 = first_state(p, pl, w, path.b, path.h);
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int d = 16 * kt + 4 * g + r;
+      S[kt][r] = (s0.p && live && d < p.da) ? s0.p[d * s0.r + col * s0.c] : 0.0;
+    }
+  const double ld = p.log_decay[path.h];
+  double reach[2][4], mask[2][4], wt[2][4];
+  row_factors(reach, mask, p, ld, after, g, lr);
+  weights(wt, p.scale_b, ld, kChunk, after, g);
+  double lam = power(ld, (int64_t)kChunk);
+
+  Tile<double, DA, FAST> a, k;
+  double c[2][4], cn[2][4];
+  a.prepare(path.ta);
+  k.prepare(path.tk);
+  auto fetch = [&](int64_t at) {
+    const int m = path.tokens(at);
+    a.load(path.a + at * path.ta, path.ta, m, p.da);
+    k.load(path.k + at * path.tk, path.tk, m, p.da);
+    load_c<double, FAST>(cn, path.c + at * path.tc, path.tc, m, g, ccol, p.dc);
+  };
+  auto stage = [&](double (&to)[2][kChunk * PITCH], int m) {
+    typedef double d2 __attribute__((ext_vector_type(2)));
+    a.store(m, p.da, [&](int row, int cc, d2 v) { *(d2*)(to[0] + row * PITCH + cc) = v; });
+    k.store(m, p.da, [&](int row, int cc, d2 v) { *(d2*)(to[1] + row * PITCH + cc) = v; });
+  };
+  if (path.total > 0) { fetch(0); stage(bufs[0], path.tokens(0)); }
   int turn = 0;
-  for (int64_t at = 0; at < total; at += kChunk) {
+  for (int64_t at = 0; at < path.total; at += kChunk) {
     const int64_t next = at + kChunk;
-    const int m = total - at < kChunk ? (int)(total - at) : kChunk;
-    const int mn = total - next < kChunk ? (int)(total - next) : kChunk;
-    const T* sQ = bufs[turn][0];
-    const T* sB = bufs[turn][1];
+    const int m = path.tokens(at);
+    const double* sQ = bufs[turn][0];
+    const double* sB = bufs[turn][1];
     take(c, cn, m, g);
     __syncthreads();
-    if (next < total) {
-      a.load(pa + next * ta, ta, mn, p.da);
-      k.load(pb + next * tb, tb, mn, p.da);
-      load_c<T, FAST>(cn, pc + next * tc, tc, mn, g, ccol, p.dc);
-    }
+    if (next < path.total) fetch(next);
     if (wave < 3) {                                         // tiles (0, 0), (1, 0), (1, 1) of A
       const int it = wave ? 1 : 0, jt = wave == 2 ? 1 : 0;
-      acc_t t = (acc_t)((T)0);
-      const T* px = sB + (16 * jt + pr) * PITCH + 4 * g;
-      const T* py = sQ + (16 * it + lr) * PITCH + 4 * g;
-      T x[2][4], y[2][4];
+      acc64 t = (acc64)(0.0);
+      const double* px = sB + (16 * jt + pr) * PITCH + 4 * g;
+      const double* py = sQ + (16 * it + lr) * PITCH + 4 * g;
+      double x[2][4], y[2][4];
       four(px, x[0]);
       four(py, y[0]);
 #pragma unroll
@@ -364,21 +401,21 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? WPE : 1) void chunks(Role<T> 
         }
         pin();
 #pragma unroll
-        for (int r = 0; r < 4; ++r) t = Mma<T>::mma(x[kt & 1][r], y[kt & 1][r], t);
+        for (int r = 0; r < 4; ++r) t = mma64(x[kt & 1][r], y[kt & 1][r], t);
         pin();
       }
-      T* q = sA + (16 * it + lr) * APITCH + 16 * jt + 4 * g;
+      double* q = sA + (16 * it + lr) * APITCH + 16 * jt + 4 * g;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const bool under = it > jt || lr >= 4 * g + r;
-        q[r] = under ? t[r] * (it > jt ? mask[1][r] : mask[0][r]) : (T)0;
+        const bool under = it > jt || lr >= 4 * g + r;      // a choice, not a product with 0: the term above may be a NaN
+        q[r] = under ? t[r] * (it > jt ? mask[1][r] : mask[0][r]) : 0.0;
       }
     }
-    acc_t o[2];
+    acc64 o[2];
     {
-      const T* px = sQ + pr * PITCH + 4 * g;
-      T x[2][2][4];
-      o[0] = o[1] = (acc_t)((T)0);
+      const double* px = sQ + pr * PITCH + 4 * g;
+      double x[2][2][4];
+      o[0] = o[1] = (acc64)(0.0);
       four(px, x[0][0]);
       four(px + 16 * PITCH, x[0][1]);
 #pragma unroll
@@ -390,8 +427,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? WPE : 1) void chunks(Role<T> 
         pin();
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          o[0] = Mma<T>::mma(x[kt & 1][0][r], S[kt][r], o[0]);
-          o[1] = Mma<T>::mma(x[kt & 1][1][r], S[kt][r], o[1]);
+          o[0] = mma64(x[kt & 1][0][r], S[kt][r], o[0]);
+          o[1] = mma64(x[kt & 1][1][r], S[kt][r], o[1]);
         }
         pin();
       }
@@ -402,58 +439,35 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? WPE : 1) void chunks(Role<T> 
       for (int r = 0; r < 4; ++r) o[it][r] *= reach[it][r];
     __syncthreads();
     {
-      const T* px = sA + pr * APITCH + 4 * g;
-      T x[3][4];
+      const double* px = sA + pr * APITCH + 4 * g;
+      double x[3][4];
       four(px, x[0]);
       four(px + 16 * APITCH, x[1]);
       four(px + 16 * APITCH + 16, x[2]);
       pin();
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        o[0] = Mma<T>::mma(x[0][r], c[0][r], o[0]);
-        o[1] = Mma<T>::mma(x[1][r], c[0][r], o[1]);
+        o[0] = mma64(x[0][r], c[0][r], o[0]);
+        o[1] = mma64(x[1][r], c[0][r], o[1]);
       }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) o[1] = Mma<T>::mma(x[2][r], c[1][r], o[1]);
+      for (int r = 0; r < 4; ++r) o[1] = mma64(x[2][r], c[1][r], o[1]);
     }
     if (m < kChunk) { weights(wt, p.scale_b, ld, m, after, g); lam = power(ld, (int64_t)m); }
 #pragma unroll
     for (int jt = 0; jt < 2; ++jt)
 #pragma unroll
       for (int r = 0; r < 4; ++r) c[jt][r] *= wt[jt][r];
-    add_tokens<T, DA>(S, sB, c, lam, pr, g);
-    if (live) {
-      T* q = po + (first + dir * at) * p.o_t;
-      if constexpr (FAST) {
-        const Chunk k = chunk_of(q, to, m, p.dc);
-        const uint32_t off = (uint32_t)((4 * g * (int)to + col) * (int)sizeof(T));
-#pragma unroll
-        for (int it = 0; it < 2; ++it)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) put(k, off + (k.first + (uint32_t)((16 * it + r) * (int)to * (int)sizeof(T))), o[it][r]);
-      } else {
-#pragma unroll
-        for (int it = 0; it < 2; ++it)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int i = 16 * it + 4 * g + r;
-            if (i < m) q[i * to + col] = o[it][r];
-          }
-      }
-    }
+    add_tokens64<DA>(S, sB, c, lam, pr, g);
+    if (live) put_o<double, acc64, FAST>(o, path.o + at * path.to, path.to, m, g, col, p.dc);
     // the next chunk into LDS: into the other buffer, or (where two do not fit) behind a barrier
     if constexpr (BUFS == 2) turn ^= 1;
     else __syncthreads();
-    if (next < total) {
-      a.store(bufs[turn][0], mn, p.da);
-      k.store(bufs[turn][1], mn, p.da);
-    }
+    if (next < path.total) stage(bufs[turn], path.tokens(next));
   }
-  if (live) {                                               // behind the sequence
-    for (int64_t t = (lo > n ? lo : n) + g; t < hi; t += 4) po[t * p.o_t + col] = (T)0;
-  }
+  if (live) zero_tail(p, path, g, col);
   if (p.s1 && w.segment == pl.segments - 1 && live) {
-    T* s1 = p.s1 + b * p.s1_b + h * p.s1_h + col * p.s1_c;
+    double* s1 = p.s1 + path.b * p.s1_b + path.h * p.s1_h + col * p.s1_c;
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -465,48 +479,40 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? WPE : 1) void chunks(Role<T> 
 }
 
 // The share of a part (of all segments but the last) in the state behind it, into the slot behind the part's own.
-template <typename T, int DA, bool BACK, bool FAST>
-__global__ __launch_bounds__(256) void segment_sums(Role<T> p, Plan<T> pl) {
-  typedef typename Mma<T>::acc_t acc_t;
-  typedef Tile<T, DA, FAST> tile_t;
-  constexpr int KT = DA / 16, PITCH = tile_t::PITCH;
+template <int DA, bool BACK, bool FAST>
+__global__ __launch_bounds__(256) void sums_f64(Role<double> p, Plan<double> pl) {
+  constexpr int KT = DA / 16, PITCH = DA + 2;
   constexpr int after = BACK ? 0 : 1;
-  __shared__ __attribute__((aligned(16))) T sB[2][kChunk * PITCH];
+  __shared__ __attribute__((aligned(16))) double sB[2][kChunk * PITCH];
   const Work w = work_of(pl, pl.slots - 1);
   if (!w.live) return;
-  const int64_t b = w.group / (int)p.heads;
-  const int h = (int)(w.group - b * p.heads);
-  const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63, g = lane >> 4, lr = lane & 15, pr = Mma<T>::row(lr);
-  const int col = w.slice * kCols + wave * 16 + lr;
+  const Path<double, BACK> path(p, w.group, w.segment * pl.part_tokens, pl.part_tokens);
+  const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63, g = lane >> 4, lr = lane & 15, pr = row64(lr);
+  const int col = w.slice * kCols64 + wave * 16 + lr;
   const bool live = col < p.dc;
-  const int64_t n = length_of(p, b);
-  const int64_t lo = w.segment * pl.part_tokens;
-  const int64_t end = lo + pl.part_tokens < n ? lo + pl.part_tokens : n;
-  const int64_t first = BACK ? n - 1 - lo : lo, dir = BACK ? -1 : 1;
-  const T* pb = p.b.p + b * p.b.b + (h / p.b.group) * p.b.h + first * p.b.t;
-  const T* pc = p.c.p + b * p.c.b + (h / p.c.group) * p.c.h + first * p.c.t;
   const int ccol = live ? col : p.dc - 1;
-  const int64_t tb = dir * p.b.t, tc = dir * p.c.t;
-  acc_t S[KT];
+  acc64 S[KT];
 #pragma unroll
-  for (int kt = 0; kt < KT; ++kt) S[kt] = (acc_t)((T)0);
-  const T ld = p.log_decay[h];
-  T wt[2][4];
+  for (int kt = 0; kt < KT; ++kt) S[kt] = (acc64)(0.0);
+  const double ld = p.log_decay[path.h];
+  double wt[2][4];
   weights(wt, p.scale_b, ld, kChunk, after, g);
-  T lam = power(ld, (int64_t)kChunk);
-  tile_t k;
-  T c[2][4], cn[2][4];
-  k.prepare(tb, p.da);
-  const int64_t total = end - lo;
-  if (total > 0) {
-    const int m = total < kChunk ? (int)total : kChunk;
-    k.load(pb, tb, m, p.da);
-    load_c<T, FAST>(cn, pc, tc, m, g, ccol, p.dc);
-  }
+  double lam = power(ld, (int64_t)kChunk);
+  Tile<double, DA, FAST> k;
+  double c[2][4], cn[2][4];
+  k.prepare(path.tk);
+  auto fetch = [&](int64_t at) {
+    const int m = path.tokens(at);
+    k.load(path.k + at * path.tk, path.tk, m, p.da);
+    load_c<double, FAST>(cn, path.c + at * path.tc, path.tc, m, g, ccol, p.dc);
+  };
+  if (path.total > 0) fetch(0);
   int turn = 0;
-  for (int64_t at = 0; at < total; at += kChunk, turn ^= 1) {
-    const int m = total - at < kChunk ? (int)(total - at) : kChunk;
-    k.store(sB[turn], m, p.da);                             // (two buffers: one barrier a chunk)
+  for (int64_t at = 0; at < path.total; at += kChunk, turn ^= 1) {
+    typedef double d2 __attribute__((ext_vector_type(2)));
+    const int m = path.tokens(at);
+    double* to = sB[turn];                                  // (two buffers: one barrier a chunk)
+    k.store(m, p.da, [&](int row, int cc, d2 v) { *(d2*)(to + row * PITCH + cc) = v; });
     if (m < kChunk) { weights(wt, p.scale_b, ld, m, after, g); lam = power(ld, (int64_t)m); }
     take(c, cn, m, g);
 #pragma unroll
@@ -514,16 +520,11 @@ __global__ __launch_bounds__(256) void segment_sums(Role<T> p, Plan<T> pl) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) c[jt][r] *= wt[jt][r];
     __syncthreads();
-    if (at + kChunk < total) {
-      const int64_t next = at + kChunk;
-      const int mn = total - next < kChunk ? (int)(total - next) : kChunk;
-      k.load(pb + next * tb, tb, mn, p.da);
-      load_c<T, FAST>(cn, pc + next * tc, tc, mn, g, ccol, p.dc);
-    }
-    add_tokens<T, DA>(S, sB[turn], c, lam, pr, g);
+    if (at + kChunk < path.total) fetch(at + kChunk);
+    add_tokens64<DA>(S, sB[turn], c, lam, pr, g);
   }
   if (!live) return;
-  T* s1 = pl.states + ((int64_t)w.group * pl.slots + w.segment + 1) * p.da * p.dc + col;
+  double* s1 = pl.states + ((int64_t)w.group * pl.slots + w.segment + 1) * p.da * p.dc + col;
 #pragma unroll
   for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -531,6 +532,335 @@ __global__ __launch_bounds__(256) void segment_sums(Role<T> p, Plan<T> pl) {
       const int d = 16 * kt + 4 * g + r;
       if (d < p.da) s1[(int64_t)d * p.dc] = S[kt][r];
     }
+}
+
+// ---- float32 ----
+// The 16 x 16 x 32 product of bfloat16: a lane brings eight k of row (column) lane % 16 and gets rows 4 g + i of the result,
+// g = lane / 16. Its k may be any eight as long as both operands agree:
+//   - over da: k = 32 m + 8 g + e. The rows of S's tiles are ordered to match: registers i of tiles 2 m and 2 m + 1 are rows
+//     32 m + 8 g + i and 32 m + 8 g + 4 + i, the eight that the lane needs when S is the right operand.
+//   - over the chunk's tokens: the four j = 4 g + e, then the four 16 + 4 g + e, which is how c is loaded and how a lane holds
+//     a transposed tile pair of A. b^T wants four tokens of one column there: the transposing LDS read gathers them from the
+//     row-major pieces of b (lane i of sixteen points at row i / 4, four columns i % 4; it gets column i of the 4 x 16 block).
+typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef float acc32 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// x = out[0] + out[1] + out[2] up to 2^-27 |x|, each rounded to nearest: the residues are exact. (A residue below the smallest
+// normal bfloat16 is lost: elements below 2^-108 keep 16 bits or fewer.)
+template <typename V, int N> __device__ __forceinline__ void split(const float (&x)[N], V (&out)[3]) {
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    f32x2 v = {x[i], x[i + 1]};
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+      const bf2 t = __builtin_convertvector(v, bf2);
+      out[q][i] = t[0];
+      out[q][i + 1] = t[1];
+      v -= __builtin_convertvector(t, f32x2);
+    }
+  }
+}
+
+// c + x y, the six pairs of pieces that count, small ones first
+__device__ __forceinline__ acc32 mma6(const bf8 (&x)[3], const bf8 (&y)[3], acc32 c) {
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[2], y[0], c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[0], y[2], c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[1], y[1], c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[1], y[0], c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[0], y[1], c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[0], y[0], c, 0, 0, 0);
+}
+
+// Pieces of 32 rows in LDS, rows padded by 16 bytes.
+template <int DA> struct Pieces {
+  static constexpr int PITCH = DA + 8;
+  __bf16 at[3][kChunk * PITCH];
+  template <bool FAST> __device__ __forceinline__ void fill(const Tile<float, DA, FAST>& t, int n, int da) {
+    t.store(n, da, [&](int row, int c, f32x4 v) {
+      const float x[4] = {v[0], v[1], v[2], v[3]};
+      bf4 q[3];
+      split(x, q);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) *(bf4*)(at[i] + row * PITCH + c) = q[i];
+    });
+  }
+  // eight neighbouring elements
+  __device__ __forceinline__ void row8(int row, int c, bf8 (&x)[3]) const {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) x[i] = *(const bf8*)(at[i] + row * PITCH + c);
+  }
+  // left operand of b^T's rows 32 m + 4 t + 8 (lr / 4) + lr % 4 over the chunk's tokens
+  __device__ __forceinline__ void tokens8(int m, int t, int g, int lr, bf8 (&x)[3]) const {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s4 lds4;
+    const int where = (4 * g + (lr >> 2)) * PITCH + 32 * m + 8 * (lr & 3) + 4 * t;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const bf4 lo = __builtin_bit_cast(bf4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(at[i] + where)));
+      const bf4 hi = __builtin_bit_cast(bf4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(at[i] + where + 16 * PITCH)));
+      x[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+};
+
+// S <- e^{g N} S + b^T (w c) of a wavefront's CT column tiles, c given weighted.
+template <int DA, int CT>
+__device__ __forceinline__ void add_tokens32(acc32 (&S)[CT][DA / 16], const Pieces<DA>& sB, const float (&wc)[CT][2][4], float lam, int g, int lr) {
+  bf8 x[2][3], y[CT][3];
+  sB.tokens8(0, 0, g, lr, x[0]);
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const float v[8] = {wc[ct][0][0], wc[ct][0][1], wc[ct][0][2], wc[ct][0][3], wc[ct][1][0], wc[ct][1][1], wc[ct][1][2], wc[ct][1][3]};
+    split(v, y[ct]);
+  }
+#pragma unroll
+  for (int kt = 0; kt < DA / 16; ++kt) {
+    if (kt + 1 < DA / 16) sB.tokens8((kt + 1) >> 1, (kt + 1) & 1, g, lr, x[(kt + 1) & 1]);
+    pin();
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) S[ct][kt] = mma6(x[kt & 1], y[ct], S[ct][kt] * lam);
+    pin();
+  }
+}
+
+template <int DA, int CT, bool BACK, bool FAST>
+__global__ __launch_bounds__(256, 2) void chunks_f32(Role<float> p, Plan<float> pl) {
+  constexpr int KT = DA / 16, APITCH = kChunk + 8;
+  constexpr int after = BACK ? 0 : 1;
+  __shared__ __attribute__((aligned(16))) Pieces<DA> sQ, sB;
+  __shared__ __attribute__((aligned(16))) __bf16 sA[3][kChunk * APITCH];
+  const Work w = work_of(pl, pl.segments);
+  if (!w.live) return;
+  const Path<float, BACK> path(p, w.group, w.segment * pl.seg_tokens, pl.seg_tokens);
+  const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63, g = lane >> 4, lr = lane & 15;
+  int col[CT], ccol[CT];
+  bool live[CT];
+  acc32 S[CT][KT];
+  const First<float> s0 = first_state(p, pl, w, path.b, path.h);
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    col[ct] = ((w.slice * 4 + wave) * CT + ct) * 16 + lr;
+    live[ct] = col[ct] < p.dc;
+    ccol[ct] = live[ct] ? col[ct] : p.dc - 1;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int d = 32 * (kt >> 1) + 8 * g + 4 * (kt & 1) + r;
+        S[ct][kt][r] = (s0.p && live[ct] && d < p.da) ? s0.p[d * s0.r + col[ct] * s0.c] : 0.0f;
+      }
+  }
+  const float ld = p.log_decay[path.h];
+  // reach: of rows 4 g + r of o, `half` times that of rows 16 + 4 g + r; keep: the weights of tokens 16 + 4 g + r, `half` times
+  // that of tokens 4 g + r
+  const int at_it = wave ? 1 : 0, at_jt = wave == 2 ? 1 : 0;  // this wavefront's tile of A: (0, 0), (1, 0), (1, 1); the fourth has none
+  float reach[4], mask[4], keep[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    reach[r] = p.scale_a * power(ld, (int64_t)(4 * g + r + after));
+    const int apart = 16 * (at_it - at_jt) + lr - 4 * g - r;
+    mask[r] = apart >= 0 ? p.scale_a * p.scale_b * power(ld, (int64_t)apart) : 0.0f;
+    keep[r] = p.scale_b * power(ld, (int64_t)(16 - after - 4 * g - r));
+  }
+  const float half = power(ld, (int64_t)16);
+  float lam = power(ld, (int64_t)kChunk);
+  // A's rows 0 .. 15 have no tokens 16 .. 31: zeros once
+  for (int i = (int)threadIdx.x; i < 3 * 16 * APITCH; i += 256) sA[i / (16 * APITCH)][i % (16 * APITCH)] = (__bf16)0.0f;
+
+  Tile<float, DA, FAST> a, k;
+  float c[CT][2][4];
+  a.prepare(path.ta);
+  k.prepare(path.tk);
+  auto fetch = [&](int64_t at) {
+    const int m = path.tokens(at);
+    a.load(path.a + at * path.ta, path.ta, m, p.da);
+    k.load(path.k + at * path.tk, path.tk, m, p.da);
+  };
+  if (path.total > 0) fetch(0);
+  for (int64_t at = 0; at < path.total; at += kChunk) {
+    const int64_t next = at + kChunk;
+    const int m = path.tokens(at);
+    __syncthreads();                                        // the chunk before has been read
+    sQ.fill(a, m, p.da);
+    sB.fill(k, m, p.da);
+    // (c is wanted behind the next barrier but one, far enough away for its loads)
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) load_c<float, FAST>(c[ct], path.c + at * path.tc, path.tc, m, g, ccol[ct], p.dc);
+    __syncthreads();
+    if (wave < 3) {                                         // a tile of A, transposed
+      const int it = at_it, jt = at_jt;
+      acc32 t = (acc32)(0.0f);
+      bf8 x[2][3], y[2][3];
+      sB.row8(16 * jt + lr, 8 * g, x[0]);
+      sQ.row8(16 * it + lr, 8 * g, y[0]);
+#pragma unroll
+      for (int kt = 0; kt < DA / 32; ++kt) {
+        if (kt + 1 < DA / 32) {
+          sB.row8(16 * jt + lr, 32 * (kt + 1) + 8 * g, x[(kt + 1) & 1]);
+          sQ.row8(16 * it + lr, 32 * (kt + 1) + 8 * g, y[(kt + 1) & 1]);
+        }
+        pin();
+        t = mma6(x[kt & 1], y[kt & 1], t);
+        pin();
+      }
+      float v[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const bool under = it > jt || lr >= 4 * g + r;      // a choice, not a product with 0: the term above may be a NaN
+        v[r] = under ? t[r] * mask[r] : 0.0f;
+      }
+      bf4 q[3];
+      split(v, q);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) *(bf4*)(sA[i] + (16 * it + lr) * APITCH + 8 * g + 4 * jt) = q[i];
+    }
+    acc32 o[CT][2];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) o[ct][0] = o[ct][1] = (acc32)(0.0f);
+#pragma unroll
+    for (int kt = 0; kt < DA / 32; ++kt) {
+      bf8 x[2][3];
+      sQ.row8(lr, 32 * kt + 8 * g, x[0]);
+      sQ.row8(16 + lr, 32 * kt + 8 * g, x[1]);
+      pin();                                                // (the reads arrive while S is split)
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        const float v[8] = {S[ct][2 * kt][0], S[ct][2 * kt][1], S[ct][2 * kt][2], S[ct][2 * kt][3],
+                            S[ct][2 * kt + 1][0], S[ct][2 * kt + 1][1], S[ct][2 * kt + 1][2], S[ct][2 * kt + 1][3]};
+        bf8 y[3];
+        split(v, y);
+        o[ct][0] = mma6(x[0], y, o[ct][0]);
+        o[ct][1] = mma6(x[1], y, o[ct][1]);
+      }
+    }
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (int it = 0; it < 2; ++it)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[ct][it][r] *= it ? reach[r] * half : reach[r];
+    if (next < path.total) fetch(next);
+    __syncthreads();
+    {
+      bf8 x[2][3];
+#pragma unroll
+      for (int it = 0; it < 2; ++it)
+#pragma unroll
+        for (int i = 0; i < 3; ++i) x[it][i] = *(const bf8*)(sA[i] + (16 * it + lr) * APITCH + 8 * g);
+      pin();
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        take(c[ct], c[ct], m, g);
+        const float v[8] = {c[ct][0][0], c[ct][0][1], c[ct][0][2], c[ct][0][3], c[ct][1][0], c[ct][1][1], c[ct][1][2], c[ct][1][3]};
+        bf8 y[3];
+        split(v, y);
+        o[ct][0] = mma6(x[0], y, o[ct][0]);
+        o[ct][1] = mma6(x[1], y, o[ct][1]);
+      }
+    }
+    float wt[2][4];
+    if (m < kChunk) {
+      weights(wt, p.scale_b, ld, m, after, g);
+      lam = power(ld, (int64_t)m);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) { wt[1][r] = keep[r]; wt[0][r] = keep[r] * half; }
+    }
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      if (live[ct]) put_o<float, acc32, FAST>(o[ct], path.o + at * path.to, path.to, m, g, col[ct], p.dc);
+#pragma unroll
+      for (int jt = 0; jt < 2; ++jt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) c[ct][jt][r] *= wt[jt][r];
+    }
+    add_tokens32<DA, CT>(S, sB, c, lam, g, lr);
+  }
+  // (the compiler would keep every row's offset from the loads of the first state to here, in registers the loop needs)
+  int ge = g;
+  asm volatile("" : "+v"(ge));
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    if (!live[ct]) continue;
+    zero_tail(p, path, g, col[ct]);
+    if (p.s1 && w.segment == pl.segments - 1) {
+      float* s1 = p.s1 + path.b * p.s1_b + path.h * p.s1_h + col[ct] * p.s1_c;
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int d = 32 * (kt >> 1) + 8 * ge + 4 * (kt & 1) + r;
+          if (d < p.da) s1[d * p.s1_r] = S[ct][kt][r];
+        }
+    }
+  }
+}
+
+template <int DA, int CT, bool BACK, bool FAST>
+__global__ __launch_bounds__(256, 2) void sums_f32(Role<float> p, Plan<float> pl) {
+  constexpr int KT = DA / 16;
+  constexpr int after = BACK ? 0 : 1;
+  __shared__ __attribute__((aligned(16))) Pieces<DA> sB[2];
+  const Work w = work_of(pl, pl.slots - 1);
+  if (!w.live) return;
+  const Path<float, BACK> path(p, w.group, w.segment * pl.part_tokens, pl.part_tokens);
+  const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63, g = lane >> 4, lr = lane & 15;
+  int col[CT], ccol[CT];
+  acc32 S[CT][KT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    col[ct] = ((w.slice * 4 + wave) * CT + ct) * 16 + lr;
+    ccol[ct] = col[ct] < p.dc ? col[ct] : p.dc - 1;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) S[ct][kt] = (acc32)(0.0f);
+  }
+  const float ld = p.log_decay[path.h];
+  float wt[2][4];
+  weights(wt, p.scale_b, ld, kChunk, after, g);
+  float lam = power(ld, (int64_t)kChunk);
+  Tile<float, DA, FAST> k;
+  float c[CT][2][4], cn[CT][2][4];
+  k.prepare(path.tk);
+  auto fetch = [&](int64_t at) {
+    const int m = path.tokens(at);
+    k.load(path.k + at * path.tk, path.tk, m, p.da);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) load_c<float, FAST>(cn[ct], path.c + at * path.tc, path.tc, m, g, ccol[ct], p.dc);
+  };
+  if (path.total > 0) fetch(0);
+  int turn = 0;
+  for (int64_t at = 0; at < path.total; at += kChunk, turn ^= 1) {
+    const int m = path.tokens(at);
+    sB[turn].fill(k, m, p.da);                              // (two buffers: one barrier a chunk)
+    if (m < kChunk) { weights(wt, p.scale_b, ld, m, after, g); lam = power(ld, (int64_t)m); }
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      take(c[ct], cn[ct], m, g);
+#pragma unroll
+      for (int jt = 0; jt < 2; ++jt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) c[ct][jt][r] *= wt[jt][r];
+    }
+    __syncthreads();
+    if (at + kChunk < path.total) fetch(at + kChunk);
+    add_tokens32<DA, CT>(S, sB[turn], c, lam, g, lr);
+  }
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    if (col[ct] >= p.dc) continue;
+    float* s1 = pl.states + ((int64_t)w.group * pl.slots + w.segment + 1) * p.da * p.dc + col[ct];
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int d = 32 * (kt >> 1) + 8 * g + 4 * (kt & 1) + r;
+        if (d < p.da) s1[(int64_t)d * p.dc] = S[ct][kt][r];
+      }
+  }
 }
 
 // From the parts' shares to the states in front of the segments (the slots at multiples of `parts`): one lane per element of
@@ -579,21 +909,20 @@ static int workgroups_per_cu(const void* kernel) {
   return n;
 }
 
-#ifndef MINSEG
-#define MINSEG 2
-#endif
-template <typename T, int DA, bool BACK, bool FAST>
-static int run_chunks(const Role<T>& p) {
+template <typename T> using Kernel = void (*)(Role<T>, Plan<T>);
+
+// cols: columns of a workgroup
+template <typename T, Kernel<T> CHUNKS, Kernel<T> SUMS>
+static int run_chunks(const Role<T>& p, int cols) {
   Plan<T> pl = {};
-  pl.slices = (p.dc + kCols - 1) / kCols;
+  pl.slices = (p.dc + cols - 1) / cols;
   pl.groups = (int)(p.batch * p.heads);
-  pl.segments = 1;
   const int64_t wgs = (int64_t)pl.groups * pl.slices;
   const int64_t n_chunks = (p.tokens + kChunk - 1) / kChunk;
-  // As many segments as the device has room for workgroups, of MINSEG chunks at least.
-  static const int room = workgroups_per_cu((const void*)chunks<T, DA, BACK, FAST>), sums_room = workgroups_per_cu((const void*)segment_sums<T, DA, BACK, FAST>);
+  // As many segments as the device has room for workgroups, of two chunks at least.
+  static const int room = workgroups_per_cu((const void*)CHUNKS), sums_room = workgroups_per_cu((const void*)SUMS);
   int64_t segments = (int64_t)room * num_cus() / wgs;
-  if (segments > n_chunks / MINSEG) segments = n_chunks / MINSEG;
+  if (segments > n_chunks / 2) segments = n_chunks / 2;
   if (segments < 1) segments = 1;
   int64_t per_segment = n_chunks ? (n_chunks + segments - 1) / segments : 1;
   int64_t parts = 1;
@@ -614,33 +943,41 @@ static int run_chunks(const Role<T>& p) {
     AM_TRY(states.take((size_t)pl.groups * pl.slots * p.da * p.dc * sizeof(T)));
     pl.states = (T*)states.p;
     const int64_t ids = ((int64_t)pl.groups * (pl.slots - 1) + 7) / 8 * 8 * pl.slices;
-    hipLaunchKernelGGL((segment_sums<T, DA, BACK, FAST>), dim3((unsigned)ids), dim3(256), 0, stream(), p, pl);
-    AM_TRY(check_launch("segment_sums"));
+    hipLaunchKernelGGL(SUMS, dim3((unsigned)ids), dim3(256), 0, stream(), p, pl);
+    AM_TRY(check_launch("decay attention: sums"));
     hipLaunchKernelGGL((segment_states<T>), dim3((unsigned)(pl.groups * ((p.da * p.dc + 255) / 256))), dim3(256), 0, stream(), p, pl);
-    AM_TRY(check_launch("segment_states"));
+    AM_TRY(check_launch("decay attention: states"));
   }
   const int64_t ids = ((int64_t)pl.groups * pl.segments + 7) / 8 * 8 * pl.slices;
-  hipLaunchKernelGGL((chunks<T, DA, BACK, FAST>), dim3((unsigned)ids), dim3(256), 0, stream(), p, pl);
-  return check_launch("chunks");
+  hipLaunchKernelGGL(CHUNKS, dim3((unsigned)ids), dim3(256), 0, stream(), p, pl);
+  return check_launch("decay attention: chunks");
 }
 
-template <typename T, int DA, bool BACK>
-static int run_sized(const Role<T>& p) {
-  // FAST: rows of whole vectors, and 32 tokens of every operand within 2^31 bytes
-  const int64_t most = ((int64_t)1 << 31) / (kChunk * (int64_t)sizeof(T)) - kMostDim;
-  auto near = [&](int64_t t) { return t < most && -t < most; };
-  const bool fast = p.da % (16 / (int)sizeof(T)) == 0 && near(p.a.t) && near(p.b.t) && near(p.c.t) && near(p.o_t);
-  return fast ? run_chunks<T, DA, BACK, true>(p) : run_chunks<T, DA, BACK, false>(p);
+template <int DA, bool BACK, bool FAST> static int run_sized(const Role<double>& p) {
+  return run_chunks<double, chunks_f64<DA, BACK, FAST>, sums_f64<DA, BACK, FAST>>(p, kCols64);
+}
+// Up to 64 columns a wavefront takes one tile of 16, else two: b's and a's pieces are then read from LDS once for both.
+template <int DA, bool BACK, bool FAST> static int run_sized(const Role<float>& p) {
+  if (p.dc <= 64) return run_chunks<float, chunks_f32<DA, 1, BACK, FAST>, sums_f32<DA, 1, BACK, FAST>>(p, 64);
+  return run_chunks<float, chunks_f32<DA, 2, BACK, FAST>, sums_f32<DA, 2, BACK, FAST>>(p, 128);
+}
+
+template <bool BACK, bool FAST, typename T> static int run_fast(const Role<T>& p) {
+  if (p.da <= 32) return run_sized<32, BACK, FAST>(p);
+  if (p.da <= 64) return run_sized<64, BACK, FAST>(p);
+  if (p.da <= 96) return run_sized<96, BACK, FAST>(p);
+  if (p.da <= 128) return run_sized<128, BACK, FAST>(p);
+  if (p.da <= 192) return run_sized<192, BACK, FAST>(p);
+  return run_sized<256, BACK, FAST>(p);
 }
 
 template <typename T, bool BACK>
 static int run_role(const Role<T>& p) {
-  if (p.da <= 32) return run_sized<T, 32, BACK>(p);
-  if (p.da <= 64) return run_sized<T, 64, BACK>(p);
-  if (p.da <= 96) return run_sized<T, 96, BACK>(p);
-  if (p.da <= 128) return run_sized<T, 128, BACK>(p);
-  if (p.da <= 192) return run_sized<T, 192, BACK>(p);
-  return run_sized<T, 256, BACK>(p);
+  // FAST: rows of whole vectors, and 32 tokens of every operand within 2^31 bytes
+  const int64_t most = ((int64_t)1 << 31) / (kChunk * (int64_t)sizeof(T)) - kMostDim;
+  auto near = [&](int64_t t) { return t < most && -t < most; };
+  const bool fast = p.da % (16 / (int)sizeof(T)) == 0 && near(p.a.t) && near(p.b.t) && near(p.c.t) && near(p.o_t);
+  return fast ? run_fast<BACK, true>(p) : run_fast<BACK, false>(p);
 }
 
 // One token: the state is read and written once. A workgroup takes one head's state in rows of 16-byte vectors: `lanes`
