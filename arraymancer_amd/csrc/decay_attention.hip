@@ -70,7 +70,8 @@ constexpr int kChunk = 32;
 constexpr int kLds = 160 * 1024;
 
 template <typename T> struct Plan {
-  T* states;                   // [batch * heads][slots][da][dc]: the state in front of each part; null: one segment
+  T* states;                   // [batch * heads][slots][da * dc]: the state in front of each part; null: one segment
+  int st_r, st_c;              // strides of a state's rows and columns there
   int segments, slices;
   int parts, slots;            // parts of a segment; slots = parts * (segments - 1) + 1, one in front of every part but the last segment's later ones
   int64_t seg_tokens, part_tokens;   // multiples of kChunk, seg_tokens = parts * part_tokens
@@ -298,7 +299,7 @@ __device__ __forceinline__ void row_factors(T (&reach)[2][4], T (&mask)[2][4], c
 // Where the first state of a segment is read, and its strides.
 template <typename T> struct First { const T* p; int64_t r, c; };
 template <typename T> __device__ __forceinline__ First<T> first_state(const Role<T>& p, const Plan<T>& pl, const Work& w, int64_t b, int h) {
-  if (pl.states) return {pl.states + ((int64_t)w.group * pl.slots + w.segment * pl.parts) * p.da * p.dc, p.dc, 1};
+  if (pl.states) return {pl.states + ((int64_t)w.group * pl.slots + w.segment * pl.parts) * p.da * p.dc, pl.st_r, pl.st_c};
   return {p.s0 ? p.s0 + b * p.s0_b + h * p.s0_h : nullptr, p.s0_r, p.s0_c};
 }
 
@@ -867,18 +868,18 @@ __global__ __launch_bounds__(256, 2) void sums_f32(Role<float> p, Plan<float> pl
 // a head's state, BATCH slots on their way at a time (no load may pass the stores of the batch before).
 template <typename T, int BATCH>
 __device__ __forceinline__ void carry(T* at, int64_t per, int& k, T& s, T ld, int64_t n, const Plan<T>& pl) {
-  for (; k + BATCH <= pl.slots; k += BATCH) {
-    T v[BATCH];
+  T v[BATCH];
 #pragma unroll
-    for (int u = 0; u < BATCH; ++u) v[u] = at[(int64_t)(k + u) * per];
+  for (int u = 0; u < BATCH; ++u) v[u] = at[(int64_t)(k + u < pl.slots ? k + u : pl.slots - 1) * per];
 #pragma unroll
-    for (int u = 0; u < BATCH; ++u) {
-      int64_t len = n - (k + u - 1) * pl.part_tokens;
-      len = len < 0 ? 0 : (len < pl.part_tokens ? len : pl.part_tokens);
-      s = s * power(ld, len) + v[u];
-      if ((k + u) % pl.parts == 0) at[(int64_t)(k + u) * per] = s;
-    }
+  for (int u = 0; u < BATCH; ++u) {
+    if (k + u >= pl.slots) break;
+    int64_t len = n - (k + u - 1) * pl.part_tokens;
+    len = len < 0 ? 0 : (len < pl.part_tokens ? len : pl.part_tokens);
+    s = s * power(ld, len) + v[u];
+    if ((k + u) % pl.parts == 0) at[(int64_t)(k + u) * per] = s;
   }
+  k += BATCH;
 }
 
 template <typename T>
@@ -897,10 +898,8 @@ __global__ __launch_bounds__(256) void segment_states(Role<T> p, Plan<T> pl) {
   T s = p.s0 ? p.s0[b * p.s0_b + h * p.s0_h + r * p.s0_r + c * p.s0_c] : (T)0;
   at[0] = s;
   int k = 1;
-  carry<T, 32>(at, per, k, s, ld, n, pl);
-  carry<T, 8>(at, per, k, s, ld, n, pl);
-  carry<T, 2>(at, per, k, s, ld, n, pl);
-  carry<T, 1>(at, per, k, s, ld, n, pl);
+  while (k + 24 < pl.slots) carry<T, 32>(at, per, k, s, ld, n, pl);
+  while (k < pl.slots) carry<T, 8>(at, per, k, s, ld, n, pl);
 }
 
 static int workgroups_per_cu(const void* kernel) {
@@ -911,73 +910,89 @@ static int workgroups_per_cu(const void* kernel) {
 
 template <typename T> using Kernel = void (*)(Role<T>, Plan<T>);
 
+// The states in front of the segments of one walk. The two backward roles of a backward pass walk the same keys and values
+// with their parts exchanged, so the second reads the first's states transposed.
+template <typename T> struct Segments {
+  Plan<T> plan = {};
+  Scratch states;
+  bool made = false;
+};
+
 // cols: columns of a workgroup
 template <typename T, Kernel<T> CHUNKS, Kernel<T> SUMS>
-static int run_chunks(const Role<T>& p, int cols) {
-  Plan<T> pl = {};
+static int run_chunks(const Role<T>& p, Segments<T>& seg, int cols) {
+  Plan<T>& pl = seg.plan;
   pl.slices = (p.dc + cols - 1) / cols;
-  pl.groups = (int)(p.batch * p.heads);
-  const int64_t wgs = (int64_t)pl.groups * pl.slices;
-  const int64_t n_chunks = (p.tokens + kChunk - 1) / kChunk;
-  // As many segments as the device has room for workgroups, of two chunks at least.
-  static const int room = workgroups_per_cu((const void*)CHUNKS), sums_room = workgroups_per_cu((const void*)SUMS);
-  int64_t segments = (int64_t)room * num_cus() / wgs;
-  if (segments > n_chunks / 2) segments = n_chunks / 2;
-  if (segments < 1) segments = 1;
-  int64_t per_segment = n_chunks ? (n_chunks + segments - 1) / segments : 1;
-  int64_t parts = 1;
-  if (segments > 1) {
-    // the sums run in parts of a segment, so that they too fill the device
-    parts = (int64_t)sums_room * num_cus() / (wgs * (segments - 1));
-    if (parts > per_segment / 2) parts = per_segment / 2;
-    if (parts < 1) parts = 1;
-    per_segment = (per_segment + parts - 1) / parts * parts;
-  }
-  pl.parts = (int)parts;
-  pl.part_tokens = per_segment / parts * kChunk;
-  pl.seg_tokens = per_segment * kChunk;
-  pl.segments = (int)(n_chunks ? (n_chunks + per_segment - 1) / per_segment : 1);
-  pl.slots = pl.parts * (pl.segments - 1) + 1;
-  Scratch states;
-  if (pl.segments > 1) {
-    AM_TRY(states.take((size_t)pl.groups * pl.slots * p.da * p.dc * sizeof(T)));
-    pl.states = (T*)states.p;
-    const int64_t ids = ((int64_t)pl.groups * (pl.slots - 1) + 7) / 8 * 8 * pl.slices;
-    hipLaunchKernelGGL(SUMS, dim3((unsigned)ids), dim3(256), 0, stream(), p, pl);
-    AM_TRY(check_launch("decay attention: sums"));
-    hipLaunchKernelGGL((segment_states<T>), dim3((unsigned)(pl.groups * ((p.da * p.dc + 255) / 256))), dim3(256), 0, stream(), p, pl);
-    AM_TRY(check_launch("decay attention: states"));
+  if (seg.made) {
+    pl.st_r = 1; pl.st_c = p.da;
+  } else {
+    pl.groups = (int)(p.batch * p.heads);
+    pl.st_r = p.dc; pl.st_c = 1;
+    const int64_t wgs = (int64_t)pl.groups * pl.slices;
+    const int64_t n_chunks = (p.tokens + kChunk - 1) / kChunk;
+    // As many segments as the device has room for workgroups, of two chunks at least.
+    static const int room = workgroups_per_cu((const void*)CHUNKS), sums_room = workgroups_per_cu((const void*)SUMS);
+    int64_t segments = (int64_t)room * num_cus() / wgs;
+    if (segments > n_chunks / 2) segments = n_chunks / 2;
+    if (segments < 1) segments = 1;
+    int64_t per_segment = n_chunks ? (n_chunks + segments - 1) / segments : 1;
+    int64_t parts = 1;
+    if (segments > 1) {
+      // the sums run in parts of a segment, so that they too fill the device
+      parts = (int64_t)sums_room * num_cus() / (wgs * (segments - 1));
+      if (parts > per_segment / 2) parts = per_segment / 2;
+      if (parts < 1) parts = 1;
+      per_segment = (per_segment + parts - 1) / parts * parts;
+    }
+    pl.parts = (int)parts;
+    pl.part_tokens = per_segment / parts * kChunk;
+    pl.seg_tokens = per_segment * kChunk;
+    pl.segments = (int)(n_chunks ? (n_chunks + per_segment - 1) / per_segment : 1);
+    pl.slots = pl.parts * (pl.segments - 1) + 1;
+    if (pl.segments > 1) {
+      AM_TRY(seg.states.take((size_t)pl.groups * pl.slots * p.da * p.dc * sizeof(T)));
+      pl.states = (T*)seg.states.p;
+      const int64_t ids = ((int64_t)pl.groups * (pl.slots - 1) + 7) / 8 * 8 * pl.slices;
+      hipLaunchKernelGGL(SUMS, dim3((unsigned)ids), dim3(256), 0, stream(), p, pl);
+      AM_TRY(check_launch("decay attention: sums"));
+      hipLaunchKernelGGL((segment_states<T>), dim3((unsigned)(pl.groups * ((p.da * p.dc + 255) / 256))), dim3(256), 0, stream(), p, pl);
+      AM_TRY(check_launch("decay attention: states"));
+    }
+    seg.made = true;
   }
   const int64_t ids = ((int64_t)pl.groups * pl.segments + 7) / 8 * 8 * pl.slices;
   hipLaunchKernelGGL(CHUNKS, dim3((unsigned)ids), dim3(256), 0, stream(), p, pl);
   return check_launch("decay attention: chunks");
 }
 
-template <int DA, bool BACK, bool FAST> static int run_sized(const Role<double>& p) {
-  return run_chunks<double, chunks_f64<DA, BACK, FAST>, sums_f64<DA, BACK, FAST>>(p, kCols64);
+template <int DA, bool BACK, bool FAST> static int run_sized(const Role<double>& p, Segments<double>& seg) {
+  return run_chunks<double, chunks_f64<DA, BACK, FAST>, sums_f64<DA, BACK, FAST>>(p, seg, kCols64);
 }
-// Up to 64 columns a wavefront takes one tile of 16, else two: b's and a's pieces are then read from LDS once for both.
-template <int DA, bool BACK, bool FAST> static int run_sized(const Role<float>& p) {
-  if (p.dc <= 64) return run_chunks<float, chunks_f32<DA, 1, BACK, FAST>, sums_f32<DA, 1, BACK, FAST>>(p, 64);
-  return run_chunks<float, chunks_f32<DA, 2, BACK, FAST>, sums_f32<DA, 2, BACK, FAST>>(p, 128);
+// A wavefront takes two tiles of 16 columns where there are more than 64 (a's and b's pieces are then read from LDS once for
+// both), unless the workgroups of 128 columns leave CUs without work however short their segments.
+template <int DA, bool BACK, bool FAST> static int run_sized(const Role<float>& p, Segments<float>& seg) {
+  const int64_t pairs = (p.tokens + 2 * kChunk - 1) / (2 * kChunk);
+  const bool wide = p.dc > 64 && p.batch * p.heads * ((p.dc + 127) / 128) * (pairs > 1 ? pairs : 1) >= num_cus();
+  if (!wide) return run_chunks<float, chunks_f32<DA, 1, BACK, FAST>, sums_f32<DA, 1, BACK, FAST>>(p, seg, 64);
+  return run_chunks<float, chunks_f32<DA, 2, BACK, FAST>, sums_f32<DA, 2, BACK, FAST>>(p, seg, 128);
 }
 
-template <bool BACK, bool FAST, typename T> static int run_fast(const Role<T>& p) {
-  if (p.da <= 32) return run_sized<32, BACK, FAST>(p);
-  if (p.da <= 64) return run_sized<64, BACK, FAST>(p);
-  if (p.da <= 96) return run_sized<96, BACK, FAST>(p);
-  if (p.da <= 128) return run_sized<128, BACK, FAST>(p);
-  if (p.da <= 192) return run_sized<192, BACK, FAST>(p);
-  return run_sized<256, BACK, FAST>(p);
+template <bool BACK, bool FAST, typename T> static int run_fast(const Role<T>& p, Segments<T>& seg) {
+  if (p.da <= 32) return run_sized<32, BACK, FAST>(p, seg);
+  if (p.da <= 64) return run_sized<64, BACK, FAST>(p, seg);
+  if (p.da <= 96) return run_sized<96, BACK, FAST>(p, seg);
+  if (p.da <= 128) return run_sized<128, BACK, FAST>(p, seg);
+  if (p.da <= 192) return run_sized<192, BACK, FAST>(p, seg);
+  return run_sized<256, BACK, FAST>(p, seg);
 }
 
 template <typename T, bool BACK>
-static int run_role(const Role<T>& p) {
+static int run_role(const Role<T>& p, Segments<T>& seg) {
   // FAST: rows of whole vectors, and 32 tokens of every operand within 2^31 bytes
   const int64_t most = ((int64_t)1 << 31) / (kChunk * (int64_t)sizeof(T)) - kMostDim;
   auto near = [&](int64_t t) { return t < most && -t < most; };
   const bool fast = p.da % (16 / (int)sizeof(T)) == 0 && near(p.a.t) && near(p.b.t) && near(p.c.t) && near(p.o_t);
-  return fast ? run_fast<BACK, true>(p) : run_fast<BACK, false>(p);
+  return fast ? run_fast<BACK, true>(p, seg) : run_fast<BACK, false>(p, seg);
 }
 
 // One token: the state is read and written once. A workgroup takes one head's state in rows of 16-byte vectors: `lanes`
@@ -1069,7 +1084,8 @@ static int forward(const char* fn, int64_t batch, int64_t tokens, int64_t heads,
   p.da = (int)dk; p.dc = (int)dv;
   p.log_decay = log_decay; p.lengths = lengths;
   p.batch = batch; p.tokens = tokens; p.heads = heads;
-  return run_role<T, false>(p);
+  Segments<T> seg;
+  return run_role<T, false>(p, seg);
 }
 
 // out[b, t, head, :] = the sum of the `group` heads' shares that follow each other, in the heads' order
@@ -1125,11 +1141,15 @@ static int backward(const char* fn, int64_t batch, int64_t tokens, int64_t heads
   p.s0 = s0; p.s0_b = s0_b; p.s0_h = s0_h; p.s0_r = 1; p.s0_c = dv;
   p.scale_a = scale; p.scale_b = (T)1;
   p.da = (int)dv; p.dc = (int)dk;
-  AM_TRY((run_role<T, false>(p)));
+  {
+    Segments<T> seg;
+    AM_TRY((run_role<T, false>(p, seg)));
+  }
   // dk and dv: backwards. Where heads share a key / value head each writes its own share, and `fold_heads` adds them up.
   // dk first: dv's walk writes the first state's gradient, which may lie over the last state's.
   p.scale_a = (T)1; p.scale_b = scale;
   p.s0 = gs; p.s0_b = gs_b; p.s0_h = gs_h;
+  Segments<T> seg;
   Scratch shares;
   if (group > 1 && tokens) AM_TRY(shares.take((size_t)batch * tokens * heads * (dk > dv ? dk : dv) * sizeof(T)));
   auto into = [&](const Result<T>& r, int64_t d) {
@@ -1140,14 +1160,14 @@ static int backward(const char* fn, int64_t batch, int64_t tokens, int64_t heads
   into(dkey, dk);
   p.s0_r = 1; p.s0_c = dv;
   p.da = (int)dv; p.dc = (int)dk;
-  AM_TRY((run_role<T, true>(p)));
+  AM_TRY((run_role<T, true>(p, seg)));
   if (group > 1) AM_TRY(fold_heads((const T*)shares.p, dkey, batch, tokens, kv_heads, group, (int)dk));
   p.a = K; p.b = Q; p.c = G;
   into(dval, dv);
   p.s0_r = dv; p.s0_c = 1;
   p.s1 = gs0; p.s1_b = gs0_b; p.s1_h = gs0_h; p.s1_r = dv; p.s1_c = 1;
   p.da = (int)dk; p.dc = (int)dv;
-  AM_TRY((run_role<T, true>(p)));
+  AM_TRY((run_role<T, true>(p, seg)));
   if (group > 1) AM_TRY(fold_heads((const T*)shares.p, dval, batch, tokens, kv_heads, group, (int)dv));
   return AM_OK;
 }
