@@ -576,9 +576,10 @@ __device__ __forceinline__ acc32 mma6(const bf8 (&x)[3], const bf8 (&y)[3], acc3
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[0], y[0], c, 0, 0, 0);
 }
 
-// Pieces of 32 rows in LDS, rows padded by 16 bytes.
+// Pieces of 32 rows in LDS, rows padded by 32 bytes (against 16 the transposing reads conflict more: 238 -> 227 us for the
+// gradients of 4 x 2048 tokens, 16 heads of 64 x 128).
 template <int DA> struct Pieces {
-  static constexpr int PITCH = DA + 8;
+  static constexpr int PITCH = DA + 16;
   __bf16 at[3][kChunk * PITCH];
   template <bool FAST> __device__ __forceinline__ void fill(const Tile<float, DA, FAST>& t, int n, int da) {
     t.store(n, da, [&](int row, int c, f32x4 v) {
