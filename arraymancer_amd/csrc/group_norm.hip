@@ -72,6 +72,12 @@ template <typename T, int ACT> __device__ __forceinline__ T through(T dy, T z) {
   } else return dy;
 }
 
+// NT: past the caches, for the last reading of a tensor larger than they keep.
+template <bool NT, typename V> __device__ __forceinline__ V fetch(const V* p) {
+  if constexpr (NT) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+
 template <typename T, int V> struct Vec { typedef T type __attribute__((ext_vector_type(V))); };
 
 // Sum over the lanes of a team: butterflies within a wavefront, then (WIDE: the team is the workgroup of four) through LDS.
@@ -115,7 +121,7 @@ template <typename T, int V, int U, bool WIDE> struct Team {
   }
 };
 
-template <typename T, int V, int U, bool WIDE, int ACT>
+template <typename T, int V, int U, bool WIDE, int ACT, bool NT>
 __global__ __launch_bounds__(256) void team_forward(Args<T> p, int lanes, int units, int64_t slots) {
   typedef typename Vec<T, V>::type vec_t;
   __shared__ T lds[4];
@@ -135,7 +141,7 @@ __global__ __launch_bounds__(256) void team_forward(Args<T> p, int lanes, int un
     const T* x = p.x + n * p.x_n + c0;
     vec_t v[U];
 #pragma unroll
-    for (int k = 0; k < U; ++k) v[k] = *(const vec_t*)(x + t.row[k] * p.x_s + t.col[k]);
+    for (int k = 0; k < U; ++k) v[k] = fetch<NT>((const vec_t*)(x + t.row[k] * p.x_s + t.col[k]));
     T sum = (T)0;
 #pragma unroll
     for (int k = 0; k < U; ++k)
@@ -163,7 +169,7 @@ __global__ __launch_bounds__(256) void team_forward(Args<T> p, int lanes, int un
   }
 }
 
-template <typename T, int V, int U, bool WIDE, int ACT>
+template <typename T, int V, int U, bool WIDE, int ACT, bool NT>
 __global__ __launch_bounds__(256) void team_backward(Args<T> p, int lanes, int units, int64_t slots) {
   typedef typename Vec<T, V>::type vec_t;
   __shared__ T lds[4];
@@ -187,8 +193,8 @@ __global__ __launch_bounds__(256) void team_backward(Args<T> p, int lanes, int u
     vec_t h[U], d[U];     // xhat and weight * dz
 #pragma unroll
     for (int k = 0; k < U; ++k) {
-      h[k] = *(const vec_t*)(x + t.row[k] * p.x_s + t.col[k]);
-      d[k] = *(const vec_t*)(dy + t.row[k] * p.dy_s + t.col[k]);
+      h[k] = fetch<NT>((const vec_t*)(x + t.row[k] * p.x_s + t.col[k]));
+      d[k] = fetch<NT>((const vec_t*)(dy + t.row[k] * p.dy_s + t.col[k]));
     }
     T s1 = (T)0, s2 = (T)0;
 #pragma unroll
@@ -463,7 +469,7 @@ __global__ __launch_bounds__(256) void channel_fold(Args<T> p, const P* part, in
 }
 
 // Second pass over the slabs: y from mean and rstd, or (BWD) dx from the averages too.
-template <typename T, int V, bool BWD, int ACT>
+template <typename T, int V, bool BWD, int ACT, bool NT>
 __global__ __launch_bounds__(256) void slab_apply(Args<T> p) {
   typedef typename Vec<T, V>::type vec_t;
   const Place w = place<T, V>(p);
@@ -482,10 +488,10 @@ __global__ __launch_bounds__(256) void slab_apply(Args<T> p) {
   const int64_t hi = lo + p.rows_per_slab < p.spatial ? lo + p.rows_per_slab : p.spatial;
 #pragma unroll 4
   for (int64_t s = lo + w.row0; s < hi; s += p.rows_at_once) {
-    const vec_t xv = *(const vec_t*)(p.x + w.n * p.x_n + s * p.x_s + w.c);
+    const vec_t xv = fetch<NT>((const vec_t*)(p.x + w.n * p.x_n + s * p.x_s + w.c));
     vec_t out;
     if constexpr (BWD) {
-      const vec_t dv = *(const vec_t*)(p.dy + w.n * p.dy_n + s * p.dy_s + w.c);
+      const vec_t dv = fetch<NT>((const vec_t*)(p.dy + w.n * p.dy_n + s * p.dy_s + w.c));
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const T h = (xv[e] - mean[e]) * rstd[e];
@@ -555,21 +561,29 @@ static int check_args(const char* fn, int64_t batch, int64_t spatial, int64_t ch
   return AM_OK;
 }
 
-template <typename T, int V, int U, bool WIDE, int ACT, bool BWD>
-static void launch_team(const Args<T>& p, int lanes, int units, int64_t slots, int64_t wgs) {
-  if constexpr (BWD) hipLaunchKernelGGL((team_backward<T, V, U, WIDE, ACT>), dim3((unsigned)wgs), dim3(256), 0, stream(), p, lanes, units, slots);
-  else hipLaunchKernelGGL((team_forward<T, V, U, WIDE, ACT>), dim3((unsigned)wgs), dim3(256), 0, stream(), p, lanes, units, slots);
+template <typename T> static bool past_caches(const Args<T>& p) {
+  return (double)p.batch * (double)p.spatial * p.channels * sizeof(T) > nt_threshold_bytes();
 }
 
-#ifndef GNW
-#define GNW 2
-#endif
+template <typename T, int V, int U, bool WIDE, int ACT, bool BWD>
+static void launch_team(const Args<T>& p, int lanes, int units, int64_t slots, int64_t wgs) {
+  const dim3 grid((unsigned)wgs), block(256);
+  const bool nt = V > 1 && past_caches(p);
+  if constexpr (BWD) {
+    if (nt) hipLaunchKernelGGL((team_backward<T, V, U, WIDE, ACT, (V > 1)>), grid, block, 0, stream(), p, lanes, units, slots);
+    else hipLaunchKernelGGL((team_backward<T, V, U, WIDE, ACT, false>), grid, block, 0, stream(), p, lanes, units, slots);
+  } else {
+    if (nt) hipLaunchKernelGGL((team_forward<T, V, U, WIDE, ACT, (V > 1)>), grid, block, 0, stream(), p, lanes, units, slots);
+    else hipLaunchKernelGGL((team_forward<T, V, U, WIDE, ACT, false>), grid, block, 0, stream(), p, lanes, units, slots);
+  }
+}
+
 template <typename T, int V, int ACT, bool BWD>
 static int team_pass(Args<T> p, int lanes, int units) {
-  // Samples per team: as many as leave eight workgroups for every CU (backwards GNW, whose shares of the parameters'
-  // gradients have to be written and read again), and at most 64, so that a lane's shares are short sums.
+  // Samples per team: as many as leave eight workgroups for every CU (backwards two, as the shares of the parameters'
+  // gradients have to be written and read again: [16384, 2048] in 16 groups 88 us, against 96 with one and 100 with four), and at most 64, so that a lane's shares are short sums.
   const int64_t at_once = 256 / lanes;
-  int64_t slots = (int64_t)num_cus() * (BWD ? GNW : 8) * at_once / p.groups;
+  int64_t slots = (int64_t)num_cus() * (BWD ? 2 : 8) * at_once / p.groups;
   if (slots < (p.batch + 63) / 64) slots = (p.batch + 63) / 64;
   if (slots < 1) slots = 1;
   if (slots > p.batch) slots = p.batch;
@@ -651,7 +665,8 @@ static int forward(Args<T> p) {
     AM_TRY(check_launch("slab_sums"));
     hipLaunchKernelGGL((group_fold<T, false>), dim3((unsigned)(p.nc * p.groups)), dim3(256), 0, stream(), p);
     AM_TRY(check_launch("group_fold"));
-    AM_GN_LAUNCH(slab_apply, V, wgs, false, ACT);
+    if (V > 1 && past_caches(all)) AM_GN_LAUNCH(slab_apply, V, wgs, false, ACT, true);
+    else AM_GN_LAUNCH(slab_apply, V, wgs, false, ACT, false);
     AM_TRY(check_launch("slab_apply"));
   }
   return AM_OK;
@@ -701,7 +716,7 @@ static int backward(Args<T> p) {
       hipLaunchKernelGGL((channel_fold<T, double>), dim3((unsigned)((p.channels + 7) / 8)), dim3(256), 0, stream(), p, (const double*)p.chan, p.nc, 1, n > 0);
       AM_TRY(check_launch("channel_fold"));
     }
-    AM_GN_LAUNCH(slab_apply, V, wgs, true, ACT);
+    AM_GN_LAUNCH(slab_apply, V, wgs, true, ACT, false);   // (past the caches 89.5 -> 94 us for [16, 64, 64, 320])
     AM_TRY(check_launch("slab_apply"));
   }
   return AM_OK;
