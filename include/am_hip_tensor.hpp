@@ -21,6 +21,7 @@
 //   isNaN, classify, sgn, clamp       am::isNaN, am::classify, am::sgn, am::clamp / t.mclamp(lo, hi)
 //   echo t, t.pretty(precision)       std::cout << t, am::pretty(t, precision, specifier)
 //   ln(t), cos(t), floor(t) ...       am::ln(t), am::cos(t), am::floor(t) ...
+//   (none: sequence layers)           am::rotary, am::decay_attention, am::decay_attention_step, am::group_norm and their _backward
 //   t.transpose, t[a..b|s, ...]       t.transpose(), t.slice(axis, first, last, step)
 //   t.broadcast(shape)                t.broadcast(shape)
 // Errors: std::invalid_argument where the reference raises ValueError, std::out_of_range where it
@@ -729,6 +730,218 @@ void gru_cell_inference(const HipTensor<T>& input, const HipTensor<T>& W3, const
     r = (*saved)[0].ptr(); z = (*saved)[1].ptr(); n = (*saved)[2].ptr(); uh = (*saved)[3].ptr();
   }
   check(detail::gru_gates_(B, H, W3x.ptr(), W3x.strides[0], U3h.ptr(), U3h.strides[0], hidden.ptr(), hidden.strides[0], r, z, n, uh, H));
+}
+
+// ---- sequence mixing (no counterpart in the reference; am_hip.h, "sequence mixing"): rotary positions, linear attention with
+// a decay for each head, channels-last group norm. The GRU's relatives for training over all tokens at once.
+namespace detail {
+inline int rotary_(int64_t b, int64_t t, int64_t h, int64_t d, int64_t r, int lay, int inv, float s, const int64_t* p, int64_t pb, int64_t pt,
+                   const double* f, const float* x, const Shape& xs, float* o, const Shape& os) {
+  return am_hip_rotary_f32(b, t, h, d, r, lay, inv, s, p, pb, pt, f, x, xs[0], xs[1], xs[2], o, os[0], os[1], os[2]);
+}
+inline int rotary_(int64_t b, int64_t t, int64_t h, int64_t d, int64_t r, int lay, int inv, double s, const int64_t* p, int64_t pb, int64_t pt,
+                   const double* f, const double* x, const Shape& xs, double* o, const Shape& os) {
+  return am_hip_rotary_f64(b, t, h, d, r, lay, inv, s, p, pb, pt, f, x, xs[0], xs[1], xs[2], o, os[0], os[1], os[2]);
+}
+#define AM_DECAY_HOST_(S, T)                                                                                                          \
+  inline int decay_(const int64_t* n, T scale, const T* g, const int64_t* len, const T* q, const Shape& qs, const T* k, const Shape& ks, \
+                    const T* v, const Shape& vs, const T* s0, const Shape& s0s, T* o, const Shape& os, T* s1, const Shape& s1s) {      \
+    return am_hip_decay_attention_##S(n[0], n[1], n[2], n[3], n[4], n[5], scale, g, len, q, qs[0], qs[1], qs[2], k, ks[0], ks[1],      \
+                                      ks[2], v, vs[0], vs[1], vs[2], s0, s0s[0], s0s[1], o, os[0], os[1], os[2], s1, s1s[0], s1s[1]);  \
+  }                                                                                                                                    \
+  inline int decay_backward_(const int64_t* n, T scale, const T* g, const int64_t* len, const T* go, const Shape& gos, const T* q,    \
+                             const Shape& qs, const T* k, const Shape& ks, const T* v, const Shape& vs, const T* s0, const Shape& s0s, \
+                             const T* gs, const Shape& gss, T* dq, const Shape& dqs, T* dk, const Shape& dks, T* dv, const Shape& dvs, \
+                             T* ds, const Shape& dss) {                                                                                \
+    return am_hip_decay_attention_backward_##S(n[0], n[1], n[2], n[3], n[4], n[5], scale, g, len, go, gos[0], gos[1], gos[2], q,       \
+                                               qs[0], qs[1], qs[2], k, ks[0], ks[1], ks[2], v, vs[0], vs[1], vs[2], s0, s0s[0],        \
+                                               s0s[1], gs, gss[0], gss[1], dq, dqs[0], dqs[1], dqs[2], dk, dks[0], dks[1], dks[2],     \
+                                               dv, dvs[0], dvs[1], dvs[2], ds, dss[0], dss[1]);                                        \
+  }                                                                                                                                    \
+  inline int decay_step_(const int64_t* n, T scale, const T* g, const T* q, const Shape& qs, const T* k, const Shape& ks, const T* v,  \
+                         const Shape& vs, T* s, const Shape& ss, T* o, const Shape& os) {                                              \
+    return am_hip_decay_attention_step_##S(n[0], n[1], n[2], n[3], n[4], scale, g, q, qs[0], qs[1], k, ks[0], ks[1], v, vs[0], vs[1],  \
+                                           s, ss[0], ss[1], o, os[0], os[1]);                                                          \
+  }                                                                                                                                    \
+  inline int group_norm_(int64_t n, int64_t s, int64_t c, int64_t g, T eps, int act, const T* x, int64_t xn, int64_t xs, const T* w,   \
+                         const T* b, T* y, T* mean, T* rstd) {                                                                         \
+    return am_hip_group_norm_##S(n, s, c, g, eps, act, x, xn, xs, w, b, y, s * c, c, mean, rstd);                                      \
+  }                                                                                                                                    \
+  inline int group_norm_backward_(int64_t n, int64_t s, int64_t c, int64_t g, int act, const T* dy, int64_t dn, int64_t ds,            \
+                                  const T* x, int64_t xn, int64_t xs, const T* w, const T* b, const T* mean, const T* rstd, T* dx,     \
+                                  T* dw, T* db) {                                                                                      \
+    return am_hip_group_norm_backward_##S(n, s, c, g, act, dy, dn, ds, x, xn, xs, w, b, mean, rstd, dx, s * c, c, dw, db);             \
+  }
+AM_DECAY_HOST_(f32, float)
+AM_DECAY_HOST_(f64, double)
+#undef AM_DECAY_HOST_
+
+template <typename T> HipTensor<T> unit_rows_(const HipTensor<T>& t) { return t.strides.back() == 1 || t.shape.back() == 1 ? t : t.clone(); }
+inline void need_(bool ok, const char* what) { if (!ok) throw std::invalid_argument(what); }
+
+// A state [batch, heads, dk, dv] whose heads are contiguous, or none.
+template <typename T> T* state_(const HipTensor<T>* s, const Shape& shape, Shape& strides) {
+  strides = Shape{0, 0};
+  if (!s) return nullptr;
+  need_(s->shape == shape, "decay_attention: a state must be [batch, heads, dk, dv]");
+  need_((s->strides[3] == 1 || shape[3] == 1) && (s->strides[2] == shape[3] || shape[2] == 1), "decay_attention: each head of a state must be contiguous");
+  strides = Shape{s->strides[0], s->strides[1]};
+  return s->ptr();
+}
+
+template <typename T>
+HipTensor<T> rotate_(const HipTensor<T>& x, const HipTensor<int64_t>* positions, const HipTensor<double>& frequencies, int layout, T scale, int inverse) {
+  static_assert(std::is_floating_point<T>::value, "rotary is defined for float tensors");
+  need_(x.rank() == 4, "rotary: x must be [batch, tokens, heads, dim]");
+  need_(frequencies.rank() == 1 && frequencies.is_C_contiguous() && 2 * frequencies.shape[0] <= x.shape[3], "rotary: frequencies must be a contiguous vector of at most dim / 2 values");
+  int64_t pb = 0, pt = 0;
+  if (positions) {
+    need_(positions->shape == (Shape{x.shape[0], x.shape[1]}), "rotary: positions must be [batch, tokens]");
+    pb = positions->strides[0]; pt = positions->strides[1];
+  }
+  const HipTensor<T> src = unit_rows_(x);
+  HipTensor<T> out(x.shape);
+  check(rotary_(x.shape[0], x.shape[1], x.shape[2], x.shape[3], 2 * frequencies.shape[0], layout, inverse, scale, positions ? positions->ptr() : nullptr, pb, pt,
+                frequencies.ptr(), src.ptr(), src.strides, out.ptr(), out.strides));
+  return out;
+}
+
+// {batch, tokens, heads, kv_heads, dk, dv} of q, k, v with `lead` leading dimensions (2: sequences, 1: single tokens)
+template <typename T>
+std::vector<int64_t> decay_sizes_(const HipTensor<T>& q, const HipTensor<T>& k, const HipTensor<T>& v, const HipTensor<T>& log_decay, size_t lead) {
+  static_assert(std::is_floating_point<T>::value, "decay_attention is defined for float tensors");
+  need_(q.shape.size() == lead + 2 && k.shape.size() == lead + 2 && v.shape.size() == lead + 2, "decay_attention: q, k and v of one rank are needed");
+  for (size_t i = 0; i < lead; ++i) need_(k.shape[i] == q.shape[i] && v.shape[i] == q.shape[i], "decay_attention: q, k and v of one batch are needed");
+  need_(k.shape[lead] == v.shape[lead] && k.shape[lead + 1] == q.shape[lead + 1], "decay_attention: q and k must share dk, k and v their heads");
+  need_(log_decay.shape == (Shape{q.shape[lead]}) && log_decay.is_C_contiguous(), "decay_attention: log_decay must be [heads]");
+  std::vector<int64_t> n(q.shape.begin(), q.shape.begin() + lead);
+  n.insert(n.end(), {q.shape[lead], k.shape[lead], q.shape[lead + 1], v.shape[lead + 1]});
+  return n;
+}
+inline const int64_t* lengths_(const HipTensor<int64_t>* lengths, int64_t batch) {
+  if (!lengths) return nullptr;
+  need_(lengths->shape == (Shape{batch}) && lengths->is_C_contiguous(), "decay_attention: lengths must be [batch]");
+  return lengths->ptr();
+}
+
+// [batch, ..., channels] with its middle dimensions walked as one: row strides of a sample and of a position.
+template <typename T> HipTensor<T> channels_last_(const HipTensor<T>& t, int64_t& sn, int64_t& ss) {
+  need_(t.rank() >= 2, "group_norm: a tensor [batch, ..., channels] is needed");
+  bool ok = t.strides.back() == 1 || t.shape.back() == 1;
+  int64_t step = 0, extent = 0;
+  for (int d = t.rank() - 2; d >= 1; --d) {
+    if (t.shape[d] == 1) continue;
+    if (!extent) { step = t.strides[d]; extent = t.shape[d]; }
+    else { ok = ok && t.strides[d] == step * extent; extent *= t.shape[d]; }
+  }
+  const HipTensor<T> r = ok ? t : t.clone();
+  sn = r.strides[0];
+  ss = ok && extent ? step : r.shape.back();
+  return r;
+}
+template <typename T> HipTensor<T> vector_(const HipTensor<T>* t, int64_t channels) {
+  if (!t) return HipTensor<T>();
+  need_(t->size() == channels && t->shape.back() == channels, "group_norm: weight and bias must be [channels]");
+  return t->is_C_contiguous() ? *t : t->clone();
+}
+}  // namespace detail
+
+// x [batch, tokens, heads, dim] with the pairs of every head turned by position * frequency (AM_ROTARY_HALF or
+// AM_ROTARY_INTERLEAVED); positions [batch, tokens], null: the token's index. rotary_backward: the gradient.
+template <typename T>
+HipTensor<T> rotary(const HipTensor<T>& x, const HipTensor<int64_t>* positions, const HipTensor<double>& frequencies, int layout = AM_ROTARY_HALF, T scale = T(1)) {
+  return detail::rotate_(x, positions, frequencies, layout, scale, 0);
+}
+template <typename T>
+HipTensor<T> rotary_backward(const HipTensor<T>& gradient, const HipTensor<int64_t>* positions, const HipTensor<double>& frequencies, int layout = AM_ROTARY_HALF, T scale = T(1)) {
+  return detail::rotate_(gradient, positions, frequencies, layout, scale, 1);
+}
+
+// S <- e^g S + k^T v, out = scale * q S over whole sequences; `last`, when given, receives the state behind the last token.
+template <typename T>
+HipTensor<T> decay_attention(const HipTensor<T>& q, const HipTensor<T>& k, const HipTensor<T>& v, const HipTensor<T>& log_decay, T scale = T(1),
+                             const HipTensor<T>* state = nullptr, HipTensor<T>* last = nullptr, const HipTensor<int64_t>* lengths = nullptr) {
+  const auto n = detail::decay_sizes_(q, k, v, log_decay, 2);
+  const Shape states{n[0], n[2], n[4], n[5]};
+  Shape s0s, s1s{0, 0};
+  const T* s0 = detail::state_(state, states, s0s);
+  const int64_t* len = detail::lengths_(lengths, n[0]);
+  const HipTensor<T> qq = detail::unit_rows_(q), kk = detail::unit_rows_(k), vv = detail::unit_rows_(v);
+  HipTensor<T> out(Shape{n[0], n[1], n[2], n[5]}), end;
+  if (last) { end = HipTensor<T>(states); s1s = Shape{end.strides[0], end.strides[1]}; }
+  check(detail::decay_(n.data(), scale, log_decay.ptr(), len, qq.ptr(), qq.strides, kk.ptr(), kk.strides, vv.ptr(), vv.strides, s0, s0s, out.ptr(), out.strides,
+                       last ? end.ptr() : nullptr, s1s));
+  if (last) *last = end;
+  return out;
+}
+
+// {dq, dk, dv} of decay_attention, and dstate behind them where a state went in.
+template <typename T>
+std::vector<HipTensor<T>> decay_attention_backward(const HipTensor<T>& grad_output, const HipTensor<T>& q, const HipTensor<T>& k, const HipTensor<T>& v,
+                                                   const HipTensor<T>& log_decay, T scale = T(1), const HipTensor<T>* state = nullptr,
+                                                   const HipTensor<T>* grad_state = nullptr, const HipTensor<int64_t>* lengths = nullptr) {
+  const auto n = detail::decay_sizes_(q, k, v, log_decay, 2);
+  const Shape states{n[0], n[2], n[4], n[5]};
+  detail::need_(grad_output.shape == (Shape{n[0], n[1], n[2], n[5]}), "decay_attention_backward: the output's gradient must be [batch, tokens, heads, dv]");
+  Shape s0s, gss, dss{0, 0};
+  const T* s0 = detail::state_(state, states, s0s);
+  const T* gs = detail::state_(grad_state, states, gss);
+  const int64_t* len = detail::lengths_(lengths, n[0]);
+  const HipTensor<T> go = detail::unit_rows_(grad_output), qq = detail::unit_rows_(q), kk = detail::unit_rows_(k), vv = detail::unit_rows_(v);
+  std::vector<HipTensor<T>> r{HipTensor<T>(q.shape), HipTensor<T>(k.shape), HipTensor<T>(v.shape)};
+  if (state) { r.push_back(HipTensor<T>(states)); dss = Shape{r[3].strides[0], r[3].strides[1]}; }
+  check(detail::decay_backward_(n.data(), scale, log_decay.ptr(), len, go.ptr(), go.strides, qq.ptr(), qq.strides, kk.ptr(), kk.strides, vv.ptr(), vv.strides, s0, s0s,
+                                gs, gss, r[0].ptr(), r[0].strides, r[1].ptr(), r[1].strides, r[2].ptr(), r[2].strides, state ? r[3].ptr() : nullptr, dss));
+  return r;
+}
+
+// One new token of every sequence: q [batch, heads, dk], k [batch, kv_heads, dk], v [batch, kv_heads, dv]; `state` in place.
+template <typename T>
+HipTensor<T> decay_attention_step(const HipTensor<T>& q, const HipTensor<T>& k, const HipTensor<T>& v, const HipTensor<T>& log_decay, HipTensor<T>& state, T scale = T(1)) {
+  const auto n = detail::decay_sizes_(q, k, v, log_decay, 1);
+  Shape ss;
+  T* s = detail::state_(&state, Shape{n[0], n[1], n[3], n[4]}, ss);
+  const HipTensor<T> qq = detail::unit_rows_(q), kk = detail::unit_rows_(k), vv = detail::unit_rows_(v);
+  HipTensor<T> out(Shape{n[0], n[1], n[4]});
+  check(detail::decay_step_(n.data(), scale, log_decay.ptr(), qq.ptr(), qq.strides, kk.ptr(), kk.strides, vv.ptr(), vv.strides, s, ss, out.ptr(), out.strides));
+  return out;
+}
+
+// act((x - mean) / sqrt(variance + eps) * weight + bias) of [batch, ..., channels] in `groups` groups of neighbouring channels
+// (AM_ACT_NONE / RELU / SILU); weight and bias may be null. `kept`, when given, receives {mean, 1 / deviation}.
+template <typename T>
+HipTensor<T> group_norm(const HipTensor<T>& x, const HipTensor<T>* weight, const HipTensor<T>* bias, int64_t groups, T eps = T(1e-5), int activation = AM_ACT_NONE,
+                        std::vector<HipTensor<T>>* kept = nullptr) {
+  static_assert(std::is_floating_point<T>::value, "group_norm is defined for float tensors");
+  int64_t sn, ss;
+  const HipTensor<T> src = detail::channels_last_(x, sn, ss);
+  const int64_t N = x.shape[0], C = x.shape.back(), S = N && C ? x.size() / (N * C) : 0;
+  const HipTensor<T> w = detail::vector_(weight, C), b = detail::vector_(bias, C);
+  HipTensor<T> y(x.shape);
+  if (kept) *kept = {HipTensor<T>(Shape{N, groups}), HipTensor<T>(Shape{N, groups})};
+  check(detail::group_norm_(N, S, C, groups, eps, activation, src.ptr(), sn, ss, weight ? w.ptr() : nullptr, bias ? b.ptr() : nullptr, y.ptr(),
+                            kept ? (*kept)[0].ptr() : nullptr, kept ? (*kept)[1].ptr() : nullptr));
+  return y;
+}
+
+// {dx, dweight, dbias} from the output's gradient, x and what group_norm kept; dweight / dbias are empty without weight / bias.
+template <typename T>
+std::vector<HipTensor<T>> group_norm_backward(const HipTensor<T>& grad_output, const HipTensor<T>& x, const HipTensor<T>* weight, const HipTensor<T>* bias,
+                                              const std::vector<HipTensor<T>>& kept, int64_t groups, int activation = AM_ACT_NONE) {
+  detail::need_(grad_output.shape == x.shape, "group_norm_backward: the output's gradient must have x's shape");
+  int64_t sn, ss, gn, gs;
+  const HipTensor<T> src = detail::channels_last_(x, sn, ss), go = detail::channels_last_(grad_output, gn, gs);
+  const int64_t N = x.shape[0], C = x.shape.back(), S = N && C ? x.size() / (N * C) : 0;
+  detail::need_(kept.size() == 2 && kept[0].shape == (Shape{N, groups}) && kept[1].shape == kept[0].shape && kept[0].is_C_contiguous() && kept[1].is_C_contiguous(),
+                "group_norm_backward: kept must be the {mean, rstd} of group_norm");
+  const HipTensor<T> w = detail::vector_(weight, C), b = detail::vector_(bias, C);
+  std::vector<HipTensor<T>> r(3);
+  r[0] = HipTensor<T>(x.shape);
+  if (weight) r[1] = HipTensor<T>(weight->shape);
+  if (bias) r[2] = HipTensor<T>(bias->shape);
+  check(detail::group_norm_backward_(N, S, C, groups, activation, go.ptr(), gn, gs, src.ptr(), sn, ss, weight ? w.ptr() : nullptr, bias ? b.ptr() : nullptr,
+                                     kept[0].ptr(), kept[1].ptr(), r[0].ptr(), weight ? r[1].ptr() : nullptr, bias ? r[2].ptr() : nullptr));
+  return r;
 }
 
 // Fold along `axis`; the result keeps the axis with extent 1 (reduce_axis_inline,

@@ -1,6 +1,8 @@
 """The sequence operators without a device: what they refuse (before anything reaches the GPU), the frequencies, and the
 definitions that the device tests compare with, checked against differences."""
 import ctypes
+import os
+import subprocess
 
 import numpy as np
 import pytest
@@ -186,3 +188,9 @@ def test_the_definitions_gradients_against_differences():
     for act in ("none", "relu", "silu"):
         for name, grad in zip(("x", "w", "b"), ref.norm_backward(dy, n["x"], n["w"], n["b"], 3, 1e-3, act)):
             _differences(lambda a: (ref.norm(*[{**n, name: a}[m] for m in "xwb"], 3, 1e-3, act) * dy).sum(), n[name], grad, rng, 1e-6)
+
+
+def test_the_cpp_host_layer_builds():
+    where = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp")
+    res = subprocess.run(["make", "-C", where, "-B", "test_sequence"], capture_output=True, text=True)
+    assert res.returncode == 0, res.stderr[-3000:]

@@ -5,6 +5,9 @@ Tolerances. u = half a step of the element type (eps / 2). A result that is a su
 n * u * (the sum of the absolute values of its terms), where n counts the roundings a term passes: the definitions are run a
 second time on absolute values to get those sums. The exponentials of the decays are good to 2 steps = 4 u and a product of
 two of them and of its exponent adds 4 more."""
+import os
+import subprocess
+
 import numpy as np
 import pytest
 
@@ -520,3 +523,13 @@ def test_a_layer_in_a_graph(hip):
         g.launch()
         want = hip.decay_attention_step(*d, mirror).toCpu()
         assert np.array_equal(res.toCpu(), want) and np.array_equal(live.toCpu(), mirror.toCpu()), f"step {turn}"
+
+
+# ---------------------------------------------------------------------- the C++ host layer
+def test_the_cpp_host_layer(hip):
+    program = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "test_sequence")
+    if not os.path.exists(program):
+        pytest.fail("tests/cpp/test_sequence is not built (python -c 'import __graft_entry__ as g; g.build()')")
+    res = subprocess.run([program], capture_output=True, text=True, timeout=60)
+    print(res.stdout)
+    assert res.returncode == 0 and " 0 failed" in res.stdout, res.stdout[-3000:] + res.stderr[-1000:]
