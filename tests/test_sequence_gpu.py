@@ -91,6 +91,13 @@ def test_rotary_of_views_and_in_place(hip, dt, layout):
     assert hip.rotary_into(inside, inside, pos, freq, layout=layout) is inside
     host = wide.toCpu()
     assert np.array_equal(host[:, :, :H], want) and np.array_equal(host[:, :, H:], x + 1), "in place, and nothing beside it"
+    some = hip.rotary_frequencies(12)                          # a part of the head in place, and into another tensor's view
+    part = hip.rotary(hip.toHip(x), pos, some, layout=layout).toCpu()
+    here, other = hip.toHip(x), hip.toHip(np.concatenate([x, x], axis=3))
+    hip.rotary_into(here, here, pos, some, layout=layout)
+    hip.rotary_into(other[:, :, :, D:], hip.toHip(x), pos, some, layout=layout)
+    assert np.array_equal(here.toCpu(), part)
+    assert np.array_equal(other.toCpu()[..., D:], part) and np.array_equal(other.toCpu()[..., :D], x)
 
 
 def test_rotary_keeps_far_positions(hip):
@@ -204,6 +211,86 @@ def test_decay_attention_of_no_tokens_and_of_extreme_decays(hip, dt):
     x = attention_inputs(hip, size, dt, 4)
     x["g"][:] = [0.0, -np.inf, -40.0]
     check_attention(hip, size, dt, x, given=True, padded=False, grads=True)
+
+
+@pytest.mark.parametrize("dt", ["f32", "f64"])
+@pytest.mark.parametrize("dk", [32, 30])
+def test_decay_attention_of_reversed_views(hip, dt, dk):
+    """Tokens stored last to first (negative strides), and one token's key standing for all (stride 0), forwards and backwards,
+    with lengths: the bits of the contiguous call."""
+    B, T, H, dv = 3, 75, 2, 34
+    x = attention_inputs(hip, (B, T, H, H, dk, dv), dt, seed_of("reversed", dt, dk))
+    x["lengths"][:] = [75, 41, 64]
+    d = {n: hip.toHip(a) for n, a in x.items() if n != "scale"}
+    back = lambda a: hip.toHip(np.ascontiguousarray(a[:, ::-1]))[:, ::-1]
+    r = {n: back(x[n]) for n in ("q", "k", "v", "go")}
+
+    def both(q, k, v, go):
+        kw = dict(state=d["state"], lengths=d["lengths"], scale=0.3)
+        return [t.toCpu() for t in hip.decay_attention(q, k, v, d["g"], **kw) + hip.decay_attention_backward(go, q, k, v, d["g"], gradState=d["gs"], **kw)]
+
+    for a, b in zip(both(r["q"], r["k"], r["v"], r["go"]), both(d["q"], d["k"], d["v"], d["go"])):
+        assert np.array_equal(a, b)
+    one = d["k"][:, 0:1].broadcast((B, T, H, dk))
+    same = hip.toHip(np.ascontiguousarray(np.broadcast_to(x["k"][:, :1], (B, T, H, dk))))
+    for a, b in zip(both(d["q"], one, d["v"], d["go"]), both(d["q"], same, d["v"], d["go"])):
+        assert np.array_equal(a, b)
+
+
+def test_the_state_may_be_carried_in_place(hip):
+    """state_out over state_in and grad_state_in over grad_state_out, which the C interface allows, in one segment and in many."""
+    from arraymancer_amd.sequence_hip import _rows
+    L = hip.load_library()
+    for B, T, H, KH, dk, dv in ((2, 40, 2, 1, 16, 24), (1, 3000, 2, 2, 32, 32)):
+        x = attention_inputs(hip, (B, T, H, KH, dk, dv), "f32", 12)
+        d = {n: hip.toHip(a) for n, a in x.items() if n not in ("scale", "lengths")}
+        out, end = hip.decay_attention(d["q"], d["k"], d["v"], d["g"], state=d["state"])
+        grads = hip.decay_attention_backward(d["go"], d["q"], d["k"], d["v"], d["g"], state=d["state"], gradState=d["gs"])
+        state, gs = hip.toHip(x["state"]), hip.toHip(x["gs"])
+        mine = [hip.empty(t.shape, np.float32) for t in (out,) + grads[:3]]
+        sizes = (B, T, H, KH, dk, dv, 1.0, d["g"].data_ptr(), None)
+        q, k, v, go = (_rows(d[n]) for n in ("q", "k", "v", "go"))
+        assert L.am_hip_decay_attention_f32(*sizes, *q, *k, *v, *_rows(state)[:3], *_rows(mine[0]), *_rows(state)[:3]) == 0
+        assert L.am_hip_decay_attention_backward_f32(*sizes, *go, *q, *k, *v, *_rows(d["state"])[:3], *_rows(gs)[:3], *_rows(mine[1]), *_rows(mine[2]),
+                                                     *_rows(mine[3]), *_rows(gs)[:3]) == 0
+        for a, b in zip(mine + [state, gs], (out,) + grads[:3] + (end, grads[3])):
+            assert np.array_equal(a.toCpu(), b.toCpu())
+
+
+def far_view(hip, base, shape, strides, offset=0):
+    from arraymancer_amd import Layout
+    from arraymancer_amd.tensor_hip import HipTensor
+    return HipTensor(Layout(shape, strides, offset), base.storage, base.dtype)
+
+
+def test_operands_farther_apart_than_32_bits(hip):
+    """Sequences 2^31 elements apart, and tokens 2^26 apart (32 of them do not fit a 32-bit offset): the bits of packed ones."""
+    base = hip.empty((2 ** 31 + 2 ** 20,), np.float32)
+    B, T, H, D = 2, 34, 1, 32
+    rng = np.random.default_rng(21)
+    host = {n: rng.normal(size=(B, T, H, D)).astype(np.float32) for n in ("q", "k", "v", "go")}
+    near = {n: hip.toHip(a) for n, a in host.items()}
+    g = hip.toHip(np.array([-0.05], np.float32))
+    apart = {n: far_view(hip, base, (B, T, H, D), (2 ** 31, H * D, D, 1), i * T * H * D) for i, n in enumerate(host)}
+    wide = {n: far_view(hip, base, (1, T - 2, H, D), (0, 2 ** 26, D, 1), 2 ** 15 + i * 64) for i, n in enumerate(host)}
+    freq = hip.rotary_frequencies(D)
+    for views, rows in ((apart, slice(0, T)), (wide, slice(0, T - 2))):
+        n = views["q"].shape[0]
+        packed = {m: hip.toHip(np.ascontiguousarray(a[:n, rows])) for m, a in host.items()}
+        for m in views:
+            _unary_into("copy", views[m], packed[m])
+        got = hip.decay_attention(views["q"], views["k"], views["v"], g) + hip.decay_attention_backward(views["go"], views["q"], views["k"], views["v"], g)[:3] + \
+            (hip.rotary(views["q"], None, freq), hip.decay_attention_step(*(views[m][:, 3].squeeze(1) for m in "qkv"), g, hip.zeros((n, H, D, D), np.float32)))
+        want = hip.decay_attention(packed["q"], packed["k"], packed["v"], g) + hip.decay_attention_backward(packed["go"], packed["q"], packed["k"], packed["v"], g)[:3] + \
+            (hip.rotary(packed["q"], None, freq), hip.decay_attention_step(*(packed[m][:, 3].squeeze(1) for m in "qkv"), g, hip.zeros((n, H, D, D), np.float32)))
+        tol = 64 * unit(np.float32)
+        for a, b in zip(got, want):     # (whole vectors and single elements take other kernels: rounding apart, not bits)
+            a, b = a.toCpu(), b.toCpu()
+            assert np.abs(a - b).max() <= tol * np.abs(b).max()
+    rows = far_view(hip, base, (2, 40, 48), (2 ** 31, 48, 1), 11)
+    x = rng.normal(size=(2, 40, 48)).astype(np.float32)
+    _unary_into("copy", rows, hip.toHip(x))
+    assert np.array_equal(hip.group_norm(rows, None, None, 4).toCpu(), hip.group_norm(far_view(hip, hip.toHip(np.concatenate([x.reshape(-1)[:11], x.reshape(-1)])), (2, 40, 48), (1920, 48, 1), 11), None, None, 4).toCpu())
 
 
 @pytest.mark.parametrize("dt", ["f32", "f64"])
@@ -341,6 +428,25 @@ def test_group_norm_without_parameters_and_of_a_large_mean(hip, shape, groups, d
     dx, dw, db = hip.group_norm_backward(hip.toHip(dy), hip.toHip(x), None, None, mean, rstd, groups)
     assert dw is None and db is None
     close(dx.toCpu(), ref.norm_backward(dy, x, None, None, groups, eps)[0], bdx, "dx")
+
+
+@pytest.mark.parametrize("dt", ["f32", "f64"])
+@pytest.mark.parametrize("shape,groups", [((6, 40), 4), ((2, 60, 50, 16), 2)], ids=str)
+def test_group_norm_activations_far_out(hip, shape, groups, dt):
+    """Weights that take silu far beyond the range of e^z on both sides: saturated, finite, and exact where it is 0 or z. The
+    float sigmoid is good to 4 steps, z itself to what the norm's own bounds say."""
+    x, w, b, dy = norm_inputs(shape, dt, seed_of("far out", shape, dt))
+    w *= DTYPES[dt](300)
+    by, bdx, bdw, bdb = norm_bounds(x, w, b, dy, groups, 1e-5, dt)
+    y, mean, rstd = hip.group_norm_forward(hip.toHip(x), hip.toHip(w), hip.toHip(b), groups, activation="silu")
+    with np.errstate(over="ignore"):
+        want = ref.norm(x, w, b, groups, 1e-5, "silu")
+        grads = ref.norm_backward(dy, x, w, b, groups, 1e-5, "silu")
+    assert (np.abs(want) > 200).any() and (want == 0).any() or dt == "f64"
+    close(y.toCpu(), want, by, "y")
+    got = hip.group_norm_backward(hip.toHip(dy), hip.toHip(x), hip.toHip(w), hip.toHip(b), mean, rstd, groups, activation="silu")
+    for name, a, r, bound in zip(("dx", "dweight", "dbias"), got, grads, (bdx, bdw, bdb)):
+        close(a.toCpu(), r, bound, name)
 
 
 @pytest.mark.parametrize("dt", ["f32", "f64"])
