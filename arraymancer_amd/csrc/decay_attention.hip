@@ -148,19 +148,24 @@ __device__ __forceinline__ void put(const Chunk& c, uint32_t off, double v) {
 // The rows of up to 32 tokens of an operand, as 16-byte vectors in registers on their way to LDS. Every lane always loads (a
 // load under a branch would have to be waited for before the next one). FAST: rows are whole vectors and the chunks buffers;
 // else element by element from clamped addresses. What lies outside becomes 0 on the way into LDS.
-template <typename T, int DA, bool FAST> struct Tile {
-  static constexpr int V = 16 / (int)sizeof(T), PER_ROW = DA / V, NV = kChunk * PER_ROW / 256;
-  static constexpr bool EVEN = 256 % PER_ROW == 0;       // vector u of a lane lies whole rows behind its first
-  static constexpr int NO = EVEN ? 1 : NV;
+template <typename T, int DA, bool FAST, int THREADS> struct Tile {
+  static constexpr int V = 16 / (int)sizeof(T), PER_ROW = DA / V, ALL = kChunk * PER_ROW, NV = (ALL + THREADS - 1) / THREADS;
+  static constexpr bool EVEN = THREADS % PER_ROW == 0;   // vector u of a lane lies whole rows behind its first
+  static constexpr bool FULL = ALL % THREADS == 0;       // every lane has NV vectors (else the last ones repeat the tile's last)
+  static constexpr int NO = EVEN && FULL ? 1 : NV;
   typedef T vec_t __attribute__((ext_vector_type(V)));
   vec_t v[NV];
   uint32_t off[NO];                                      // of a lane's vectors behind the chunk's first token
 
+  static __device__ __forceinline__ int vector(int u) {
+    const int f = (int)threadIdx.x + u * THREADS;
+    return FULL || f < ALL ? f : ALL - 1;
+  }
   __device__ __forceinline__ void prepare(int64_t step) {
     if constexpr (FAST) {
 #pragma unroll
       for (int u = 0; u < NO; ++u) {
-        const int f = (int)threadIdx.x + u * 256, row = f / PER_ROW, c = (f - row * PER_ROW) * V;
+        const int f = vector(u), row = f / PER_ROW, c = (f - row * PER_ROW) * V;
         off[u] = (uint32_t)((row * (int)step + c) * (int)sizeof(T));
       }
     }
@@ -171,13 +176,13 @@ template <typename T, int DA, bool FAST> struct Tile {
       const Chunk k = chunk_of(p, step, n, da);
 #pragma unroll
       for (int u = 0; u < NV; ++u) {
-        const uint32_t o = EVEN ? off[0] + (k.first + (uint32_t)(u * (256 / PER_ROW) * (int)step * (int)sizeof(T))) : off[u % NO] + k.first;
+        const uint32_t o = NO == 1 ? off[0] + (k.first + (uint32_t)(u * (THREADS / PER_ROW) * (int)step * (int)sizeof(T))) : off[u % NO] + k.first;
         v[u] = __builtin_bit_cast(vec_t, __builtin_amdgcn_raw_buffer_load_b128(k.rsrc, (int)o, 0, 0));
       }
     } else {
 #pragma unroll
       for (int u = 0; u < NV; ++u) {
-        const int f = (int)threadIdx.x + u * 256;
+        const int f = vector(u);
         int row = f / PER_ROW, c = (f - row * PER_ROW) * V;
         row = row < n ? row : n - 1;
         const T* q = p + row * step;
@@ -191,7 +196,7 @@ template <typename T, int DA, bool FAST> struct Tile {
     const bool all = n == kChunk && da == DA;
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
-      const int f = (int)threadIdx.x + u * 256, row = f / PER_ROW, c = (f - row * PER_ROW) * V;
+      const int f = vector(u), row = f / PER_ROW, c = (f - row * PER_ROW) * V;
       vec_t w = v[u];
       if (!all) {
 #pragma unroll
@@ -206,13 +211,16 @@ template <typename T, int DA, bool FAST> struct Tile {
 // the scheduler puts every read right in front of its use, and the wavefront waits for LDS in every step.
 __device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0); }
 
+// v, computed where it stands: what depends on it is not kept in registers over the loop around it.
+__device__ __forceinline__ uint32_t here(uint32_t v) { asm volatile("" : "+v"(v)); return v; }
+
 // c of a chunk of n >= 1 tokens, in the layout of a right operand: register r of tile jt is token 16 jt + 4 g + r, in column
 // `col`. `take` makes tokens behind the n-th 0.
 template <typename T, bool FAST>
 __device__ __forceinline__ void load_c(T (&c)[2][4], const T* p, int64_t step, int n, int g, int col, int width) {
   if constexpr (FAST) {
     const Chunk k = chunk_of(p, step, n, width);
-    const uint32_t off = (uint32_t)((4 * g * (int)step + col) * (int)sizeof(T));
+    const uint32_t off = here((uint32_t)((4 * g * (int)step + col) * (int)sizeof(T)));
 #pragma unroll
     for (int jt = 0; jt < 2; ++jt)
 #pragma unroll
@@ -247,7 +255,7 @@ template <typename T, typename A, bool FAST>
 __device__ __forceinline__ void put_o(const A (&o)[2], T* p, int64_t step, int n, int g, int col, int width) {
   if constexpr (FAST) {
     const Chunk k = chunk_of(p, step, n, width);
-    const uint32_t off = (uint32_t)((4 * g * (int)step + col) * (int)sizeof(T));
+    const uint32_t off = here((uint32_t)((4 * g * (int)step + col) * (int)sizeof(T)));
 #pragma unroll
     for (int it = 0; it < 2; ++it)
 #pragma unroll
@@ -309,7 +317,7 @@ template <typename T> __device__ __forceinline__ First<T> first_state(const Role
 typedef double acc64 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ acc64 mma64(double a, double b, acc64 c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ int row64(int r) { return 4 * (r & 3) + (r >> 2); }
-constexpr int kCols64 = 64;    // columns of a workgroup
+constexpr int kWaves64 = 4, kCols64 = 16 * kWaves64;    // wavefronts and columns of a workgroup
 
 __device__ __forceinline__ void four(const double* lds, double (&out)[4]) {
   typedef double d2 __attribute__((ext_vector_type(2)));
@@ -333,7 +341,7 @@ __device__ __forceinline__ void add_tokens64(acc64 (&S)[DA / 16], const double* 
 }
 
 template <int DA, bool BACK, bool FAST>
-__global__ __launch_bounds__(256) void chunks_f64(Role<double> p, Plan<double> pl) {
+__global__ __launch_bounds__(256, DA <= 64 ? 2 : 1) void chunks_f64(Role<double> p, Plan<double> pl) {
   constexpr int KT = DA / 16, PITCH = DA + 2, APITCH = kChunk + 2;
   constexpr int after = BACK ? 0 : 1;
   constexpr int BUFS = (4 * kChunk * PITCH + kChunk * APITCH) * 8 <= kLds ? 2 : 1;
@@ -361,7 +369,7 @@ __global__ __launch_bounds__(256) void chunks_f64(Role<double> p, Plan<double> p
   weights(wt, p.scale_b, ld, kChunk, after, g);
   double lam = power(ld, (int64_t)kChunk);
 
-  Tile<double, DA, FAST> a, k;
+  Tile<double, DA, FAST, 256> a, k;
   double c[2][4], cn[2][4];
   a.prepare(path.ta);
   k.prepare(path.tk);
@@ -499,7 +507,7 @@ __global__ __launch_bounds__(256) void sums_f64(Role<double> p, Plan<double> pl)
   double wt[2][4];
   weights(wt, p.scale_b, ld, kChunk, after, g);
   double lam = power(ld, (int64_t)kChunk);
-  Tile<double, DA, FAST> k;
+  Tile<double, DA, FAST, 256> k;
   double c[2][4], cn[2][4];
   k.prepare(path.tk);
   auto fetch = [&](int64_t at) {
@@ -581,7 +589,7 @@ __device__ __forceinline__ acc32 mma6(const bf8 (&x)[3], const bf8 (&y)[3], acc3
 template <int DA> struct Pieces {
   static constexpr int PITCH = DA + 16;
   __bf16 at[3][kChunk * PITCH];
-  template <bool FAST> __device__ __forceinline__ void fill(const Tile<float, DA, FAST>& t, int n, int da) {
+  template <typename TILE> __device__ __forceinline__ void fill(const TILE& t, int n, int da) {
     t.store(n, da, [&](int row, int c, f32x4 v) {
       const float x[4] = {v[0], v[1], v[2], v[3]};
       bf4 q[3];
@@ -609,72 +617,59 @@ template <int DA> struct Pieces {
   }
 };
 
-// S <- e^{g N} S + b^T (w c) of a wavefront's CT column tiles, c given weighted.
-template <int DA, int CT>
-__device__ __forceinline__ void add_tokens32(acc32 (&S)[CT][DA / 16], const Pieces<DA>& sB, const float (&wc)[CT][2][4], float lam, int g, int lr) {
-  bf8 x[2][3], y[CT][3];
-  sB.tokens8(0, 0, g, lr, x[0]);
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    const float v[8] = {wc[ct][0][0], wc[ct][0][1], wc[ct][0][2], wc[ct][0][3], wc[ct][1][0], wc[ct][1][1], wc[ct][1][2], wc[ct][1][3]};
-    split(v, y[ct]);
-  }
+// S <- e^{g N} S + b^T (w c) of a wavefront's 16 columns, c given weighted.
+template <int DA>
+__device__ __forceinline__ void add_tokens32(acc32 (&S)[DA / 16], const Pieces<DA>& sB, const float (&wc)[2][4], float lam, int g, int lr) {
+  const float v[8] = {wc[0][0], wc[0][1], wc[0][2], wc[0][3], wc[1][0], wc[1][1], wc[1][2], wc[1][3]};
+  bf8 y[3];
+  split(v, y);
 #pragma unroll
   for (int kt = 0; kt < DA / 16; ++kt) {
-    if (kt + 1 < DA / 16) sB.tokens8((kt + 1) >> 1, (kt + 1) & 1, g, lr, x[(kt + 1) & 1]);
-    pin();
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) S[ct][kt] = mma6(x[kt & 1], y[ct], S[ct][kt] * lam);
-    pin();
+    bf8 x[3];
+    sB.tokens8(kt >> 1, kt & 1, g, lr, x);
+    S[kt] = mma6(x, y, S[kt] * lam);
   }
 }
 
-template <int DA, int CT, bool BACK, bool FAST>
-__global__ __launch_bounds__(256, 2) void chunks_f32(Role<float> p, Plan<float> pl) {
+// Wavefronts of a workgroup: eight for 128 columns, four for 64. A chunk is a chain (LDS, split, product, barrier) that one
+// wavefront spends mostly waiting in, so the registers are held down to let four share a SIMD wherever LDS has room for their
+// workgroups. 4 x 4096 tokens, 16 heads of 128 x 128: 145 us of 112 that q, k, v and o take at a copy's rate, 2.1 GHz,
+// vector instructions 58 % and matrix instructions 40 % of the cycles; with two tiles of columns a wavefront, and half the
+// wavefronts, 168 us.
+template <int DA, int WAVES> constexpr int kWaves = WAVES == 8 ? (DA <= 128 ? 4 : 2) : (DA <= 32 ? 4 : DA <= 64 ? 3 : 2);
+
+template <int DA, int WAVES, bool BACK, bool FAST>
+__global__ __launch_bounds__(64 * WAVES, (kWaves<DA, WAVES>)) void chunks_f32(Role<float> p, Plan<float> pl) {
   constexpr int KT = DA / 16, APITCH = kChunk + 8;
   constexpr int after = BACK ? 0 : 1;
   __shared__ __attribute__((aligned(16))) Pieces<DA> sQ, sB;
   __shared__ __attribute__((aligned(16))) __bf16 sA[3][kChunk * APITCH];
+  __shared__ float sP[kChunk + 1];                          // e^{g n}: read when wanted, for the registers' sake
   const Work w = work_of(pl, pl.segments);
   if (!w.live) return;
   const Path<float, BACK> path(p, w.group, w.segment * pl.seg_tokens, pl.seg_tokens);
   const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63, g = lane >> 4, lr = lane & 15;
-  int col[CT], ccol[CT];
-  bool live[CT];
-  acc32 S[CT][KT];
+  const int col = (w.slice * WAVES + wave) * 16 + lr;
+  const bool live = col < p.dc;
+  const int ccol = live ? col : p.dc - 1;
+  acc32 S[KT];
   const First<float> s0 = first_state(p, pl, w, path.b, path.h);
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    col[ct] = ((w.slice * 4 + wave) * CT + ct) * 16 + lr;
-    live[ct] = col[ct] < p.dc;
-    ccol[ct] = live[ct] ? col[ct] : p.dc - 1;
+  for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int d = 32 * (kt >> 1) + 8 * g + 4 * (kt & 1) + r;
-        S[ct][kt][r] = (s0.p && live[ct] && d < p.da) ? s0.p[d * s0.r + col[ct] * s0.c] : 0.0f;
-      }
-  }
+    for (int r = 0; r < 4; ++r) {
+      const int d = 32 * (kt >> 1) + 8 * g + 4 * (kt & 1) + r;
+      S[kt][r] = (s0.p && live && d < p.da) ? s0.p[d * s0.r + col * s0.c] : 0.0f;
+    }
   const float ld = p.log_decay[path.h];
-  // reach: of rows 4 g + r of o, `half` times that of rows 16 + 4 g + r; keep: the weights of tokens 16 + 4 g + r, `half` times
-  // that of tokens 4 g + r
-  const int at_it = wave ? 1 : 0, at_jt = wave == 2 ? 1 : 0;  // this wavefront's tile of A: (0, 0), (1, 0), (1, 1); the fourth has none
-  float reach[4], mask[4], keep[4];
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    reach[r] = p.scale_a * power(ld, (int64_t)(4 * g + r + after));
-    const int apart = 16 * (at_it - at_jt) + lr - 4 * g - r;
-    mask[r] = apart >= 0 ? p.scale_a * p.scale_b * power(ld, (int64_t)apart) : 0.0f;
-    keep[r] = p.scale_b * power(ld, (int64_t)(16 - after - 4 * g - r));
-  }
-  const float half = power(ld, (int64_t)16);
-  float lam = power(ld, (int64_t)kChunk);
+  const int at_it = wave ? 1 : 0, at_jt = wave == 2 ? 1 : 0;  // the first three wavefronts' tiles of A: (0, 0), (1, 0), (1, 1)
+  if ((int)threadIdx.x <= kChunk) sP[threadIdx.x] = power(ld, (int64_t)threadIdx.x);
+  const float ab = p.scale_a * p.scale_b;
   // A's rows 0 .. 15 have no tokens 16 .. 31: zeros once
-  for (int i = (int)threadIdx.x; i < 3 * 16 * APITCH; i += 256) sA[i / (16 * APITCH)][i % (16 * APITCH)] = (__bf16)0.0f;
+  for (int i = (int)threadIdx.x; i < 3 * 16 * APITCH; i += 64 * WAVES) sA[i / (16 * APITCH)][i % (16 * APITCH)] = (__bf16)0.0f;
 
-  Tile<float, DA, FAST> a, k;
-  float c[CT][2][4];
+  Tile<float, DA, FAST, 64 * WAVES> a, k;
+  float c[2][4];
   a.prepare(path.ta);
   k.prepare(path.tk);
   auto fetch = [&](int64_t at) {
@@ -690,120 +685,87 @@ __global__ __launch_bounds__(256, 2) void chunks_f32(Role<float> p, Plan<float> 
     sQ.fill(a, m, p.da);
     sB.fill(k, m, p.da);
     // (c is wanted behind the next barrier but one, far enough away for its loads)
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) load_c<float, FAST>(c[ct], path.c + at * path.tc, path.tc, m, g, ccol[ct], p.dc);
+    load_c<float, FAST>(c, path.c + at * path.tc, path.tc, m, g, ccol, p.dc);
     __syncthreads();
     if (wave < 3) {                                         // a tile of A, transposed
-      const int it = at_it, jt = at_jt;
       acc32 t = (acc32)(0.0f);
-      bf8 x[2][3], y[2][3];
-      sB.row8(16 * jt + lr, 8 * g, x[0]);
-      sQ.row8(16 * it + lr, 8 * g, y[0]);
 #pragma unroll
       for (int kt = 0; kt < DA / 32; ++kt) {
-        if (kt + 1 < DA / 32) {
-          sB.row8(16 * jt + lr, 32 * (kt + 1) + 8 * g, x[(kt + 1) & 1]);
-          sQ.row8(16 * it + lr, 32 * (kt + 1) + 8 * g, y[(kt + 1) & 1]);
-        }
-        pin();
-        t = mma6(x[kt & 1], y[kt & 1], t);
-        pin();
+        bf8 x[3], y[3];
+        sB.row8(16 * at_jt + lr, 32 * kt + 8 * g, x);
+        sQ.row8(16 * at_it + lr, 32 * kt + 8 * g, y);
+        t = mma6(x, y, t);
       }
       float v[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const bool under = it > jt || lr >= 4 * g + r;      // a choice, not a product with 0: the term above may be a NaN
-        v[r] = under ? t[r] * mask[r] : 0.0f;
+        const int apart = 16 * (at_it - at_jt) + lr - 4 * g - r;
+        v[r] = apart >= 0 ? t[r] * (ab * sP[apart > 0 ? apart : 0]) : 0.0f;   // a choice, not a product with 0: the term above may be a NaN
       }
       bf4 q[3];
       split(v, q);
 #pragma unroll
-      for (int i = 0; i < 3; ++i) *(bf4*)(sA[i] + (16 * it + lr) * APITCH + 8 * g + 4 * jt) = q[i];
+      for (int i = 0; i < 3; ++i) *(bf4*)(sA[i] + (16 * at_it + lr) * APITCH + 8 * g + 4 * at_jt) = q[i];
     }
-    acc32 o[CT][2];
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) o[ct][0] = o[ct][1] = (acc32)(0.0f);
+    acc32 o[2];
+    o[0] = o[1] = (acc32)(0.0f);
 #pragma unroll
     for (int kt = 0; kt < DA / 32; ++kt) {
-      bf8 x[2][3];
-      sQ.row8(lr, 32 * kt + 8 * g, x[0]);
-      sQ.row8(16 + lr, 32 * kt + 8 * g, x[1]);
-      pin();                                                // (the reads arrive while S is split)
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        const float v[8] = {S[ct][2 * kt][0], S[ct][2 * kt][1], S[ct][2 * kt][2], S[ct][2 * kt][3],
-                            S[ct][2 * kt + 1][0], S[ct][2 * kt + 1][1], S[ct][2 * kt + 1][2], S[ct][2 * kt + 1][3]};
-        bf8 y[3];
-        split(v, y);
-        o[ct][0] = mma6(x[0], y, o[ct][0]);
-        o[ct][1] = mma6(x[1], y, o[ct][1]);
-      }
+      const float v[8] = {S[2 * kt][0], S[2 * kt][1], S[2 * kt][2], S[2 * kt][3], S[2 * kt + 1][0], S[2 * kt + 1][1], S[2 * kt + 1][2], S[2 * kt + 1][3]};
+      bf8 x[3], y[3];
+      sQ.row8(lr, 32 * kt + 8 * g, x);
+      split(v, y);
+      o[0] = mma6(x, y, o[0]);
+      sQ.row8(16 + lr, 32 * kt + 8 * g, x);
+      o[1] = mma6(x, y, o[1]);
     }
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct)
+    for (int it = 0; it < 2; ++it)
 #pragma unroll
-      for (int it = 0; it < 2; ++it)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) o[ct][it][r] *= it ? reach[r] * half : reach[r];
-    if (next < path.total) fetch(next);
+      for (int r = 0; r < 4; ++r) o[it][r] *= p.scale_a * sP[16 * it + 4 * g + r + after];
     __syncthreads();
     {
-      bf8 x[2][3];
+      take(c, c, m, g);
+      const float v[8] = {c[0][0], c[0][1], c[0][2], c[0][3], c[1][0], c[1][1], c[1][2], c[1][3]};
+      bf8 x[3], y[3];
 #pragma unroll
-      for (int it = 0; it < 2; ++it)
+      for (int i = 0; i < 3; ++i) x[i] = *(const bf8*)(sA[i] + lr * APITCH + 8 * g);
+      split(v, y);
+      o[0] = mma6(x, y, o[0]);
 #pragma unroll
-        for (int i = 0; i < 3; ++i) x[it][i] = *(const bf8*)(sA[i] + (16 * it + lr) * APITCH + 8 * g);
-      pin();
+      for (int i = 0; i < 3; ++i) x[i] = *(const bf8*)(sA[i] + (16 + lr) * APITCH + 8 * g);
+      o[1] = mma6(x, y, o[1]);
+    }
+    if (live) put_o<float, acc32, FAST>(o, path.o + at * path.to, path.to, m, g, col, p.dc);
+    if (next < path.total) fetch(next);                     // (not earlier: its registers are wanted until here)
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        take(c[ct], c[ct], m, g);
-        const float v[8] = {c[ct][0][0], c[ct][0][1], c[ct][0][2], c[ct][0][3], c[ct][1][0], c[ct][1][1], c[ct][1][2], c[ct][1][3]};
-        bf8 y[3];
-        split(v, y);
-        o[ct][0] = mma6(x[0], y, o[ct][0]);
-        o[ct][1] = mma6(x[1], y, o[ct][1]);
+    for (int jt = 0; jt < 2; ++jt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int e = m - after - (16 * jt + 4 * g + r);
+        c[jt][r] *= p.scale_b * sP[e > 0 ? e : 0];
       }
-    }
-    float wt[2][4];
-    if (m < kChunk) {
-      weights(wt, p.scale_b, ld, m, after, g);
-      lam = power(ld, (int64_t)m);
-    } else {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) { wt[1][r] = keep[r]; wt[0][r] = keep[r] * half; }
-    }
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      if (live[ct]) put_o<float, acc32, FAST>(o[ct], path.o + at * path.to, path.to, m, g, col[ct], p.dc);
-#pragma unroll
-      for (int jt = 0; jt < 2; ++jt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) c[ct][jt][r] *= wt[jt][r];
-    }
-    add_tokens32<DA, CT>(S, sB, c, lam, g, lr);
+    add_tokens32<DA>(S, sB, c, sP[m], g, lr);
   }
   // (the compiler would keep every row's offset from the loads of the first state to here, in registers the loop needs)
   int ge = g;
   asm volatile("" : "+v"(ge));
+  if (!live) return;
+  zero_tail(p, path, g, col);
+  if (p.s1 && w.segment == pl.segments - 1) {
+    float* s1 = p.s1 + path.b * p.s1_b + path.h * p.s1_h + col * p.s1_c;
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    if (!live[ct]) continue;
-    zero_tail(p, path, g, col[ct]);
-    if (p.s1 && w.segment == pl.segments - 1) {
-      float* s1 = p.s1 + path.b * p.s1_b + path.h * p.s1_h + col[ct] * p.s1_c;
+    for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int d = 32 * (kt >> 1) + 8 * ge + 4 * (kt & 1) + r;
-          if (d < p.da) s1[d * p.s1_r] = S[ct][kt][r];
-        }
-    }
+      for (int r = 0; r < 4; ++r) {
+        const int d = 32 * (kt >> 1) + 8 * ge + 4 * (kt & 1) + r;
+        if (d < p.da) s1[d * p.s1_r] = S[kt][r];
+      }
   }
 }
 
-template <int DA, int CT, bool BACK, bool FAST>
-__global__ __launch_bounds__(256, 2) void sums_f32(Role<float> p, Plan<float> pl) {
+template <int DA, int WAVES, bool BACK, bool FAST>
+__global__ __launch_bounds__(64 * WAVES, (kWaves<DA, WAVES>)) void sums_f32(Role<float> p, Plan<float> pl) {
   constexpr int KT = DA / 16;
   constexpr int after = BACK ? 0 : 1;
   __shared__ __attribute__((aligned(16))) Pieces<DA> sB[2];
@@ -811,27 +773,22 @@ __global__ __launch_bounds__(256, 2) void sums_f32(Role<float> p, Plan<float> pl
   if (!w.live) return;
   const Path<float, BACK> path(p, w.group, w.segment * pl.part_tokens, pl.part_tokens);
   const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63, g = lane >> 4, lr = lane & 15;
-  int col[CT], ccol[CT];
-  acc32 S[CT][KT];
+  const int col = (w.slice * WAVES + wave) * 16 + lr;
+  const int ccol = col < p.dc ? col : p.dc - 1;
+  acc32 S[KT];
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    col[ct] = ((w.slice * 4 + wave) * CT + ct) * 16 + lr;
-    ccol[ct] = col[ct] < p.dc ? col[ct] : p.dc - 1;
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt) S[ct][kt] = (acc32)(0.0f);
-  }
+  for (int kt = 0; kt < KT; ++kt) S[kt] = (acc32)(0.0f);
   const float ld = p.log_decay[path.h];
   float wt[2][4];
   weights(wt, p.scale_b, ld, kChunk, after, g);
   float lam = power(ld, (int64_t)kChunk);
-  Tile<float, DA, FAST> k;
-  float c[CT][2][4], cn[CT][2][4];
+  Tile<float, DA, FAST, 64 * WAVES> k;
+  float c[2][4], cn[2][4];
   k.prepare(path.tk);
   auto fetch = [&](int64_t at) {
     const int m = path.tokens(at);
     k.load(path.k + at * path.tk, path.tk, m, p.da);
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) load_c<float, FAST>(cn[ct], path.c + at * path.tc, path.tc, m, g, ccol[ct], p.dc);
+    load_c<float, FAST>(cn, path.c + at * path.tc, path.tc, m, g, ccol, p.dc);
   };
   if (path.total > 0) fetch(0);
   int turn = 0;
@@ -839,30 +796,24 @@ __global__ __launch_bounds__(256, 2) void sums_f32(Role<float> p, Plan<float> pl
     const int m = path.tokens(at);
     sB[turn].fill(k, m, p.da);                              // (two buffers: one barrier a chunk)
     if (m < kChunk) { weights(wt, p.scale_b, ld, m, after, g); lam = power(ld, (int64_t)m); }
+    take(c, cn, m, g);
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      take(c[ct], cn[ct], m, g);
+    for (int jt = 0; jt < 2; ++jt)
 #pragma unroll
-      for (int jt = 0; jt < 2; ++jt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) c[ct][jt][r] *= wt[jt][r];
-    }
+      for (int r = 0; r < 4; ++r) c[jt][r] *= wt[jt][r];
     __syncthreads();
     if (at + kChunk < path.total) fetch(at + kChunk);
-    add_tokens32<DA, CT>(S, sB[turn], c, lam, g, lr);
+    add_tokens32<DA>(S, sB[turn], c, lam, g, lr);
   }
+  if (col >= p.dc) return;
+  float* s1 = pl.states + ((int64_t)w.group * pl.slots + w.segment + 1) * p.da * p.dc + col;
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    if (col[ct] >= p.dc) continue;
-    float* s1 = pl.states + ((int64_t)w.group * pl.slots + w.segment + 1) * p.da * p.dc + col[ct];
+  for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int d = 32 * (kt >> 1) + 8 * g + 4 * (kt & 1) + r;
-        if (d < p.da) s1[(int64_t)d * p.dc] = S[ct][kt][r];
-      }
-  }
+    for (int r = 0; r < 4; ++r) {
+      const int d = 32 * (kt >> 1) + 8 * g + 4 * (kt & 1) + r;
+      if (d < p.da) s1[(int64_t)d * p.dc] = S[kt][r];
+    }
 }
 
 // From the parts' shares to the states in front of the segments (the slots at multiples of `parts`): one lane per element of
@@ -903,9 +854,9 @@ __global__ __launch_bounds__(256) void segment_states(Role<T> p, Plan<T> pl) {
   while (k < pl.slots) carry<T, 8>(at, per, k, s, ld, n, pl);
 }
 
-static int workgroups_per_cu(const void* kernel) {
+static int workgroups_per_cu(const void* kernel, int threads) {
   int n = 0;
-  if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, 256, 0) != hipSuccess || n < 1) { (void)hipGetLastError(); n = 1; }
+  if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0) != hipSuccess || n < 1) { (void)hipGetLastError(); n = 1; }
   return n;
 }
 
@@ -919,9 +870,11 @@ template <typename T> struct Segments {
   bool made = false;
 };
 
-// cols: columns of a workgroup
+// A wavefront takes 16 columns.
 template <typename T, Kernel<T> CHUNKS, Kernel<T> SUMS>
-static int run_chunks(const Role<T>& p, Segments<T>& seg, int cols) {
+static int run_chunks(const Role<T>& p, Segments<T>& seg, int waves) {
+  const int cols = 16 * waves;
+  const dim3 block((unsigned)(64 * waves));
   Plan<T>& pl = seg.plan;
   pl.slices = (p.dc + cols - 1) / cols;
   if (seg.made) {
@@ -931,9 +884,12 @@ static int run_chunks(const Role<T>& p, Segments<T>& seg, int cols) {
     pl.st_r = p.dc; pl.st_c = 1;
     const int64_t wgs = (int64_t)pl.groups * pl.slices;
     const int64_t n_chunks = (p.tokens + kChunk - 1) / kChunk;
-    // As many segments as the device has room for workgroups, of two chunks at least.
-    static const int room = workgroups_per_cu((const void*)CHUNKS), sums_room = workgroups_per_cu((const void*)SUMS);
-    int64_t segments = (int64_t)room * num_cus() / wgs;
+    // As many segments as the device has room for workgroups, up to two of eight wavefronts or three of four on a CU (more
+    // win nothing: 32 x 1024 tokens, 16 heads of 64 x 64 in one segment, two workgroups a CU, take 124 us, in two segments
+    // 173); a segment has two chunks at least.
+    static const int room = workgroups_per_cu((const void*)CHUNKS, 64 * waves), sums_room = workgroups_per_cu((const void*)SUMS, 64 * waves);
+    const int a_cu = waves == 8 ? 2 : 3;
+    int64_t segments = (int64_t)(room < a_cu ? room : a_cu) * num_cus() / wgs;
     if (segments > n_chunks / 2) segments = n_chunks / 2;
     if (segments < 1) segments = 1;
     int64_t per_segment = n_chunks ? (n_chunks + segments - 1) / segments : 1;
@@ -954,7 +910,7 @@ static int run_chunks(const Role<T>& p, Segments<T>& seg, int cols) {
       AM_TRY(seg.states.take((size_t)pl.groups * pl.slots * p.da * p.dc * sizeof(T)));
       pl.states = (T*)seg.states.p;
       const int64_t ids = ((int64_t)pl.groups * (pl.slots - 1) + 7) / 8 * 8 * pl.slices;
-      hipLaunchKernelGGL(SUMS, dim3((unsigned)ids), dim3(256), 0, stream(), p, pl);
+      hipLaunchKernelGGL(SUMS, dim3((unsigned)ids), block, 0, stream(), p, pl);
       AM_TRY(check_launch("decay attention: sums"));
       hipLaunchKernelGGL((segment_states<T>), dim3((unsigned)(pl.groups * ((p.da * p.dc + 255) / 256))), dim3(256), 0, stream(), p, pl);
       AM_TRY(check_launch("decay attention: states"));
@@ -962,20 +918,20 @@ static int run_chunks(const Role<T>& p, Segments<T>& seg, int cols) {
     seg.made = true;
   }
   const int64_t ids = ((int64_t)pl.groups * pl.segments + 7) / 8 * 8 * pl.slices;
-  hipLaunchKernelGGL(CHUNKS, dim3((unsigned)ids), dim3(256), 0, stream(), p, pl);
+  hipLaunchKernelGGL(CHUNKS, dim3((unsigned)ids), block, 0, stream(), p, pl);
   return check_launch("decay attention: chunks");
 }
 
 template <int DA, bool BACK, bool FAST> static int run_sized(const Role<double>& p, Segments<double>& seg) {
-  return run_chunks<double, chunks_f64<DA, BACK, FAST>, sums_f64<DA, BACK, FAST>>(p, seg, kCols64);
+  return run_chunks<double, chunks_f64<DA, BACK, FAST>, sums_f64<DA, BACK, FAST>>(p, seg, kWaves64);
 }
-// A wavefront takes two tiles of 16 columns where there are more than 64 (a's and b's pieces are then read from LDS once for
-// both), unless the workgroups of 128 columns leave CUs without work however short their segments.
+// Eight wavefronts where there are more than 64 columns (a and b are then split and staged once for all), unless the workgroups
+// of 128 columns leave CUs without work however short their segments.
 template <int DA, bool BACK, bool FAST> static int run_sized(const Role<float>& p, Segments<float>& seg) {
   const int64_t pairs = (p.tokens + 2 * kChunk - 1) / (2 * kChunk);
   const bool wide = p.dc > 64 && p.batch * p.heads * ((p.dc + 127) / 128) * (pairs > 1 ? pairs : 1) >= num_cus();
-  if (!wide) return run_chunks<float, chunks_f32<DA, 1, BACK, FAST>, sums_f32<DA, 1, BACK, FAST>>(p, seg, 64);
-  return run_chunks<float, chunks_f32<DA, 2, BACK, FAST>, sums_f32<DA, 2, BACK, FAST>>(p, seg, 128);
+  if (!wide) return run_chunks<float, chunks_f32<DA, 4, BACK, FAST>, sums_f32<DA, 4, BACK, FAST>>(p, seg, 4);
+  return run_chunks<float, chunks_f32<DA, 8, BACK, FAST>, sums_f32<DA, 8, BACK, FAST>>(p, seg, 8);
 }
 
 template <bool BACK, bool FAST, typename T> static int run_fast(const Role<T>& p, Segments<T>& seg) {
