@@ -24,7 +24,8 @@ import numpy as np
 
 from . import _lib
 from ._lib import ACT, ROTARY, check
-from .tensor_hip import HipTensor, _same_dtype, empty, toHip, zeros
+from .metadata import Layout
+from .tensor_hip import HipStorage, HipTensor, _same_dtype, toHip, zeros
 
 _INT64 = np.dtype(np.int64)
 _FLOAT64 = np.dtype(np.float64)
@@ -45,6 +46,15 @@ def _entry(name: str, t: HipTensor):
     return fn
 
 
+def _new(shape, dtype) -> HipTensor:
+    """`empty` for a shape of ints and a float dtype that have been looked at already: a small operator's call is mostly host time."""
+    strides, n = [], 1
+    for d in reversed(shape):
+        strides.append(n)
+        n *= d
+    return HipTensor(Layout(shape, tuple(strides[::-1]), 0), HipStorage(n, dtype.itemsize), dtype)
+
+
 def _unit_rows(t: HipTensor) -> HipTensor:
     """`t`, or a copy of it, with unit stride in the last dimension."""
     lay = t.layout
@@ -52,7 +62,7 @@ def _unit_rows(t: HipTensor) -> HipTensor:
 
 
 def _shape(name: str, what: str, t: HipTensor, shape):
-    if t.shape != shape:
+    if t.layout.shape != shape:
         raise ValueError(f"{name}: {what} of shape {list(t.shape)}, {list(shape)} expected")
 
 
@@ -90,9 +100,10 @@ def rotary_frequencies(rot_dim: int, base: float = 10000.0, scaling: str = "none
 
 def _rotate(name, out: HipTensor | None, x: HipTensor, positions: HipTensor | None, frequencies: HipTensor, layout: str, scale: float, inverse: int):
     fn = _entry("rotary", x)
-    if x.rank != 4:
+    shape = x.layout.shape
+    if len(shape) != 4:
         raise ValueError(f"{name}: a tensor [batch, tokens, heads, dim] is needed, not one of rank {x.rank}")
-    B, T, H, D = x.shape
+    B, T, H, D = shape
     if out is not None:
         _same_dtype(x, out)
         _shape(name, "a result", out, x.shape)
@@ -100,28 +111,27 @@ def _rotate(name, out: HipTensor | None, x: HipTensor, positions: HipTensor | No
             raise ValueError(f"{name}: the last dimension of the result needs unit stride")
     if layout not in ROTARY:
         raise ValueError(f"{name}: unknown layout {layout!r}, one of {', '.join(ROTARY)}")
-    if frequencies.dtype != _FLOAT64 or frequencies.rank != 1 or not frequencies.is_C_contiguous():
+    if frequencies.dtype != _FLOAT64 or frequencies.rank != 1 or (frequencies.strides[0] != 1 and frequencies.size > 1):
         raise TypeError(f"{name}: frequencies must be a contiguous float64 vector (rotary_frequencies makes one)")
-    R = 2 * frequencies.shape[0]
+    R = 2 * frequencies.layout.shape[0]
     if R > D:
         raise ValueError(f"{name}: {R} turning elements in a head of {D}")
     pp, pb, pt = None, 0, 0
     if positions is not None:
         if positions.dtype != _INT64:
             raise TypeError(f"{name}: positions must be int64, not {positions.dtype}")
-        if positions.shape == (T,):
-            pt = positions.strides[0]
-        elif positions.shape == (B, T):
-            pb, pt = positions.strides
+        lay = positions.layout
+        if lay.shape == (B, T):
+            pb, pt = lay.strides
+        elif lay.shape == (T,):
+            pt = lay.strides[0]
         else:
             raise ValueError(f"{name}: positions of shape {list(positions.shape)} for {B} sequences of {T} tokens")
         pp = positions.data_ptr()
     if out is None:
-        out = empty(x.shape, x.dtype)
+        out = _new(shape, x.dtype)
     src = x if x is out else _unit_rows(x)
-    xs, os = src.strides, out.strides
-    check(fn(B, T, H, D, R, ROTARY[layout], inverse, scale, pp, pb, pt, frequencies.data_ptr(), src.data_ptr(), xs[0], xs[1], xs[2],
-             out.data_ptr(), os[0], os[1], os[2]))
+    check(fn(B, T, H, D, R, ROTARY[layout], inverse, scale, pp, pb, pt, frequencies.data_ptr(), *_rows(src), *_rows(out)))
     return out
 
 
@@ -147,13 +157,14 @@ def rotary_backward(gradient: HipTensor, positions: HipTensor | None, frequencie
 # ---------------------------------------------------------------------- linear attention with decay
 def _attention_sizes(name, q, k, v, log_decay, lead):
     """Checks q [*lead, heads, dk], k [*lead, kv_heads, dk], v [*lead, kv_heads, dv] and log_decay [heads]."""
-    if not (q.rank == k.rank == v.rank == lead + 2):
+    qs, ks, vs = q.layout.shape, k.layout.shape, v.layout.shape
+    if not (len(qs) == len(ks) == len(vs) == lead + 2):
         raise ValueError(f"{name}: q, k and v of rank {lead + 2} are needed, not {q.rank}, {k.rank} and {v.rank}")
     _same_dtype(q, k, v, log_decay)
-    front, H, dk = q.shape[:lead], q.shape[-2], q.shape[-1]
-    KH, dv = v.shape[-2:]
-    _shape(name, "k", k, front + (KH, dk))
-    _shape(name, "v", v, front + (KH, dv))
+    front, H, dk = qs[:lead], qs[lead], qs[lead + 1]
+    KH, dv = vs[lead:]
+    if ks != front + (KH, dk) or vs[:lead] != front:
+        raise ValueError(f"{name}: q {list(qs)}, k {list(ks)} and v {list(vs)} do not belong together")
     if H and (KH == 0 or H % KH):
         raise ValueError(f"{name}: {H} heads cannot share {KH} key / value heads evenly")
     _shape(name, "log_decay", log_decay, (H,))
@@ -196,8 +207,8 @@ def decay_attention(q: HipTensor, k: HipTensor, v: HipTensor, log_decay: HipTens
     (B, T), H, KH, dk, dv = _attention_sizes(name, q, k, v, log_decay, 2)
     s0 = _head_state(name, state, (B, H, dk, dv), q) if state is not None else (None, 0, 0)
     n = _lengths(name, lengths, B)
-    q, k, v, g = _unit_rows(q), _unit_rows(k), _unit_rows(v), log_decay.asContiguous()
-    out, end = empty((B, T, H, dv), q.dtype), empty((B, H, dk, dv), q.dtype)
+    q, k, v, g = _unit_rows(q), _unit_rows(k), _unit_rows(v), _unit_rows(log_decay)
+    out, end = _new((B, T, H, dv), q.dtype), _new((B, H, dk, dv), q.dtype)
     check(fn(B, T, H, KH, dk, dv, scale, g.data_ptr(), n, *_rows(q), *_rows(k), *_rows(v), *s0,
              *_rows(out), *_rows(end)[:3]))
     return out, end
@@ -217,9 +228,9 @@ def decay_attention_backward(gradOutput: HipTensor, q: HipTensor, k: HipTensor, 
     s0 = _head_state(name, state, (B, H, dk, dv), q) if state is not None else (None, 0, 0)
     gs = _head_state(name, gradState, (B, H, dk, dv), q) if gradState is not None else (None, 0, 0)
     n = _lengths(name, lengths, B)
-    q, k, v, do, g = _unit_rows(q), _unit_rows(k), _unit_rows(v), _unit_rows(gradOutput), log_decay.asContiguous()
-    dq, dkey, dval = empty((B, T, H, dk), q.dtype), empty((B, T, KH, dk), q.dtype), empty((B, T, KH, dv), q.dtype)
-    dstate = empty((B, H, dk, dv), q.dtype) if state is not None else None
+    q, k, v, do, g = _unit_rows(q), _unit_rows(k), _unit_rows(v), _unit_rows(gradOutput), _unit_rows(log_decay)
+    dq, dkey, dval = _new((B, T, H, dk), q.dtype), _new((B, T, KH, dk), q.dtype), _new((B, T, KH, dv), q.dtype)
+    dstate = _new((B, H, dk, dv), q.dtype) if state is not None else None
     check(fn(B, T, H, KH, dk, dv, scale, g.data_ptr(), n, *_rows(do), *_rows(q), *_rows(k), *_rows(v),
              *s0, *gs, *_rows(dq), *_rows(dkey), *_rows(dval), *(_rows(dstate)[:3] if dstate is not None else (None, 0, 0))))
     return dq, dkey, dval, dstate
@@ -232,8 +243,8 @@ def decay_attention_step(q: HipTensor, k: HipTensor, v: HipTensor, log_decay: Hi
     fn = _entry(name, q)
     (B,), H, KH, dk, dv = _attention_sizes(name, q, k, v, log_decay, 1)
     s = _head_state(name, state, (B, H, dk, dv), q)
-    q, k, v, g = _unit_rows(q), _unit_rows(k), _unit_rows(v), log_decay.asContiguous()
-    out = empty((B, H, dv), q.dtype)
+    q, k, v, g = _unit_rows(q), _unit_rows(k), _unit_rows(v), _unit_rows(log_decay)
+    out = _new((B, H, dv), q.dtype)
     check(fn(B, H, KH, dk, dv, scale, g.data_ptr(), *_rows(q), *_rows(k), *_rows(v), *s, *_rows(out)))
     return out
 
@@ -264,22 +275,25 @@ def _norm_sizes(name, x: HipTensor, weight, bias, groups: int, activation: str):
         raise ValueError(f"{name}: a tensor [batch, ..., channels] is needed")
     if activation not in ACT:
         raise ValueError(f"{name}: unknown activation {activation!r}, one of {', '.join(ACT)}")
-    C = x.shape[-1]
+    shape = x.layout.shape
+    C = shape[-1]
     spatial = 1
-    for d in x.shape[1:-1]:
+    for d in shape[1:-1]:
         spatial *= d
     if groups < 1 or C % groups:
         raise ValueError(f"{name}: {C} channels cannot form {groups} groups")
     for what, w in (("weight", weight), ("bias", bias)):
         if w is not None:
             _same_dtype(x, w)
-            if w.size != C or w.shape[-1] != C:
+            ws = w.layout.shape
+            if ws != (C,) and ws != (1, C):
                 raise ValueError(f"{name}: {what} of shape {list(w.shape)} for {C} channels")
-    return x.shape[0], spatial, C
+    return shape[0], spatial, C
 
 
 def _vector(t: HipTensor | None):
-    return None if t is None else t.asContiguous()
+    """`t` [channels] or [1, channels] with its channels next to each other."""
+    return t if t is None else _unit_rows(t)
 
 
 def _ptr(t: HipTensor | None):
@@ -291,10 +305,10 @@ def _normalise(name, x, weight, bias, groups, eps, activation, keep):
     B, S, C = _norm_sizes(name, x, weight, bias, groups, activation)
     src, sn, ss = _channels_last(x)
     w, b = _vector(weight), _vector(bias)
-    y = empty(x.shape, x.dtype)
+    y = _new(x.layout.shape, x.dtype)
     mean = rstd = None
     if keep:
-        make = empty if S * C else zeros
+        make = _new if S * C else zeros
         mean, rstd = make((B, groups), x.dtype), make((B, groups), x.dtype)
     check(fn(B, S, C, groups, eps, ACT[activation], src.data_ptr(), sn, ss, _ptr(w), _ptr(b), y.data_ptr(), S * C, C, _ptr(mean), _ptr(rstd)))
     return y, mean, rstd
@@ -329,9 +343,9 @@ def group_norm_backward(gradOutput: HipTensor, x: HipTensor, weight: HipTensor |
     src, xn, xs = _channels_last(x)
     dy, gn, gs = _channels_last(gradOutput)
     w, b, m, r = _vector(weight), _vector(bias), mean.asContiguous(), rstd.asContiguous()
-    dx = empty(x.shape, x.dtype)
-    dw = empty(weight.shape, x.dtype) if weight is not None else None
-    db = empty(bias.shape, x.dtype) if bias is not None else None
+    dx = _new(x.shape, x.dtype)
+    dw = _new(weight.shape, x.dtype) if weight is not None else None
+    db = _new(bias.shape, x.dtype) if bias is not None else None
     check(fn(B, S, C, groups, ACT[activation], dy.data_ptr(), gn, gs, src.data_ptr(), xn, xs, _ptr(w), _ptr(b), m.data_ptr(), r.data_ptr(),
              dx.data_ptr(), S * C, C, _ptr(dw), _ptr(db)))
     return dx, dw, db

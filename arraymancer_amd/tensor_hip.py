@@ -41,7 +41,7 @@ class HipStorage:
     def __init__(self, nelems: int, itemsize: int):
         L = _lib.load()
         out = ctypes.c_void_p()
-        check(L.am_hip_malloc(ctypes.c_size_t(nelems * itemsize), ctypes.byref(out)))
+        check(L.am_hip_malloc(nelems * itemsize, ctypes.byref(out)))
         self.ptr = out.value or 0
         self.nelems = nelems
         self.itemsize = itemsize
