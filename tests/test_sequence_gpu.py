@@ -198,6 +198,19 @@ def test_decay_attention_of_a_padded_batch(hip, size, dt):
 
 
 @pytest.mark.parametrize("dt", ["f32", "f64"])
+@pytest.mark.parametrize("size", [(2, 321, 4, 2, 64, 128), (2, 260, 8, 8, 64, 126), (1, 1411, 2, 1, 24, 40)], ids=str)
+def test_decay_attention_in_segments(hip, size, dt):
+    """Long enough to be cut into segments: states between them in vectors, in single elements, over many slots; a sequence that
+    ends within the first segments and one without tokens."""
+    x = attention_inputs(hip, size, dt, seed_of("segments", size, dt))
+    check_attention(hip, size, dt, x, given=True, padded=False, grads=True)
+    for short in (0, 70):
+        x["lengths"] = np.full(size[0], size[1], np.int64)
+        x["lengths"][-1] = short
+        check_attention(hip, size, dt, x, given=True, padded=True, grads=True)
+
+
+@pytest.mark.parametrize("dt", ["f32", "f64"])
 def test_decay_attention_of_no_tokens_and_of_extreme_decays(hip, dt):
     x = attention_inputs(hip, (2, 0, 2, 1, 6, 5), dt, 3)
     d = {n: hip.toHip(a) for n, a in x.items() if n not in ("scale", "lengths")}
