@@ -251,18 +251,18 @@ __device__ __forceinline__ void take(T (&c)[2][4], const T (&from)[2][4], int n,
 }
 
 // The lane's column of a chunk's result: register r of tile it is token 16 it + 4 g + r.
-template <typename T, typename A, bool FAST>
-__device__ __forceinline__ void put_o(const A (&o)[2], T* p, int64_t step, int n, int g, int col, int width) {
+template <typename T, typename A, bool FAST, int TILES>
+__device__ __forceinline__ void put_o(const A (&o)[TILES], T* p, int64_t step, int n, int g, int col, int width) {
   if constexpr (FAST) {
     const Chunk k = chunk_of(p, step, n, width);
     const uint32_t off = here((uint32_t)((4 * g * (int)step + col) * (int)sizeof(T)));
 #pragma unroll
-    for (int it = 0; it < 2; ++it)
+    for (int it = 0; it < TILES; ++it)
 #pragma unroll
       for (int r = 0; r < 4; ++r) put(k, off + (k.first + (uint32_t)((16 * it + r) * (int)step * (int)sizeof(T))), o[it][r]);
   } else {
 #pragma unroll
-    for (int it = 0; it < 2; ++it)
+    for (int it = 0; it < TILES; ++it)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int i = 16 * it + 4 * g + r;
@@ -468,7 +468,7 @@ __global__ __launch_bounds__(256, DA <= 64 ? 2 : 1) void chunks_f64(Role<double>
 #pragma unroll
       for (int r = 0; r < 4; ++r) c[jt][r] *= wt[jt][r];
     add_tokens64<DA>(S, sB, c, lam, pr, g);
-    if (live) put_o<double, acc64, FAST>(o, path.o + at * path.to, path.to, m, g, col, p.dc);
+    if (live) put_o<double, acc64, FAST, 2>(o, path.o + at * path.to, path.to, m, g, col, p.dc);
     // the next chunk into LDS: into the other buffer, or (where two do not fit) behind a barrier
     if constexpr (BUFS == 2) turn ^= 1;
     else __syncthreads();
@@ -617,39 +617,43 @@ template <int DA> struct Pieces {
   }
 };
 
-// S <- e^{g N} S + b^T (w c) of a wavefront's 16 columns, c given weighted.
-template <int DA>
-__device__ __forceinline__ void add_tokens32(acc32 (&S)[DA / 16], const Pieces<DA>& sB, const float (&wc)[2][4], float lam, int g, int lr) {
+// S <- e^{g N} S + b^T (w c) of a wavefront's 16 columns and its rows from 32 m on, c given weighted.
+template <int DA, int KT>
+__device__ __forceinline__ void add_tokens32(acc32 (&S)[KT], const Pieces<DA>& sB, const float (&wc)[2][4], float lam, int m, int g, int lr) {
   const float v[8] = {wc[0][0], wc[0][1], wc[0][2], wc[0][3], wc[1][0], wc[1][1], wc[1][2], wc[1][3]};
   bf8 y[3];
   split(v, y);
 #pragma unroll
-  for (int kt = 0; kt < DA / 16; ++kt) {
+  for (int kt = 0; kt < KT; ++kt) {
     bf8 x[3];
-    sB.tokens8(kt >> 1, kt & 1, g, lr, x);
+    sB.tokens8(m + (kt >> 1), kt & 1, g, lr, x);
     S[kt] = mma6(x, y, S[kt] * lam);
   }
 }
 
-// Wavefronts of a workgroup: eight for 128 columns, four for 64. A chunk is a chain (LDS, split, product, barrier) that one
-// wavefront spends mostly waiting in, so the registers are held down to let four share a SIMD wherever LDS has room for their
-// workgroups. 4 x 4096 tokens, 16 heads of 128 x 128: 145 us of 112 that q, k, v and o take at a copy's rate, 2.1 GHz,
-// vector instructions 58 % and matrix instructions 40 % of the cycles; with two tiles of columns a wavefront, and half the
-// wavefronts, 168 us.
+// Wavefronts of a workgroup: eight for 128 columns; four for 64, or eight that halve the rows of the state (HALVES): two of them
+// share columns, each adds up a S over its rows and finishes one of the two tiles of o. A chunk is a chain (LDS, split, product,
+// barrier) that one wavefront spends mostly waiting in, so the registers are held down to let four share a SIMD wherever LDS has
+// room for their workgroups. 4 x 4096 tokens, 16 heads of 128 x 128: 145 us of 112 that q, k, v and o take at a copy's rate,
+// 2.1 GHz, vector instructions 58 % and matrix instructions 40 % of the cycles, LDS about as much; with two tiles of columns a
+// wavefront, and half the wavefronts, 168 us; with the residues of `split` as two-element dot products (seven instructions for
+// two elements in place of eleven) the same 145.
 template <int DA, int WAVES> constexpr int kWaves = WAVES == 8 ? (DA <= 128 ? 4 : 2) : (DA <= 32 ? 4 : DA <= 64 ? 3 : 2);
 
-template <int DA, int WAVES, bool BACK, bool FAST>
+template <int DA, int WAVES, int HALVES, bool BACK, bool FAST>
 __global__ __launch_bounds__(64 * WAVES, (kWaves<DA, WAVES>)) void chunks_f32(Role<float> p, Plan<float> pl) {
-  constexpr int KT = DA / 16, APITCH = kChunk + 8;
+  constexpr int KT = DA / 16 / HALVES, CT = WAVES / HALVES, APITCH = kChunk + 8;
   constexpr int after = BACK ? 0 : 1;
   __shared__ __attribute__((aligned(16))) Pieces<DA> sQ, sB;
   __shared__ __attribute__((aligned(16))) __bf16 sA[3][kChunk * APITCH];
+  __shared__ __attribute__((aligned(16))) acc32 sX[HALVES == 2 ? WAVES : 1][64];
   __shared__ float sP[kChunk + 1];                          // e^{g n}: read when wanted, for the registers' sake
   const Work w = work_of(pl, pl.segments);
   if (!w.live) return;
   const Path<float, BACK> path(p, w.group, w.segment * pl.seg_tokens, pl.seg_tokens);
   const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63, g = lane >> 4, lr = lane & 15;
-  const int col = (w.slice * WAVES + wave) * 16 + lr;
+  const int half = HALVES == 2 ? wave / CT : 0, m0 = half * (KT / 2);
+  const int col = (w.slice * CT + wave % CT) * 16 + lr;
   const bool live = col < p.dc;
   const int ccol = live ? col : p.dc - 1;
   acc32 S[KT];
@@ -658,7 +662,7 @@ __global__ __launch_bounds__(64 * WAVES, (kWaves<DA, WAVES>)) void chunks_f32(Ro
   for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int d = 32 * (kt >> 1) + 8 * g + 4 * (kt & 1) + r;
+      const int d = 32 * (m0 + (kt >> 1)) + 8 * g + 4 * (kt & 1) + r;
       S[kt][r] = (s0.p && live && d < p.da) ? s0.p[d * s0.r + col * s0.c] : 0.0f;
     }
   const float ld = p.log_decay[path.h];
@@ -710,33 +714,43 @@ __global__ __launch_bounds__(64 * WAVES, (kWaves<DA, WAVES>)) void chunks_f32(Ro
     acc32 o[2];
     o[0] = o[1] = (acc32)(0.0f);
 #pragma unroll
-    for (int kt = 0; kt < DA / 32; ++kt) {
+    for (int kt = 0; kt < KT / 2; ++kt) {
       const float v[8] = {S[2 * kt][0], S[2 * kt][1], S[2 * kt][2], S[2 * kt][3], S[2 * kt + 1][0], S[2 * kt + 1][1], S[2 * kt + 1][2], S[2 * kt + 1][3]};
       bf8 x[3], y[3];
-      sQ.row8(lr, 32 * kt + 8 * g, x);
+      sQ.row8(lr, 32 * (m0 + kt) + 8 * g, x);
       split(v, y);
       o[0] = mma6(x, y, o[0]);
-      sQ.row8(16 + lr, 32 * kt + 8 * g, x);
+      sQ.row8(16 + lr, 32 * (m0 + kt) + 8 * g, x);
       o[1] = mma6(x, y, o[1]);
     }
-#pragma unroll
-    for (int it = 0; it < 2; ++it)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) o[it][r] *= p.scale_a * sP[16 * it + 4 * g + r + after];
+    // of two wavefronts on the same columns each finishes one of the tiles
+    acc32 e[2 / HALVES];
+    if constexpr (HALVES == 2) {
+      e[0] = half ? o[1] : o[0];
+      sX[wave][lane] = half ? o[0] : o[1];
+    } else {
+      e[0] = o[0];
+      e[1] = o[1];
+    }
     __syncthreads();
+    if constexpr (HALVES == 2) e[0] += sX[wave ^ CT][lane];
     {
       take(c, c, m, g);
       const float v[8] = {c[0][0], c[0][1], c[0][2], c[0][3], c[1][0], c[1][1], c[1][2], c[1][3]};
-      bf8 x[3], y[3];
-#pragma unroll
-      for (int i = 0; i < 3; ++i) x[i] = *(const bf8*)(sA[i] + lr * APITCH + 8 * g);
+      bf8 y[3];
       split(v, y);
-      o[0] = mma6(x, y, o[0]);
 #pragma unroll
-      for (int i = 0; i < 3; ++i) x[i] = *(const bf8*)(sA[i] + (16 + lr) * APITCH + 8 * g);
-      o[1] = mma6(x, y, o[1]);
+      for (int it = 0; it < 2 / HALVES; ++it) {
+        const int row = 16 * (half + it);
+        bf8 x[3];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) x[i] = *(const bf8*)(sA[i] + (row + lr) * APITCH + 8 * g);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) e[it][r] *= p.scale_a * sP[row + 4 * g + r + after];
+        e[it] = mma6(x, y, e[it]);
+      }
     }
-    if (live) put_o<float, acc32, FAST>(o, path.o + at * path.to, path.to, m, g, col, p.dc);
+    if (live && m > 16 * half) put_o<float, acc32, FAST, 2 / HALVES>(e, path.o + (at + 16 * half) * path.to, path.to, m - 16 * half, g, col, p.dc);
     if (next < path.total) fetch(next);                     // (not earlier: its registers are wanted until here)
 #pragma unroll
     for (int jt = 0; jt < 2; ++jt)
@@ -745,35 +759,36 @@ __global__ __launch_bounds__(64 * WAVES, (kWaves<DA, WAVES>)) void chunks_f32(Ro
         const int e = m - after - (16 * jt + 4 * g + r);
         c[jt][r] *= p.scale_b * sP[e > 0 ? e : 0];
       }
-    add_tokens32<DA>(S, sB, c, sP[m], g, lr);
+    add_tokens32<DA, KT>(S, sB, c, sP[m], m0, g, lr);
   }
   // (the compiler would keep every row's offset from the loads of the first state to here, in registers the loop needs)
   int ge = g;
   asm volatile("" : "+v"(ge));
   if (!live) return;
-  zero_tail(p, path, g, col);
+  if (half == 0) zero_tail(p, path, g, col);
   if (p.s1 && w.segment == pl.segments - 1) {
     float* s1 = p.s1 + path.b * p.s1_b + path.h * p.s1_h + col * p.s1_c;
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int d = 32 * (kt >> 1) + 8 * ge + 4 * (kt & 1) + r;
+        const int d = 32 * (m0 + (kt >> 1)) + 8 * ge + 4 * (kt & 1) + r;
         if (d < p.da) s1[d * p.s1_r] = S[kt][r];
       }
   }
 }
 
-template <int DA, int WAVES, bool BACK, bool FAST>
+template <int DA, int WAVES, int HALVES, bool BACK, bool FAST>
 __global__ __launch_bounds__(64 * WAVES, (kWaves<DA, WAVES>)) void sums_f32(Role<float> p, Plan<float> pl) {
-  constexpr int KT = DA / 16;
+  constexpr int KT = DA / 16 / HALVES, CT = WAVES / HALVES;
   constexpr int after = BACK ? 0 : 1;
   __shared__ __attribute__((aligned(16))) Pieces<DA> sB[2];
   const Work w = work_of(pl, pl.slots - 1);
   if (!w.live) return;
   const Path<float, BACK> path(p, w.group, w.segment * pl.part_tokens, pl.part_tokens);
   const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63, g = lane >> 4, lr = lane & 15;
-  const int col = (w.slice * WAVES + wave) * 16 + lr;
+  const int half = HALVES == 2 ? wave / CT : 0, m0 = half * (KT / 2);
+  const int col = (w.slice * CT + wave % CT) * 16 + lr;
   const int ccol = col < p.dc ? col : p.dc - 1;
   acc32 S[KT];
 #pragma unroll
@@ -803,7 +818,7 @@ __global__ __launch_bounds__(64 * WAVES, (kWaves<DA, WAVES>)) void sums_f32(Role
       for (int r = 0; r < 4; ++r) c[jt][r] *= wt[jt][r];
     __syncthreads();
     if (at + kChunk < path.total) fetch(at + kChunk);
-    add_tokens32<DA>(S, sB[turn], c, lam, g, lr);
+    add_tokens32<DA, KT>(S, sB[turn], c, lam, m0, g, lr);
   }
   if (col >= p.dc) return;
   float* s1 = pl.states + ((int64_t)w.group * pl.slots + w.segment + 1) * p.da * p.dc + col;
@@ -811,7 +826,7 @@ __global__ __launch_bounds__(64 * WAVES, (kWaves<DA, WAVES>)) void sums_f32(Role
   for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int d = 32 * (kt >> 1) + 8 * g + 4 * (kt & 1) + r;
+      const int d = 32 * (m0 + (kt >> 1)) + 8 * g + 4 * (kt & 1) + r;
       if (d < p.da) s1[(int64_t)d * p.dc] = S[kt][r];
     }
 }
@@ -881,8 +896,7 @@ template <typename T> struct Segments {
 
 // A wavefront takes 16 columns.
 template <typename T, Kernel<T> CHUNKS, Kernel<T> SUMS>
-static int run_chunks(const Role<T>& p, Segments<T>& seg, int waves) {
-  const int cols = 16 * waves;
+static int run_chunks(const Role<T>& p, Segments<T>& seg, int waves, int cols) {
   const dim3 block((unsigned)(64 * waves));
   Plan<T>& pl = seg.plan;
   pl.slices = (p.dc + cols - 1) / cols;
@@ -939,15 +953,19 @@ static int run_chunks(const Role<T>& p, Segments<T>& seg, int waves) {
 }
 
 template <int DA, bool BACK, bool FAST> static int run_sized(const Role<double>& p, Segments<double>& seg) {
-  return run_chunks<double, chunks_f64<DA, BACK, FAST>, sums_f64<DA, BACK, FAST>>(p, seg, kWaves64);
+  return run_chunks<double, chunks_f64<DA, BACK, FAST>, sums_f64<DA, BACK, FAST>>(p, seg, kWaves64, kCols64);
 }
 // Eight wavefronts where there are more than 64 columns (a and b are then split and staged once for all), unless the workgroups
 // of 128 columns leave CUs without work however short their segments.
 template <int DA, bool BACK, bool FAST> static int run_sized(const Role<float>& p, Segments<float>& seg) {
   const int64_t pairs = (p.tokens + 2 * kChunk - 1) / (2 * kChunk);
   const bool wide = p.dc > 64 && p.batch * p.heads * ((p.dc + 127) / 128) * (pairs > 1 ? pairs : 1) >= num_cus();
-  if (!wide) return run_chunks<float, chunks_f32<DA, 4, BACK, FAST>, sums_f32<DA, 4, BACK, FAST>>(p, seg, 4);
-  return run_chunks<float, chunks_f32<DA, 8, BACK, FAST>, sums_f32<DA, 8, BACK, FAST>>(p, seg, 8);
+  if (wide) return run_chunks<float, chunks_f32<DA, 8, 1, BACK, FAST>, sums_f32<DA, 8, 1, BACK, FAST>>(p, seg, 8, 128);
+  // 64 columns: from 128 rows on the rows are halved, and twice as many wavefronts share a workgroup's LDS. 8 x 1024 tokens, 8 heads
+  // of 192 x 64: 82 -> 67 us, of 128 x 64: 52 either way, 8 x 64 tokens, 16 heads of 128 x 128: 15 -> 13; with 64 rows 32 x 1024
+  // tokens, 16 heads of 64 x 64 lose: 126 -> 137.
+  if constexpr (DA % 64 == 0 && DA >= 128) return run_chunks<float, chunks_f32<DA, 8, 2, BACK, FAST>, sums_f32<DA, 8, 2, BACK, FAST>>(p, seg, 8, 64);
+  else return run_chunks<float, chunks_f32<DA, 4, 1, BACK, FAST>, sums_f32<DA, 4, 1, BACK, FAST>>(p, seg, 4, 64);
 }
 
 template <bool BACK, bool FAST, typename T> static int run_fast(const Role<T>& p, Segments<T>& seg) {
