@@ -7,11 +7,13 @@
 //     dx = rstd * (weight dz - avg(weight dz) - xhat * avg(weight dz xhat))
 //     dweight[c] = sum dz xhat      dbias[c] = sum dz                       (over batch and spatial)
 //
-// Two ways through it:
+// Three ways through it:
 //  - `team_*`: the elements of a group fit the registers of a team of lanes (8 .. 64, or a workgroup of 256). One launch,
 //    x is read once, mean and squared deviations are two folds over registers. A team keeps its group and walks over samples,
 //    with the group's parameters in registers; backwards it also adds up its lanes' shares of dweight and dbias on the way.
-//  - slabs: a workgroup takes a slab of rows of one sample and reads them whole, channels next to each other, whatever the
+//  - `image_*`: the elements of a group fit the registers of a workgroup of 1024 lanes, and a row of the group is no short run
+//    of memory. As the teams do it: one launch, every tensor moves once (backwards the activation is computed once too).
+//  - slabs, for the rest: a workgroup takes a slab of rows of one sample and reads them whole, channels next to each other, whatever the
 //    group's width; a lane owns V channels and keeps two sums for each. The slabs' sums per channel go to scratch memory
 //    and a small kernel folds them in a fixed order, per group (mean, rstd, or the two averages of the backward pass) and,
 //    backwards, per channel; then a second pass over the slabs writes the result. The sums of the forward pass are of
@@ -258,6 +260,196 @@ __global__ __launch_bounds__(256) void team_backward(Args<T> p, int lanes, int u
 #pragma unroll
       for (int e = 0; e < V; ++e) { at[2 * e] = dw[k][e]; at[2 * e + 1] = db[k][e]; }
     }
+  }
+}
+
+// ---- groups of an image in the registers of a workgroup ----
+// Bound by memory, and by the reductions between reading and writing that nothing overlaps: a CU has registers for one
+// workgroup of 1024 lanes (128 registers each; forwards fewer), for two of 512, four of 256. [128, 24, 24, 512] in 16 groups: 302 MB
+// forwards in 63 us, 453 MB backwards in 101 with 512 lanes, in 139 with 1024.
+constexpr int kImage = 1024;                   // lanes at most
+template <typename T> constexpr int kImageHeld = 192 / (int)sizeof(T);   // elements of a tensor that a lane holds at most
+
+// A sample's rows, channels of one group, as a buffer: the hardware adds a lane's 32-bit offset, and what lies behind the last
+// row reads as 0 and is not written.
+template <typename T> __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const T* p, int64_t spatial, int64_t step, int per) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)(((spatial - 1) * step + per) * (int64_t)sizeof(T)), 0x00020000);
+}
+template <typename V> __device__ __forceinline__ V get(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+  if constexpr (sizeof(V) == 4) return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b32(r, (int)off, 0, 0));
+  else if constexpr (sizeof(V) == 8) return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b64(r, (int)off, 0, 0));
+  else return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0));
+}
+template <typename V> __device__ __forceinline__ void put(__amdgpu_buffer_rsrc_t r, uint32_t off, V v) {
+  typedef unsigned u2 __attribute__((ext_vector_type(2)));
+  typedef unsigned u4 __attribute__((ext_vector_type(4)));
+  if constexpr (sizeof(V) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), r, (int)off, 0, 0);
+  else if constexpr (sizeof(V) == 8) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u2, v), r, (int)off, 0, 0);
+  else __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, v), r, (int)off, 0, 0);
+}
+
+// The sums of two values over the workgroup, the same in every lane.
+template <typename T, int WAVES> __device__ __forceinline__ void image_sums(T& a, T& b, T (&lds)[2][WAVES]) {
+  for (int d = 32; d >= 1; d >>= 1) { a += __shfl_xor(a, d, 64); b += __shfl_xor(b, d, 64); }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) { lds[0][threadIdx.x >> 6] = a; lds[1][threadIdx.x >> 6] = b; }
+  __syncthreads();
+  T s[2][4] = {};
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) { s[0][i & 3] += lds[0][i]; s[1][i & 3] += lds[1][i]; }
+  a = (s[0][0] + s[0][1]) + (s[0][2] + s[0][3]);
+  b = (s[1][0] + s[1][1]) + (s[1][2] + s[1][3]);
+}
+
+// A workgroup's place: workgroups that run together on a die take neighbouring groups, which share cache lines. A lane stays
+// with V channels (c) and takes rows row, row + rows_at_once, ...
+template <typename T, int V> struct Image {
+  int64_t n;
+  int g, row;
+  uint32_t c;
+  bool there, live;
+  __device__ __forceinline__ Image(const Args<T>& p) {
+    const uint32_t all = (uint32_t)(p.batch * p.groups), each = (all + 7) / 8;
+    const uint32_t item = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
+    there = (blockIdx.x >> 3) < each && item < all;
+    uint32_t gi;
+    n = p.groups_div.divmod(item, gi);
+    g = (int)gi;
+    row = (int)p.units_div.divmod(threadIdx.x, c);
+    c *= V;
+    live = row < p.rows_at_once;
+  }
+  // a lane without rows reads and writes behind the last one
+  __device__ __forceinline__ uint32_t first(int64_t step) const { return live ? (uint32_t)((row * step + c) * (int64_t)sizeof(T)) : 0x7fffffffu & ~15u; }
+};
+
+template <typename T, int LANES, int V, int U, int ACT>
+__global__ __launch_bounds__(LANES, 4) void image_forward(Args<T> p) {
+  typedef typename Vec<T, V>::type vec_t;
+  __shared__ T lds[2][LANES / 64];
+  const Image<T, V> t(p);
+  if (!t.there) return;
+  const int c0 = t.g * p.per, spatial = (int)p.spatial;
+  vec_t v[U];
+  {
+    const __amdgpu_buffer_rsrc_t x = rows_of(p.x + t.n * p.x_n + c0, p.spatial, p.x_s, p.per);
+    const uint32_t first = t.first(p.x_s), step = (uint32_t)(p.rows_at_once * p.x_s * (int64_t)sizeof(T));
+#pragma unroll
+    for (int k = 0; k < U; ++k) v[k] = get<vec_t>(x, first + (uint32_t)k * step);
+  }
+  T w[V], b[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    w[e] = p.weight ? p.weight[c0 + t.c + e] : (T)1;
+    b[e] = p.bias ? p.bias[c0 + t.c + e] : (T)0;
+  }
+  const T count = (T)((T)p.spatial * (T)p.per);
+  T part[4] = {}, none = (T)0;                 // four short sums in a lane
+#pragma unroll
+  for (int k = 0; k < U; ++k)
+#pragma unroll
+    for (int e = 0; e < V; ++e) part[(k * V + e) & 3] += v[k][e];
+  T sum = (part[0] + part[1]) + (part[2] + part[3]);
+  image_sums(sum, none, lds);
+  const T mean = sum / count;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) part[i] = (T)0;
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const bool is = t.live && t.row + k * p.rows_at_once < spatial;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      v[k][e] -= mean;
+      part[(k * V + e) & 3] += is ? v[k][e] * v[k][e] : (T)0;
+    }
+  }
+  T sq = (part[0] + part[1]) + (part[2] + part[3]);
+  image_sums(sq, none, lds);
+  const T rstd = dev_rsqrt(sq / count + p.eps);
+  if (threadIdx.x == 0 && p.mean) { p.mean[t.n * p.groups + t.g] = mean; p.rstd[t.n * p.groups + t.g] = rstd; }
+  const __amdgpu_buffer_rsrc_t y = rows_of(p.y + t.n * p.y_n + c0, p.spatial, p.y_s, p.per);
+  const uint32_t first = t.first(p.y_s), step = (uint32_t)(p.rows_at_once * p.y_s * (int64_t)sizeof(T));
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    vec_t out;
+#pragma unroll
+    for (int e = 0; e < V; ++e) out[e] = activate<T, ACT>(v[k][e] * rstd * w[e] + b[e]);
+    put(y, first + (uint32_t)k * step, out);
+  }
+}
+
+template <typename T, int LANES, int V, int U, int ACT>
+__global__ __launch_bounds__(LANES, 4) void image_backward(Args<T> p) {
+  typedef typename Vec<T, V>::type vec_t;
+  __shared__ T lds[2][LANES / 64];
+  __shared__ T each[2][LANES * V];            // [row][channel]: the lanes' sums
+  const Image<T, V> t(p);
+  if (!t.there) return;
+  const int c0 = t.g * p.per, spatial = (int)p.spatial;
+  vec_t h[U], d[U];                            // xhat and dz
+  {
+    const __amdgpu_buffer_rsrc_t x = rows_of(p.x + t.n * p.x_n + c0, p.spatial, p.x_s, p.per);
+    const __amdgpu_buffer_rsrc_t dy = rows_of(p.dy + t.n * p.dy_n + c0, p.spatial, p.dy_s, p.per);
+    const uint32_t x0 = t.first(p.x_s), xs = (uint32_t)(p.rows_at_once * p.x_s * (int64_t)sizeof(T));
+    const uint32_t d0 = t.first(p.dy_s), ds = (uint32_t)(p.rows_at_once * p.dy_s * (int64_t)sizeof(T));
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      h[k] = get<vec_t>(x, x0 + (uint32_t)k * xs);
+      d[k] = get<vec_t>(dy, d0 + (uint32_t)k * ds);
+    }
+  }
+  const T mean = p.mean[t.n * p.groups + t.g], rstd = p.rstd[t.n * p.groups + t.g];
+  constexpr int H = V == 1 ? 2 : 1;            // two short sums in place of one of 48 rows
+  T w[V], b[V], dw[H * V], db[H * V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    w[e] = p.weight ? p.weight[c0 + t.c + e] : (T)1;
+    b[e] = p.bias ? p.bias[c0 + t.c + e] : (T)0;
+  }
+#pragma unroll
+  for (int e = 0; e < H * V; ++e) dw[e] = db[e] = (T)0;
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const bool is = t.live && t.row + k * p.rows_at_once < spatial;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      h[k][e] = (h[k][e] - mean) * rstd;
+      d[k][e] = is ? through<T, ACT>(d[k][e], h[k][e] * w[e] + b[e]) : (T)0;
+      dw[e + k % H] += is ? d[k][e] * h[k][e] : (T)0;
+      db[e + k % H] += d[k][e];
+    }
+  }
+  if constexpr (H == 2) { dw[0] += dw[1]; db[0] += db[1]; }
+  T s1 = (T)0, s2 = (T)0;
+#pragma unroll
+  for (int e = 0; e < V; ++e) { s1 += db[e] * w[e]; s2 += dw[e] * w[e]; }
+  if (p.share && t.live)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      each[0][t.row * p.per + t.c + e] = dw[e];
+      each[1][t.row * p.per + t.c + e] = db[e];
+    }
+  image_sums(s1, s2, lds);                     // (its barriers stand between `each` being written and read)
+  const T count = (T)((T)p.spatial * (T)p.per);
+  s1 /= count;
+  s2 /= count;
+  const __amdgpu_buffer_rsrc_t dx = rows_of(p.y + t.n * p.y_n + c0, p.spatial, p.y_s, p.per);
+  const uint32_t first = t.first(p.y_s), step = (uint32_t)(p.rows_at_once * p.y_s * (int64_t)sizeof(T));
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    vec_t out;
+#pragma unroll
+    for (int e = 0; e < V; ++e) out[e] = rstd * (d[k][e] * w[e] - s1 - h[k][e] * s2);
+    put(dx, first + (uint32_t)k * step, out);
+  }
+  if (!p.share) return;
+  // a wavefront per sum
+  for (int i = (int)threadIdx.x >> 6; i < 2 * p.per; i += LANES / 64) {
+    const int c = i >> 1, lane = (int)threadIdx.x & 63;
+    T sum = (T)0;
+    for (int r = lane; r < p.rows_at_once; r += 64) sum += each[i & 1][r * p.per + c];
+    for (int dd = 32; dd >= 1; dd >>= 1) sum += __shfl_xor(sum, dd, 64);
+    if (lane == 0) p.share[(t.n * p.channels + c0 + c) * 2 + (i & 1)] = sum;
   }
 }
 
@@ -630,12 +822,73 @@ static int try_teams(Args<T>& p, bool aligned, bool& taken) {
   return V > 1 ? team_pass<T, W, ACT, BWD>(p, lanes, units) : team_pass<T, 1, ACT, BWD>(p, lanes, units);
 }
 
+// The image's way, where a workgroup's registers hold a group.
+template <typename T, int LANES, int V, int U, int ACT, bool BWD> static void launch_image(const Args<T>& p) {
+  const dim3 grid((unsigned)((p.batch * p.groups + 7) / 8 * 8)), block(LANES);
+  if constexpr (BWD) hipLaunchKernelGGL((image_backward<T, LANES, V, U, ACT>), grid, block, 0, stream(), p);
+  else hipLaunchKernelGGL((image_forward<T, LANES, V, U, ACT>), grid, block, 0, stream(), p);
+}
+
+template <typename T, int V, int ACT, bool BWD>
+static int image_pass(Args<T> p, int lanes) {
+  constexpr int U = kImageHeld<T> / V;
+  Scratch share;
+  if (BWD && (p.dweight || p.dbias)) {
+    AM_TRY(share.take((size_t)p.batch * p.channels * 2 * sizeof(T)));
+    p.share = (T*)share.p;
+  }
+  if (lanes == 256 && p.spatial <= (int64_t)p.rows_at_once * (U / 2)) launch_image<T, 256, V, U / 2, ACT, BWD>(p);
+  else if (lanes == 256) launch_image<T, 256, V, U, ACT, BWD>(p);
+  else if (lanes == 512) launch_image<T, 512, V, U, ACT, BWD>(p);
+  else launch_image<T, 1024, V, U, ACT, BWD>(p);
+  AM_TRY(check_launch("group norm of images"));
+  if (p.share) {
+    hipLaunchKernelGGL((channel_fold<T, T>), dim3((unsigned)((p.channels + 7) / 8)), dim3(256), 0, stream(), p, (const T*)p.share, p.batch, 1, false);
+    AM_TRY(check_launch("channel_fold"));
+  }
+  return AM_OK;
+}
+
+template <typename T, int ACT, bool BWD>
+static int try_images(Args<T>& p, bool& taken) {
+  // A row of a group is a short run of memory, and a cache line that several groups share is fetched for each of them unless the
+  // die's L2 still has it. From 48 bytes on that is no loss: [16, 56, 56, 384] in 32 groups 49 + 78 us (forwards, backwards)
+  // against 49 + 88 in slabs, with 64 bytes ([32, 48, 48, 256] in 16) 43 + 63 against 47 + 81, with 256 ([16, 24, 24, 1024] in
+  // 16) 19 + 30 against 36 + 48; with 20 bytes ([16, 64, 64, 320] in 64) 75 + 115 against 52 + 88.
+  taken = false;
+  if (p.per * (int)sizeof(T) < 48 || p.batch * p.groups >= ((int64_t)1 << 31) - 8) return AM_OK;
+  int V = 16 / (int)sizeof(T);
+  // rows one behind the other, and all that the lanes may count up to within 2^31 bytes
+  constexpr int64_t most = ((int64_t)1 << 31) / ((kImageHeld<T> + 1) * kImage * (int)sizeof(T));
+  auto holds = [&](const T* base, int64_t sn, int64_t ss) {
+    while (V > 1 && (p.per % V || (uintptr_t)base % (V * sizeof(T)) || sn % V || ss % V)) V /= 2;
+    return (ss >= p.per || p.spatial == 1) && ss >= 0 && ss < most;
+  };
+  if (!holds(p.x, p.x_n, p.x_s) || !holds(p.y, p.y_n, p.y_s)) return AM_OK;
+  if (BWD && !holds(p.dy, p.dy_n, p.dy_s)) return AM_OK;
+  // The fewest lanes that hold a group, so that several workgroups share a CU and one reads while another writes.
+  const int64_t upr = p.per / V;
+  int lanes = 256;
+  while (lanes <= kImage && (upr > lanes || (p.spatial + lanes / upr - 1) / (lanes / upr) * V > kImageHeld<T>)) lanes *= 2;
+  if (lanes > kImage) return AM_OK;
+  taken = true;
+  p.units_div = FastDiv((uint32_t)upr);
+  p.rows_at_once = (int)(lanes / upr);
+  if constexpr (sizeof(T) == 4) {
+    if (V == 4) return image_pass<T, 4, ACT, BWD>(p, lanes);
+  }
+  if (V == 2) return image_pass<T, 2, ACT, BWD>(p, lanes);
+  return image_pass<T, 1, ACT, BWD>(p, lanes);
+}
+
 template <typename T, int ACT>
 static int forward(Args<T> p) {
   constexpr int W = 16 / (int)sizeof(T);
   const bool aligned = fits<T>(p.x, p.x_n, p.x_s, p.batch, p.spatial) && fits<T>(p.y, p.y_n, p.y_s, p.batch, p.spatial);
   bool taken;
   AM_TRY((try_teams<T, ACT, false>(p, aligned, taken)));
+  if (taken) return AM_OK;
+  AM_TRY((try_images<T, ACT, false>(p, taken)));
   if (taken) return AM_OK;
   const int V = aligned && p.channels % W == 0 ? W : 1;
   const Args<T> all = p;
@@ -686,6 +939,8 @@ static int backward(Args<T> p) {
                        fits<T>(p.dy, p.dy_n, p.dy_s, p.batch, p.spatial);
   bool taken;
   AM_TRY((try_teams<T, ACT, true>(p, aligned, taken)));
+  if (taken) return AM_OK;
+  AM_TRY((try_images<T, ACT, true>(p, taken)));
   if (taken) return AM_OK;
   const int V = aligned && p.channels % W == 0 ? W : 1;
   const Args<T> all = p;

@@ -377,6 +377,12 @@ NORMS = [((1, 1), 1), ((3, 8), 2), ((5, 2048), 16), ((2, 7, 5, 30), 3), ((2, 16,
          ((700, 24), 4), ((1, 9000), 1), ((2, 3, 5000), 1), ((3, 40, 41, 320), 32), ((6, 1, 1, 64), 64), ((1, 300, 1030), 2), ((2, 70, 70, 3), 3)]
 
 
+# groups that a workgroup's registers hold: vectors of four, two and one, a lane's rows few and many (48 in the last but two), lanes
+# and dies left over, just too large
+IMAGES = [((2, 40, 40, 96), 6), ((3, 33, 31, 90), 6), ((1, 47, 44, 54), 2), ((9, 26, 25, 112), 4), ((1, 20, 20, 1024), 8), ((2, 59, 58, 13), 1),
+          ((1, 64, 63, 12), 1), ((1, 65, 65, 24), 2)]
+
+
 def norm_inputs(shape, dt, seed, mean=0.5):
     rng = np.random.default_rng(seed)
     mk = lambda *s: rng.normal(size=s).astype(DTYPES[dt])
@@ -407,7 +413,7 @@ def norm_bounds(x, w, b, dy, groups, eps, dt, chain=64):
 
 @pytest.mark.parametrize("activation", ["none", "relu", "silu"])
 @pytest.mark.parametrize("dt", ["f32", "f64"])
-@pytest.mark.parametrize("shape,groups", NORMS, ids=str)
+@pytest.mark.parametrize("shape,groups", NORMS + IMAGES, ids=str)
 def test_group_norm_and_its_gradients(hip, shape, groups, dt, activation):
     x, w, b, dy = norm_inputs(shape, dt, seed_of("norm", shape, groups, dt, activation))
     eps = 1e-5
@@ -463,7 +469,7 @@ def test_group_norm_activations_far_out(hip, shape, groups, dt):
 
 
 @pytest.mark.parametrize("dt", ["f32", "f64"])
-@pytest.mark.parametrize("shape,groups", [((3, 6, 5, 24), 4), ((2, 50, 50, 16), 2)], ids=str)
+@pytest.mark.parametrize("shape,groups", [((3, 6, 5, 24), 4), ((2, 50, 50, 16), 2), ((2, 30, 40, 36), 2)], ids=str)
 def test_group_norm_of_views(hip, shape, groups, dt):
     """Images with the channels first (copied), a slice of the channels, rows with a gap, one element off a boundary."""
     x, w, b, dy = norm_inputs(shape, dt, seed_of("norm views", shape, dt))
