@@ -11,8 +11,7 @@
 //  - `team_*`: the elements of a group fit the registers of a team of lanes (8 .. 64, or a workgroup of 256). One launch,
 //    x is read once, mean and squared deviations are two folds over registers. A team keeps its group and walks over samples,
 //    with the group's parameters in registers; backwards it also adds up its lanes' shares of dweight and dbias on the way.
-//  - `image_*`: the elements of a group fit the registers of a workgroup of 1024 lanes, and a row of the group is no short run
-//    of memory. As the teams do it: one launch, every tensor moves once (backwards the activation is computed once too).
+//  - `image_*`: many rows, whose group fits the registers of a workgroup of up to 1024 lanes, in runs of memory that are not too short. As the teams do it: one launch, every tensor moves once (backwards the activation is computed once too).
 //  - slabs, for the rest: a workgroup takes a slab of rows of one sample and reads them whole, channels next to each other, whatever the
 //    group's width; a lane owns V channels and keeps two sums for each. The slabs' sums per channel go to scratch memory
 //    and a small kernel folds them in a fixed order, per group (mean, rstd, or the two averages of the backward pass) and,
@@ -851,12 +850,20 @@ static int image_pass(Args<T> p, int lanes) {
 
 template <typename T, int ACT, bool BWD>
 static int try_images(Args<T>& p, bool& taken) {
-  // A row of a group is a short run of memory, and a cache line that several groups share is fetched for each of them unless the
-  // die's L2 still has it. From 48 bytes on that is no loss: [16, 56, 56, 384] in 32 groups 49 + 78 us (forwards, backwards)
-  // against 49 + 88 in slabs, with 64 bytes ([32, 48, 48, 256] in 16) 43 + 63 against 47 + 81, with 256 ([16, 24, 24, 1024] in
-  // 16) 19 + 30 against 36 + 48; with 20 bytes ([16, 64, 64, 320] in 64) 75 + 115 against 52 + 88.
+  // us forwards + backwards, images against what else takes the shape.
+  //  - Few rows: the teams, whose lanes hold what they need and no more ([64, 8, 8, 1024] in 32 groups 13 + 30 against 10 + 17 in
+  //    teams). From 128 rows on the images ([16, 45, 45, 128] in 32: 15 + 23 against 34 + 64), forwards where there are 2048
+  //    elements ([64, 16, 16, 128] in 32: 12 + 18 against 9 + 103: backwards the teams keep shares of dweight for every row).
+  //  - A row of a group is a short run of memory, and a cache line that several groups share is fetched for each of them unless
+  //    the die's L2 still has it. From 48 bytes on that is no loss: [16, 56, 56, 384] in 32 groups 49 + 78 against 49 + 88 in
+  //    slabs, with 64 bytes ([32, 48, 48, 256] in 16) 43 + 63 against 47 + 81, with 256 ([16, 24, 24, 1024] in 16) 19 + 30 against
+  //    36 + 48. From 16 bytes on it is none while the device's last cache holds the tensors: 40 bytes of 42 MB 25 + 41 against
+  //    33 + 48, of 63 MB 51 + 79 against 44 + 73; 16 bytes of 17 MB 16 + 25 against 19 + 29; 12 bytes of 14 MB 24 + 36 against 20 + 29.
   taken = false;
-  if (p.per * (int)sizeof(T) < 48 || p.batch * p.groups >= ((int64_t)1 << 31) - 8) return AM_OK;
+  const int run = p.per * (int)sizeof(T);
+  if (p.spatial < 128 || (!BWD && p.spatial * p.per < 2048) || run < 16) return AM_OK;
+  if (run < 48 && (double)p.batch * (double)p.spatial * p.channels * sizeof(T) > 48e6) return AM_OK;
+  if (p.batch * p.groups >= ((int64_t)1 << 31) - 8) return AM_OK;
   int V = 16 / (int)sizeof(T);
   // rows one behind the other, and all that the lanes may count up to within 2^31 bytes
   constexpr int64_t most = ((int64_t)1 << 31) / ((kImageHeld<T> + 1) * kImage * (int)sizeof(T));
@@ -886,9 +893,9 @@ static int forward(Args<T> p) {
   constexpr int W = 16 / (int)sizeof(T);
   const bool aligned = fits<T>(p.x, p.x_n, p.x_s, p.batch, p.spatial) && fits<T>(p.y, p.y_n, p.y_s, p.batch, p.spatial);
   bool taken;
-  AM_TRY((try_teams<T, ACT, false>(p, aligned, taken)));
-  if (taken) return AM_OK;
   AM_TRY((try_images<T, ACT, false>(p, taken)));
+  if (taken) return AM_OK;
+  AM_TRY((try_teams<T, ACT, false>(p, aligned, taken)));
   if (taken) return AM_OK;
   const int V = aligned && p.channels % W == 0 ? W : 1;
   const Args<T> all = p;
@@ -938,9 +945,9 @@ static int backward(Args<T> p) {
   const bool aligned = fits<T>(p.x, p.x_n, p.x_s, p.batch, p.spatial) && fits<T>(p.y, p.y_n, p.y_s, p.batch, p.spatial) &&
                        fits<T>(p.dy, p.dy_n, p.dy_s, p.batch, p.spatial);
   bool taken;
-  AM_TRY((try_teams<T, ACT, true>(p, aligned, taken)));
-  if (taken) return AM_OK;
   AM_TRY((try_images<T, ACT, true>(p, taken)));
+  if (taken) return AM_OK;
+  AM_TRY((try_teams<T, ACT, true>(p, aligned, taken)));
   if (taken) return AM_OK;
   const int V = aligned && p.channels % W == 0 ? W : 1;
   const Args<T> all = p;
