@@ -753,14 +753,16 @@ static int check_args(const char* fn, int64_t batch, int64_t spatial, int64_t ch
   return AM_OK;
 }
 
-template <typename T> static bool past_caches(const Args<T>& p) {
-  return (double)p.batch * (double)p.spatial * p.channels * sizeof(T) > nt_threshold_bytes();
+// Whether x is larger than the caches keep and not read again: who asks for the statistics has a backward pass to come
+// ([16, 64, 64, 320] forwards and backwards 158 us with x read past the caches, 141 without).
+template <bool BWD, typename T> static bool last_reading(const Args<T>& p) {
+  return (BWD || !p.mean) && (double)p.batch * (double)p.spatial * p.channels * sizeof(T) > nt_threshold_bytes();
 }
 
 template <typename T, int V, int U, bool WIDE, int ACT, bool BWD>
 static void launch_team(const Args<T>& p, int lanes, int units, int64_t slots, int64_t wgs) {
   const dim3 grid((unsigned)wgs), block(256);
-  const bool nt = V > 1 && past_caches(p);
+  const bool nt = V > 1 && last_reading<BWD>(p);
   if constexpr (BWD) {
     if (nt) hipLaunchKernelGGL((team_backward<T, V, U, WIDE, ACT, (V > 1)>), grid, block, 0, stream(), p, lanes, units, slots);
     else hipLaunchKernelGGL((team_backward<T, V, U, WIDE, ACT, false>), grid, block, 0, stream(), p, lanes, units, slots);
@@ -926,7 +928,7 @@ static int forward(Args<T> p) {
     AM_TRY(check_launch("slab_sums"));
     hipLaunchKernelGGL((group_fold<T, false>), dim3((unsigned)(p.nc * p.groups)), dim3(256), 0, stream(), p);
     AM_TRY(check_launch("group_fold"));
-    if (V > 1 && past_caches(all)) AM_GN_LAUNCH(slab_apply, V, wgs, false, ACT, true);
+    if (V > 1 && last_reading<false>(all)) AM_GN_LAUNCH(slab_apply, V, wgs, false, ACT, true);
     else AM_GN_LAUNCH(slab_apply, V, wgs, false, ACT, false);
     AM_TRY(check_launch("slab_apply"));
   }

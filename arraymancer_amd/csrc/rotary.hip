@@ -8,9 +8,9 @@
 //
 // The angle depends on the token and the pair alone, so a lane keeps one 16-byte vector of pairs of one token, makes its
 // sines and cosines once and walks over the heads with them. Positions of long texts reach 10^5 and more, where a float
-// angle is off by 10^-2: the number of turns p * frequency / (2 pi) is formed in double (for double results as an
-// unevaluated sum of two doubles), its whole part dropped exactly, and only the rest, at most half a turn, is rounded to
-// the result's type for sincospi.
+// angle is off by 10^-2: the angle is formed in double and divided by 2 pi (for double results into an unevaluated sum of two
+// doubles), the whole part of these turns is dropped exactly, and only the rest, at most half a turn, is rounded to the
+// result's type for sincospi.
 #include "common.h"
 #include "fastdiv.h"
 
@@ -38,10 +38,10 @@ __device__ __forceinline__ void sincos_at(double p, double f, float& s, float& c
   sincos_turns(p * (f * 0.15915494309189535), s, c);
 }
 __device__ __forceinline__ void sincos_at(double p, double f, double& s, double& c) {
-  // 1 / (2 pi) as the sum of two doubles; f / (2 pi) = hi + lo, p * hi = whole + rest exactly through fma
+  // the angle p * f as a double, as everyone else forms it; its turns with 1 / (2 pi) as the sum of two doubles, the product
+  // with the first one exactly through fma
   const double inv_hi = 0.15915494309189535, inv_lo = -9.839338337591243e-18;
-  const double hi = f * inv_hi, lo = fma(f, inv_hi, -hi) + f * inv_lo;
-  const double t = p * hi, rest = fma(p, hi, -t) + p * lo;
+  const double a = p * f, t = a * inv_hi, rest = fma(a, inv_hi, -t) + a * inv_lo;
   sincospi(2.0 * ((t - rint(t)) + rest), &s, &c);
 }
 
