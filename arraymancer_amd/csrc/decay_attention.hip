@@ -831,6 +831,12 @@ __global__ __launch_bounds__(64 * WAVES, (kWaves<DA, WAVES>)) void sums_f32(Role
     }
 }
 
+// Tokens in front of a slot, of a sequence of n.
+template <typename T> __device__ __forceinline__ int64_t tokens_before(const Plan<T>& pl, int64_t n, int slot) {
+  const int64_t t = slot * pl.part_tokens;
+  return t < n ? t : n;
+}
+
 // From the parts' shares to the states in front of the segments (the slots at multiples of `parts`): a lane takes V neighbouring
 // elements of a head's state, BATCH slots on their way at a time (no load may pass the stores of the batch before).
 template <typename T, int V, int BATCH>
@@ -842,9 +848,7 @@ __device__ __forceinline__ void carry(T* at, int64_t per, int& k, T (&s)[V], T l
 #pragma unroll
   for (int u = 0; u < BATCH; ++u) {
     if (k + u >= pl.slots) break;
-    int64_t len = n - (k + u - 1) * pl.part_tokens;
-    len = len < 0 ? 0 : (len < pl.part_tokens ? len : pl.part_tokens);
-    const T f = power(ld, len);
+    const T f = power(ld, tokens_before(pl, n, k + u) - tokens_before(pl, n, k + u - 1));
     vec_t to;
 #pragma unroll
     for (int e = 0; e < V; ++e) to[e] = s[e] = s[e] * f + v[u][e];
@@ -873,9 +877,64 @@ __global__ __launch_bounds__(256) void segment_states(Role<T> p, Plan<T> pl) {
     at[e] = s[e];
   }
   int k = 1;
-  if constexpr (V == 1)
-    while (k + 24 < pl.slots) carry<T, V, 32>(at, per, k, s, ld, n, pl);
   while (k < pl.slots) carry<T, V, 8>(at, per, k, s, ld, n, pl);
+}
+
+// The same for few states, where the length of the chain counts: a lane takes one element, and the four wavefronts of a
+// workgroup a quarter of up to 4 MOST slots each. They add up theirs, exchange the sums and add what lies in front.
+template <typename T, int MOST>
+__device__ __forceinline__ void carry_quarters(T* at, int64_t per, int from, int count, T& s, T ld, int64_t n, const Plan<T>& pl, bool live, T (&sums)[4][64]) {
+  const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63;
+  const int each = (count + 3) / 4;
+  auto first = [&](int w) { const int k = w * each; return from + (k < count ? k : count); };
+  auto decay = [&](int lo, int hi) { return power(ld, tokens_before(pl, n, hi) - tokens_before(pl, n, lo)); };   // from slot to slot
+  const int lo = first(wave), hi = first(wave + 1);
+  T v[MOST], t = (T)0;
+#pragma unroll
+  for (int u = 0; u < MOST; ++u) v[u] = at[(int64_t)(lo + u < pl.slots ? lo + u : pl.slots - 1) * per];
+#pragma unroll
+  for (int u = 0; u < MOST; ++u) {
+    if (lo + u >= hi) break;
+    v[u] = t = t * decay(lo + u - 1, lo + u) + v[u];
+  }
+  __syncthreads();
+  sums[wave][lane] = t;
+  __syncthreads();
+  T in = s;                                                 // the state in front of this quarter
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (w == wave) in = s;
+    if (first(w) < first(w + 1)) s = s * decay(first(w) - 1, first(w + 1) - 1) + sums[w][lane];
+  }
+#pragma unroll
+  for (int u = 0; u < MOST; ++u) {
+    if (lo + u >= hi) break;
+    if ((lo + u) % pl.parts == 0 && live) at[(int64_t)(lo + u) * per] = v[u] + in * decay(lo - 1, lo + u);
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void segment_states_few(Role<T> p, Plan<T> pl) {
+  __shared__ T sums[4][64];
+  const int per = p.da * p.dc;
+  const int blocks = (per + 63) / 64;
+  const int group = (int)(blockIdx.x / (unsigned)blocks);
+  int i = (int)(blockIdx.x - (unsigned)group * (unsigned)blocks) * 64 + ((int)threadIdx.x & 63);
+  const bool live = i < per;
+  if (!live) i = 0;
+  const int64_t b = group / (int)p.heads;
+  const int h = (int)(group - b * p.heads);
+  const int64_t n = length_of(p, b);
+  const T ld = p.log_decay[h];
+  const int r = i / p.dc, c = i - r * p.dc;
+  T* at = pl.states + (int64_t)group * pl.slots * per + i;
+  T s = p.s0 ? p.s0[b * p.s0_b + h * p.s0_h + r * p.s0_r + c * p.s0_c] : (T)0;
+  if (live && threadIdx.x < 64) at[0] = s;
+  for (int k = 1; k < pl.slots; k += 128) {
+    const int count = pl.slots - k < 128 ? pl.slots - k : 128;
+    if (count <= 16) carry_quarters<T, 4>(at, per, k, count, s, ld, n, pl, live, sums);
+    else carry_quarters<T, 32>(at, per, k, count, s, ld, n, pl, live, sums);
+  }
 }
 
 static int workgroups_per_cu(const void* kernel, int threads) {
@@ -935,11 +994,14 @@ static int run_chunks(const Role<T>& p, Segments<T>& seg, int waves, int cols) {
       const int64_t ids = ((int64_t)pl.groups * (pl.slots - 1) + 7) / 8 * 8 * pl.slices;
       hipLaunchKernelGGL(SUMS, dim3((unsigned)ids), block, 0, stream(), p, pl);
       AM_TRY(check_launch("decay attention: sums"));
-      // Vectors of 16 bytes where they still make a wavefront a CU: 64 states of 128 x 128 and 8 slots, 62 MB, 21.5 us in single
-      // elements, 11.9 in vectors; 16 such states and 32 slots, the whole call 129 and 124.6 us.
+      // Vectors of 16 bytes and one walk over the slots where that still makes a wavefront a CU: 64 states of 128 x 128 and 8
+      // slots, 62 MB, 21.5 us in single elements, 11.9 in vectors; in quarters the whole call takes 225 us in place of 216. Below,
+      // quarters: 8 states of 64 x 64 and 86 slots, the whole call 67 us in one walk, 62 in quarters.
       constexpr int V = 16 / (int)sizeof(T);
       const int per = p.da * p.dc;
-      if (p.dc % V == 0 && (int64_t)pl.groups * per / V >= (int64_t)64 * num_cus())
+      if ((int64_t)pl.groups * per / V < (int64_t)64 * num_cus())
+        hipLaunchKernelGGL((segment_states_few<T>), dim3((unsigned)(pl.groups * ((per + 63) / 64))), dim3(256), 0, stream(), p, pl);
+      else if (p.dc % V == 0)
         hipLaunchKernelGGL((segment_states<T, V>), dim3((unsigned)(pl.groups * ((per + 256 * V - 1) / (256 * V)))), dim3(256), 0, stream(), p, pl);
       else
         hipLaunchKernelGGL((segment_states<T, 1>), dim3((unsigned)(pl.groups * ((per + 255) / 256))), dim3(256), 0, stream(), p, pl);

@@ -197,7 +197,7 @@ def test_decay_attention_of_a_padded_batch(hip, size, dt):
 
 
 @pytest.mark.parametrize("dt", ["f32", "f64"])
-@pytest.mark.parametrize("size", [(2, 321, 4, 2, 64, 128), (2, 260, 8, 8, 64, 126), (1, 1411, 2, 1, 24, 40)], ids=str)
+@pytest.mark.parametrize("size", [(2, 321, 4, 2, 64, 128), (2, 260, 8, 8, 64, 126), (1, 1411, 2, 1, 24, 40), (1, 9001, 1, 1, 8, 12)], ids=str)
 def test_decay_attention_in_segments(hip, size, dt):
     """Long enough to be cut into segments: states between them in vectors, in single elements, over many slots; a sequence that
     ends within the first segments and one without tokens."""
