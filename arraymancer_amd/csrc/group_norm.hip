@@ -660,6 +660,25 @@ __global__ __launch_bounds__(256) void channel_fold(Args<T> p, const P* part, in
   if (p.dbias) p.dbias[c] = (T)(add ? (double)p.dbias[c] + b : b);
 }
 
+// Sums over `each` samples at a time of [samples, columns] (a lane stays with a column), in a fixed order.
+template <typename P>
+__global__ __launch_bounds__(256) void sample_sums(const P* part, double* out, int64_t samples, int64_t each, int columns) {
+  const int c = (int)blockIdx.x * 256 + (int)threadIdx.x;
+  if (c >= columns) return;
+  const int64_t lo = (int64_t)blockIdx.y * each, hi = lo + each < samples ? lo + each : samples;
+  double sum = 0.0;
+  int64_t i = lo;
+  for (; i + 7 < hi; i += 8) {
+    P v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = part[(i + u) * columns + c];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) sum += (double)v[u];
+  }
+  for (; i < hi; ++i) sum += (double)part[i * columns + c];
+  out[(int64_t)blockIdx.y * columns + c] = sum;
+}
+
 // Second pass over the slabs: y from mean and rstd, or (BWD) dx from the averages too.
 template <typename T, int V, bool BWD, int ACT, bool NT>
 __global__ __launch_bounds__(256) void slab_apply(Args<T> p) {
@@ -728,6 +747,25 @@ template <typename T> static void set_slabs(Args<T>& p, int V, int64_t rows, int
   p.slabs = (int)((rows + p.rows_per_slab - 1) / p.rows_per_slab);
   p.tiles_div = FastDiv((uint32_t)p.tiles);
   p.slabs_div = FastDiv((uint32_t)p.slabs);
+}
+
+// dweight and dbias from every sample's sums per channel, [samples, channels, 2]. Many samples are added up in 128 runs first:
+// channel_fold has a workgroup for 8 channels, and no more of them ([8192, 16, 8, 16] in 1 group, backwards 79 -> 63 us).
+template <typename T, typename P>
+static int fold_samples(const Args<T>& p, const P* part, int64_t samples, bool add) {
+  const dim3 grid((unsigned)((p.channels + 7) / 8)), block(256);
+  if (samples <= 512) {
+    hipLaunchKernelGGL((channel_fold<T, P>), grid, block, 0, stream(), p, part, samples, 1, add);
+    return check_launch("channel_fold");
+  }
+  const int64_t each = (samples + 127) / 128, runs = (samples + each - 1) / each;
+  const int columns = 2 * p.channels;
+  Scratch sums;
+  AM_TRY(sums.take((size_t)runs * columns * sizeof(double)));
+  hipLaunchKernelGGL((sample_sums<P>), dim3((unsigned)((columns + 255) / 256), (unsigned)runs), block, 0, stream(), part, (double*)sums.p, samples, each, columns);
+  AM_TRY(check_launch("sample_sums"));
+  hipLaunchKernelGGL((channel_fold<T, double>), grid, block, 0, stream(), p, (const double*)sums.p, runs, 1, add);
+  return check_launch("channel_fold");
 }
 
 #define AM_GN_LAUNCH(KERNEL, V_, GRID, ...)                                                                         \
@@ -843,28 +881,28 @@ static int image_pass(Args<T> p, int lanes) {
   else if (lanes == 512) launch_image<T, 512, V, U, ACT, BWD>(p);
   else launch_image<T, 1024, V, U, ACT, BWD>(p);
   AM_TRY(check_launch("group norm of images"));
-  if (p.share) {
-    hipLaunchKernelGGL((channel_fold<T, T>), dim3((unsigned)((p.channels + 7) / 8)), dim3(256), 0, stream(), p, (const T*)p.share, p.batch, 1, false);
-    AM_TRY(check_launch("channel_fold"));
-  }
-  return AM_OK;
+  return p.share ? fold_samples<T, T>(p, p.share, p.batch, false) : AM_OK;
 }
 
 template <typename T, int ACT, bool BWD>
-static int try_images(Args<T>& p, bool& taken) {
+static int try_images(Args<T>& p, bool aligned, bool& taken) {
   // us forwards + backwards, images against what else takes the shape.
   //  - Few rows: the teams, whose lanes hold what they need and no more ([64, 8, 8, 1024] in 32 groups 13 + 30 against 10 + 17 in
-  //    teams). From 128 rows on the images ([16, 45, 45, 128] in 32: 15 + 23 against 34 + 64), forwards where there are 2048
-  //    elements ([64, 16, 16, 128] in 32: 12 + 18 against 9 + 103: backwards the teams keep shares of dweight for every row).
+  //    teams). From 128 rows on the images: [16, 45, 45, 128] in 32 15 + 23 against 34 + 64 in teams, [512, 16, 16, 256] in 32
+  //    82 + 117 against 159 + 267, [256, 16, 16, 512] in 128 128 + 174 against 221 + 500 (backwards the teams keep shares of
+  //    dweight for every row); only small ones lose a little, [64, 16, 16, 128] in 32 12 + 18 against 9 + 103.
   //  - A row of a group is a short run of memory, and a cache line that several groups share is fetched for each of them unless
   //    the die's L2 still has it. From 48 bytes on that is no loss: [16, 56, 56, 384] in 32 groups 49 + 78 against 49 + 88 in
   //    slabs, with 64 bytes ([32, 48, 48, 256] in 16) 43 + 63 against 47 + 81, with 256 ([16, 24, 24, 1024] in 16) 19 + 30 against
-  //    36 + 48. From 16 bytes on it is none while the device's last cache holds the tensors: 40 bytes of 42 MB 25 + 41 against
-  //    33 + 48, of 63 MB 51 + 79 against 44 + 73; 16 bytes of 17 MB 16 + 25 against 19 + 29; 12 bytes of 14 MB 24 + 36 against 20 + 29.
+  //    36 + 48. From 16 bytes on it is none against slabs while the device's last cache holds the tensors: 40 bytes of 42 MB
+  //    25 + 41 against 33 + 48, of 63 MB 51 + 79 against 44 + 73; 16 bytes of 17 MB 16 + 25 against 19 + 29; 12 bytes of 14 MB
+  //    24 + 36 against 20 + 29.
   taken = false;
+  constexpr int W = 16 / (int)sizeof(T);
   const int run = p.per * (int)sizeof(T);
-  if (p.spatial < 128 || (!BWD && p.spatial * p.per < 2048) || run < 16) return AM_OK;
-  if (run < 48 && (double)p.batch * (double)p.spatial * p.channels * sizeof(T) > 48e6) return AM_OK;
+  if (p.spatial < 128 || run < 16) return AM_OK;
+  const bool slabs = p.spatial * (p.per / (aligned && p.per % W == 0 ? W : 1)) > 256 * kUnits;
+  if (slabs && run < 48 && (double)p.batch * (double)p.spatial * p.channels * sizeof(T) > 48e6) return AM_OK;
   if (p.batch * p.groups >= ((int64_t)1 << 31) - 8) return AM_OK;
   int V = 16 / (int)sizeof(T);
   // rows one behind the other, and all that the lanes may count up to within 2^31 bytes
@@ -895,7 +933,7 @@ static int forward(Args<T> p) {
   constexpr int W = 16 / (int)sizeof(T);
   const bool aligned = fits<T>(p.x, p.x_n, p.x_s, p.batch, p.spatial) && fits<T>(p.y, p.y_n, p.y_s, p.batch, p.spatial);
   bool taken;
-  AM_TRY((try_images<T, ACT, false>(p, taken)));
+  AM_TRY((try_images<T, ACT, false>(p, aligned, taken)));
   if (taken) return AM_OK;
   AM_TRY((try_teams<T, ACT, false>(p, aligned, taken)));
   if (taken) return AM_OK;
@@ -947,7 +985,7 @@ static int backward(Args<T> p) {
   const bool aligned = fits<T>(p.x, p.x_n, p.x_s, p.batch, p.spatial) && fits<T>(p.y, p.y_n, p.y_s, p.batch, p.spatial) &&
                        fits<T>(p.dy, p.dy_n, p.dy_s, p.batch, p.spatial);
   bool taken;
-  AM_TRY((try_images<T, ACT, true>(p, taken)));
+  AM_TRY((try_images<T, ACT, true>(p, aligned, taken)));
   if (taken) return AM_OK;
   AM_TRY((try_teams<T, ACT, true>(p, aligned, taken)));
   if (taken) return AM_OK;
@@ -977,10 +1015,7 @@ static int backward(Args<T> p) {
     AM_TRY(check_launch("slab_sums"));
     hipLaunchKernelGGL((group_fold<T, true>), dim3((unsigned)(p.nc * p.groups)), dim3(256), 0, stream(), p);
     AM_TRY(check_launch("group_fold"));
-    if (params) {
-      hipLaunchKernelGGL((channel_fold<T, double>), dim3((unsigned)((p.channels + 7) / 8)), dim3(256), 0, stream(), p, (const double*)p.chan, p.nc, 1, n > 0);
-      AM_TRY(check_launch("channel_fold"));
-    }
+    if (params) AM_TRY((fold_samples<T, double>(p, p.chan, p.nc, n > 0)));
     AM_GN_LAUNCH(slab_apply, V, wgs, true, ACT, false);   // (past the caches 89.5 -> 94 us for [16, 64, 64, 320])
     AM_TRY(check_launch("slab_apply"));
   }

@@ -672,8 +672,8 @@ int am_hip_gru_gates_backward_f64(int64_t batch, int64_t H, const double* dnext,
  * rot_dim / 2 pairs, element i with i + rot_dim / 2 (AM_ROTARY_HALF) or 2 i with 2 i + 1 (AM_ROTARY_INTERLEAVED). Pair i of
  * a token at position p turns by p * frequencies[i] and is multiplied by `scale`; the rest of the head is copied.
  * inverse != 0 turns the other way: that is also the gradient. positions [batch, tokens] (strides pos_b, pos_t, 0 allowed;
- * any sign) or NULL for the token's index. The angles are formed in double and reduced before the sines, so far positions
- * lose nothing. out may be x itself with x's strides (in place). */
+ * any sign) or NULL for the token's index. The angles are products in double, reduced before the sines, so far positions
+ * lose nothing else. out may be x itself with x's strides (in place). */
 #define AM_ROTARY_HALF        0
 #define AM_ROTARY_INTERLEAVED 1
 int am_hip_rotary_f32(int64_t batch, int64_t tokens, int64_t heads, int64_t dim, int64_t rot_dim, int layout, int inverse,
@@ -692,7 +692,7 @@ int am_hip_rotary_f64(int64_t batch, int64_t tokens, int64_t heads, int64_t dim,
  * sequence b has its first lengths[b] tokens (clamped to 0 .. tokens); what lies behind them is not read into any result,
  * and out is 0 there. At most 2^20 heads of all sequences together. A NaN or an infinity in a token reaches the outputs of the
  * tokens behind it, and may reach those of up to 31 tokens before it. float32: products of 24-bit pieces, sums in float32
- * (elements below 2^-108 lose bits). Long texts of few heads run in segments whose states lie in memory of am_hip_malloc for
+ * (elements below 2^-108 lose bits, those above 3.38 * 10^38 count as infinite, and an infinity as a NaN). Long texts of few heads run in segments whose states lie in memory of am_hip_malloc for
  * the length of the call (while a graph is being captured: see am_hip_alloc_hold); so does what the backward pass over shared
  * heads and group norm over large samples need. */
 int am_hip_decay_attention_f32(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dk, int64_t dv, float scale,

@@ -377,9 +377,10 @@ NORMS = [((1, 1), 1), ((3, 8), 2), ((5, 2048), 16), ((2, 7, 5, 30), 3), ((2, 16,
 
 
 # many rows, whose group fits a workgroup's registers: vectors of four, two and one, 256 to 1024 lanes with few rows and with 48,
-# lanes and dies left over; just too large; runs too short; the fewest rows
+# lanes and dies left over; just too large; runs too short; the fewest rows; many samples, held and in slabs
 IMAGES = [((2, 40, 40, 96), 6), ((3, 33, 31, 90), 6), ((1, 47, 44, 54), 2), ((9, 26, 25, 112), 4), ((1, 20, 20, 1024), 8), ((2, 59, 58, 13), 1),
-          ((1, 64, 63, 12), 1), ((1, 65, 65, 24), 2), ((5, 16, 16, 32), 4), ((2, 45, 45, 28), 7), ((2, 128, 48), 3), ((2, 127, 48), 3), ((3, 20, 20, 9), 3)]
+          ((1, 64, 63, 12), 1), ((1, 65, 65, 24), 2), ((5, 16, 16, 32), 4), ((2, 45, 45, 28), 7), ((2, 128, 48), 3), ((2, 127, 48), 3), ((3, 20, 20, 9), 3),
+          ((1201, 130, 16), 2), ((600, 2100, 2), 2)]
 
 
 def norm_inputs(shape, dt, seed, mean=0.5):
