@@ -47,8 +47,8 @@ template <typename T> __device__ __forceinline__ T power(T g, int64_t n) { retur
 // For the tokens of a chunk, i and j counted within it, and the state S in front of it,
 //     o_i = sum_{j <= i} A_ij c_j + e^{g (i + after)} a_i S      A_ij = e^{g (i - j)} (a_i . b_j)
 //     S <- e^{g N} S + sum_j e^{g (N - after - j)} b_j^T c_j
-// so a chunk is four products: a b^T (32 x 32), A c, a S and b^T c. A workgroup of four wavefronts walks the chunks of one
-// head, a wavefront owning columns of S and of o for all da rows, as accumulators that never leave its registers: the product
+// so a chunk is four products: a b^T (32 x 32), A c, a S and b^T c. A workgroup walks the chunks of one head, a wavefront
+// owning columns of S and of o for all da rows (or half of them, below), as accumulators that never leave its registers: the product
 // instructions leave neighbouring rows of a result in a lane, and the sum over k may take its k in any order that both
 // operands share, so the rows of S a lane holds are k of the next product's right operand as they stand.
 //   - a b^T is computed transposed, so that a lane's four values lie next to each other in a row of A in LDS; the three
@@ -61,7 +61,7 @@ template <typename T> __device__ __forceinline__ T power(T g, int64_t n) { retur
 // a sixteenth of the bfloat16 rate: every operand is the sum of three bfloat16 (8 bits each, 24 in all: `split`), and a
 // product takes the six pairs of pieces down to 2^-16 (the three that are left out are below 2^-24 of the term, a float's
 // half step), with float32 sums inside the instruction: `chunks_f32`. Measured on 4 x 4096 tokens, 16 heads of 128 x 128:
-// 291 us with the float instruction, 223 us in pieces.
+// 291 us with the float instruction, 223 us in pieces, both before the steps noted at the kernels below; with them 212.
 //
 // Where the heads alone do not fill the device, the tokens are cut into segments: `sums_*` add up each segment's share of the
 // state, `segment_states` carries them from segment to segment, and the chunk kernels start every segment from its own.
@@ -751,7 +751,7 @@ __global__ __launch_bounds__(64 * WAVES, (kWaves<DA, WAVES>)) void chunks_f32(Ro
       }
     }
     if (live && m > 16 * half) put_o<float, acc32, FAST, 2 / HALVES>(e, path.o + (at + 16 * half) * path.to, path.to, m - 16 * half, g, col, p.dc);
-    if (next < path.total) fetch(next);                     // (not earlier: its registers are wanted until here)
+    if (next < path.total) fetch(next);                     // (in front of A's tiles: the same time, and more registers)
 #pragma unroll
     for (int jt = 0; jt < 2; ++jt)
 #pragma unroll

@@ -650,6 +650,62 @@ def test_a_layer_in_a_graph(hip):
         assert np.array_equal(res.toCpu(), want) and np.array_equal(live.toCpu(), mirror.toCpu()), f"step {turn}"
 
 
+@pytest.mark.parametrize("shape,groups", [((3, 20, 20, 48), 3), ((600, 130, 16), 2), ((2, 70, 71, 24), 8)], ids=str)
+def test_group_norm_of_images_in_a_graph(hip, shape, groups):
+    """Held groups, many samples' sums in runs, and slabs, with the memory they take for the call, recorded twice and replayed in
+    turn: the eager bits every time."""
+    made = []
+    for i in range(2):
+        x, w, b, dy = (hip.toHip(a) for a in norm_inputs(shape, "f32", seed_of("norm graph", shape, i)))
+
+        def train(into=None, x=x, w=w, b=b, dy=dy):
+            y, mean, rstd = hip.group_norm_forward(x, w, b, groups, activation="silu")
+            got = (y,) + hip.group_norm_backward(dy, x, w, b, mean, rstd, groups, activation="silu")
+            if into is None:
+                return got
+            for dst, src in zip(into, got):
+                _unary_into("copy", dst, src)
+
+        eager = train()
+        into = [hip.empty(t.shape, np.float32) for t in eager]
+        made.append((hip.Graph.record(lambda train=train, into=into: train(into)), into, [t.toCpu() for t in eager], train))
+    for turn in range(3):
+        for g, into, want, train in made:
+            g.launch()
+            train()                                                          # the program's own work between
+            for t, w in zip(into, want):
+                assert np.array_equal(t.toCpu(), w), f"replay {turn}"
+
+
+@pytest.mark.parametrize("dt", ["f32", "f64"])
+def test_decay_attention_in_segments_in_a_graph(hip, dt):
+    """Few heads over many tokens, key / value heads shared, padded, a state carried on: segments, their states and the shared heads'
+    shares all lie in memory taken for the call."""
+    x = attention_inputs(hip, (2, 515, 4, 2, 64, 48), dt, seed_of("segments graph", dt))
+    x["lengths"][:] = (515, 131)
+    d = {n: hip.toHip(a) for n, a in x.items() if n != "scale"}
+
+    def train():
+        out = hip.decay_attention(d["q"], d["k"], d["v"], d["g"], state=d["state"], lengths=d["lengths"], scale=x["scale"])
+        return out + hip.decay_attention_backward(d["go"], d["q"], d["k"], d["v"], d["g"], state=d["state"], lengths=d["lengths"], scale=x["scale"],
+                                                  gradState=d["gs"])
+
+    eager = train()
+    want = [t.toCpu() for t in eager]
+    into = [hip.empty(t.shape, DTYPES[dt]) for t in eager]
+
+    def record():
+        for dst, src in zip(into, train()):
+            _unary_into("copy", dst, src)
+
+    g = hip.Graph.record(record)
+    for turn in range(3):
+        g.launch()
+        train()
+        for t, w in zip(into, want):
+            assert np.array_equal(t.toCpu(), w), f"replay {turn}"
+
+
 # ---------------------------------------------------------------------- the C++ host layer
 def test_the_cpp_host_layer(hip):
     program = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "test_sequence")
