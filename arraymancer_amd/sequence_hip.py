@@ -48,6 +48,15 @@ def _entry(name: str, t: HipTensor):
 
 def _new(shape, dtype) -> HipTensor:
     """`empty` for a shape of ints and a float dtype that have been looked at already: a small operator's call is mostly host time."""
+    if len(shape) == 2:
+        a, b = shape
+        return HipTensor(Layout(shape, (b, 1), 0), HipStorage(a * b, dtype.itemsize), dtype)
+    if len(shape) == 3:
+        a, b, c = shape
+        return HipTensor(Layout(shape, (b * c, c, 1), 0), HipStorage(a * b * c, dtype.itemsize), dtype)
+    if len(shape) == 4:
+        a, b, c, d = shape
+        return HipTensor(Layout(shape, (b * c * d, c * d, d, 1), 0), HipStorage(a * b * c * d, dtype.itemsize), dtype)
     strides, n = [], 1
     for d in reversed(shape):
         strides.append(n)
@@ -131,7 +140,11 @@ def _rotate(name, out: HipTensor | None, x: HipTensor, positions: HipTensor | No
     if out is None:
         out = _new(shape, x.dtype)
     src = x if x is out else _unit_rows(x)
-    check(fn(B, T, H, D, R, ROTARY[layout], inverse, scale, pp, pb, pt, frequencies.data_ptr(), *_rows(src), *_rows(out)))
+    xs, os = src.layout.strides, out.layout.strides
+    code = fn(B, T, H, D, R, ROTARY[layout], inverse, scale, pp, pb, pt, frequencies.data_ptr(), src.data_ptr(), xs[0], xs[1], xs[2],
+              out.data_ptr(), os[0], os[1], os[2])
+    if code:
+        check(code)
     return out
 
 
@@ -160,7 +173,9 @@ def _attention_sizes(name, q, k, v, log_decay, lead):
     qs, ks, vs = q.layout.shape, k.layout.shape, v.layout.shape
     if not (len(qs) == len(ks) == len(vs) == lead + 2):
         raise ValueError(f"{name}: q, k and v of rank {lead + 2} are needed, not {q.rank}, {k.rank} and {v.rank}")
-    _same_dtype(q, k, v, log_decay)
+    dt = q.dtype
+    if k.dtype is not dt or v.dtype is not dt or log_decay.dtype is not dt:
+        _same_dtype(q, k, v, log_decay)
     front, H, dk = qs[:lead], qs[lead], qs[lead + 1]
     KH, dv = vs[lead:]
     if ks != front + (KH, dk) or vs[:lead] != front:
@@ -173,10 +188,11 @@ def _attention_sizes(name, q, k, v, log_decay, lead):
 
 def _head_state(name, t: HipTensor, shape, like: HipTensor):
     """Pointer and (batch, head) strides of a state [batch, heads, dk, dv] whose heads are contiguous."""
-    _same_dtype(like, t)
+    if t.dtype is not like.dtype:
+        _same_dtype(like, t)
     _shape(name, "a state", t, shape)
-    s = t.strides
-    if (shape[3] > 1 and s[3] != 1) or (shape[2] > 1 and s[2] != shape[3]):
+    s = t.layout.strides
+    if (s[3] != 1 and shape[3] > 1) or (s[2] != shape[3] and shape[2] > 1):
         raise ValueError(f"{name}: each head of a state must be contiguous")
     return t.data_ptr(), s[0], s[1]
 
@@ -245,7 +261,11 @@ def decay_attention_step(q: HipTensor, k: HipTensor, v: HipTensor, log_decay: Hi
     s = _head_state(name, state, (B, H, dk, dv), q)
     q, k, v, g = _unit_rows(q), _unit_rows(k), _unit_rows(v), _unit_rows(log_decay)
     out = _new((B, H, dv), q.dtype)
-    check(fn(B, H, KH, dk, dv, scale, g.data_ptr(), *_rows(q), *_rows(k), *_rows(v), *s, *_rows(out)))
+    qs, ks, vs = q.layout.strides, k.layout.strides, v.layout.strides
+    code = fn(B, H, KH, dk, dv, scale, g.data_ptr(), q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+              *s, out.storage.ptr, H * dv, dv)
+    if code:
+        check(code)
     return out
 
 
@@ -253,7 +273,9 @@ def decay_attention_step(q: HipTensor, k: HipTensor, v: HipTensor, log_decay: Hi
 def _channels_last(t: HipTensor):
     """(tensor, row stride of the sample, row stride of a position) of t [batch, ..., channels] with the middle dimensions
     walked as one; a copy where the strides do not allow that."""
-    s, sh = t.strides, t.shape
+    s, sh = t.layout.strides, t.layout.shape
+    if len(sh) == 2 and s[1] == 1:
+        return t, s[0], sh[1]
     if s[-1] == 1 or sh[-1] == 1:
         step, ok = None, True
         for d in range(t.rank - 2, 0, -1):
@@ -271,11 +293,11 @@ def _channels_last(t: HipTensor):
 
 
 def _norm_sizes(name, x: HipTensor, weight, bias, groups: int, activation: str):
-    if x.rank < 2:
+    shape = x.layout.shape
+    if len(shape) < 2:
         raise ValueError(f"{name}: a tensor [batch, ..., channels] is needed")
     if activation not in ACT:
         raise ValueError(f"{name}: unknown activation {activation!r}, one of {', '.join(ACT)}")
-    shape = x.layout.shape
     C = shape[-1]
     spatial = 1
     for d in shape[1:-1]:
@@ -284,7 +306,8 @@ def _norm_sizes(name, x: HipTensor, weight, bias, groups: int, activation: str):
         raise ValueError(f"{name}: {C} channels cannot form {groups} groups")
     for what, w in (("weight", weight), ("bias", bias)):
         if w is not None:
-            _same_dtype(x, w)
+            if w.dtype is not x.dtype:
+                _same_dtype(x, w)
             ws = w.layout.shape
             if ws != (C,) and ws != (1, C):
                 raise ValueError(f"{name}: {what} of shape {list(w.shape)} for {C} channels")
@@ -310,7 +333,9 @@ def _normalise(name, x, weight, bias, groups, eps, activation, keep):
     if keep:
         make = _new if S * C else zeros
         mean, rstd = make((B, groups), x.dtype), make((B, groups), x.dtype)
-    check(fn(B, S, C, groups, eps, ACT[activation], src.data_ptr(), sn, ss, _ptr(w), _ptr(b), y.data_ptr(), S * C, C, _ptr(mean), _ptr(rstd)))
+    code = fn(B, S, C, groups, eps, ACT[activation], src.data_ptr(), sn, ss, _ptr(w), _ptr(b), y.storage.ptr, S * C, C, _ptr(mean), _ptr(rstd))
+    if code:
+        check(code)
     return y, mean, rstd
 
 
