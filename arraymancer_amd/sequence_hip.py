@@ -48,6 +48,8 @@ def _entry(name: str, t: HipTensor):
 
 def _new(shape, dtype) -> HipTensor:
     """`empty` for a shape of ints and a float dtype that have been looked at already: a small operator's call is mostly host time."""
+    if len(shape) == 1:
+        return HipTensor(Layout(shape, (1,), 0), HipStorage(shape[0], dtype.itemsize), dtype)
     if len(shape) == 2:
         a, b = shape
         return HipTensor(Layout(shape, (b, 1), 0), HipStorage(a * b, dtype.itemsize), dtype)
@@ -361,16 +363,21 @@ def group_norm_backward(gradOutput: HipTensor, x: HipTensor, weight: HipTensor |
     name = "group_norm_backward"
     fn = _entry(name, x)
     B, S, C = _norm_sizes(name, x, weight, bias, groups, activation)
-    _same_dtype(x, gradOutput, mean, rstd)
-    _shape(name, "the output's gradient", gradOutput, x.shape)
+    dt = x.dtype
+    if gradOutput.dtype is not dt or mean.dtype is not dt or rstd.dtype is not dt:
+        _same_dtype(x, gradOutput, mean, rstd)
+    _shape(name, "the output's gradient", gradOutput, x.layout.shape)
     _shape(name, "mean", mean, (B, groups))
     _shape(name, "rstd", rstd, (B, groups))
     src, xn, xs = _channels_last(x)
     dy, gn, gs = _channels_last(gradOutput)
-    w, b, m, r = _vector(weight), _vector(bias), mean.asContiguous(), rstd.asContiguous()
-    dx = _new(x.shape, x.dtype)
-    dw = _new(weight.shape, x.dtype) if weight is not None else None
-    db = _new(bias.shape, x.dtype) if bias is not None else None
-    check(fn(B, S, C, groups, ACT[activation], dy.data_ptr(), gn, gs, src.data_ptr(), xn, xs, _ptr(w), _ptr(b), m.data_ptr(), r.data_ptr(),
-             dx.data_ptr(), S * C, C, _ptr(dw), _ptr(db)))
+    w, b = _vector(weight), _vector(bias)
+    m, r = (t if t.layout.strides == (groups, 1) else t.asContiguous() for t in (mean, rstd))
+    dx = _new(x.layout.shape, dt)
+    dw = _new(weight.layout.shape, dt) if weight is not None else None
+    db = _new(bias.layout.shape, dt) if bias is not None else None
+    code = fn(B, S, C, groups, ACT[activation], dy.data_ptr(), gn, gs, src.data_ptr(), xn, xs, _ptr(w), _ptr(b), m.data_ptr(), r.data_ptr(),
+              dx.storage.ptr, S * C, C, _ptr(dw), _ptr(db))
+    if code:
+        check(code)
     return dx, dw, db
