@@ -41,6 +41,7 @@ template <typename T> struct Args {
   int channels, groups, per;
   int64_t n0, nc;                    // samples of this launch: n0 .. n0 + nc
   int slabs; int64_t rows_per_slab;
+  int folds;                         // slabs, backward: the first so many workgroups of the second pass fold the parameters' gradients
   int tiles, lanes, rows_at_once;    // channel tiles; lanes per row of a tile; rows a workgroup reads at once
   FastDiv per_div, tiles_div, slabs_div, groups_div, units_div;
 };
@@ -454,9 +455,9 @@ __global__ __launch_bounds__(LANES, 4) void image_backward(Args<T> p) {
 
 // Where a lane of the slab kernels stands: its sample, slab, first channel and first row.
 struct Place { int64_t n; int slab, c, row0; bool live; };
-template <typename T, int V> __device__ __forceinline__ Place place(const Args<T>& p) {
+template <typename T, int V> __device__ __forceinline__ Place place(const Args<T>& p, unsigned id) {
   uint32_t tile, slab;
-  const uint32_t rest = p.tiles_div.divmod(blockIdx.x, tile);
+  const uint32_t rest = p.tiles_div.divmod(id, tile);
   Place w;
   w.n = p.slabs_div.divmod(rest, slab);
   w.slab = (int)slab;
@@ -471,7 +472,7 @@ template <typename T, int V, bool BWD, int ACT>
 __global__ __launch_bounds__(256) void slab_sums(Args<T> p) {
   typedef typename Vec<T, V>::type vec_t;
   __shared__ double lds[256 * V * 2];
-  const Place w = place<T, V>(p);
+  const Place w = place<T, V>(p, blockIdx.x);
   double a[V], b[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) a[e] = b[e] = 0.0;
@@ -629,11 +630,11 @@ __global__ __launch_bounds__(256) void group_fold(Args<T> p) {
 
 // dweight and dbias of 8 channels: 8 lanes side by side, 32 of them over the parts, folded through LDS. Part i (slot, row) of
 // channel c (group, channel of it) lies at ((slot * groups + group) * rows + row) * per + channel; rows = 1: at i * channels + c.
-template <typename T, typename P>
-__global__ __launch_bounds__(256) void channel_fold(Args<T> p, const P* part, int64_t slots, int rows, bool add) {
+template <int DEPTH, typename T, typename P>
+__device__ __forceinline__ void fold_channels(const Args<T>& p, const P* part, int64_t slots, int rows, bool add, int block) {
   typedef typename Vec<P, 2>::type pair_t;
   __shared__ double lds[256][2];
-  const int c = (int)blockIdx.x * 8 + ((int)threadIdx.x & 7), k = (int)threadIdx.x >> 3;
+  const int c = block * 8 + ((int)threadIdx.x & 7), k = (int)threadIdx.x >> 3;
   double a = 0.0, b = 0.0;
   if (c < p.channels) {
     uint32_t cg;
@@ -642,12 +643,12 @@ __global__ __launch_bounds__(256) void channel_fold(Args<T> p, const P* part, in
     const int64_t pitch = (int64_t)p.channels * rows, parts = slots * rows;
     auto where = [&](int64_t i) { const int64_t slot = rows == 1 ? i : i / rows; return slot * pitch + (i - slot * rows) * p.per; };
     int64_t i = k;
-    for (; i + 7 * 32 < parts; i += 8 * 32) {
-      pair_t v[8];
+    for (; i + (DEPTH - 1) * 32 < parts; i += DEPTH * 32) {
+      pair_t v[DEPTH];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) v[u] = at[where(i + u * 32)];
+      for (int u = 0; u < DEPTH; ++u) v[u] = at[where(i + u * 32)];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) { a += (double)v[u][0]; b += (double)v[u][1]; }
+      for (int u = 0; u < DEPTH; ++u) { a += (double)v[u][0]; b += (double)v[u][1]; }
     }
     for (; i < parts; i += 32) { const pair_t v = at[where(i)]; a += (double)v[0]; b += (double)v[1]; }
   }
@@ -655,9 +656,15 @@ __global__ __launch_bounds__(256) void channel_fold(Args<T> p, const P* part, in
   lds[threadIdx.x][1] = b;
   __syncthreads();
   if (k != 0 || c >= p.channels) return;
+#pragma unroll 4                     // (all at once is 132 registers, for every wavefront of the second pass)
   for (int r = 1; r < 32; ++r) { a += lds[threadIdx.x + 8 * r][0]; b += lds[threadIdx.x + 8 * r][1]; }
   if (p.dweight) p.dweight[c] = (T)(add ? (double)p.dweight[c] + a : a);
   if (p.dbias) p.dbias[c] = (T)(add ? (double)p.dbias[c] + b : b);
+}
+
+template <typename T, typename P>
+__global__ __launch_bounds__(256) void channel_fold(Args<T> p, const P* part, int64_t slots, int rows, bool add) {
+  fold_channels<8>(p, part, slots, rows, add, (int)blockIdx.x);
 }
 
 // Sums over `each` samples at a time of [samples, columns] (a lane stays with a column), in a fixed order.
@@ -683,7 +690,13 @@ __global__ __launch_bounds__(256) void sample_sums(const P* part, double* out, i
 template <typename T, int V, bool BWD, int ACT, bool NT>
 __global__ __launch_bounds__(256) void slab_apply(Args<T> p) {
   typedef typename Vec<T, V>::type vec_t;
-  const Place w = place<T, V>(p);
+  if constexpr (BWD) {
+    if (blockIdx.x < (unsigned)p.folds) {                  // uniform
+      fold_channels<4>(p, (const double*)p.chan, p.nc, 1, p.n0 > 0, (int)blockIdx.x);
+      return;
+    }
+  }
+  const Place w = place<T, V>(p, blockIdx.x - (BWD ? (unsigned)p.folds : 0u));
   if (!w.live) return;
   T mean[V], rstd[V], wt[V], bs[V], c1[V], c2[V];
 #pragma unroll
@@ -1015,8 +1028,11 @@ static int backward(Args<T> p) {
     AM_TRY(check_launch("slab_sums"));
     hipLaunchKernelGGL((group_fold<T, true>), dim3((unsigned)(p.nc * p.groups)), dim3(256), 0, stream(), p);
     AM_TRY(check_launch("group_fold"));
-    if (params) AM_TRY((fold_samples<T, double>(p, p.chan, p.nc, n > 0)));
-    AM_GN_LAUNCH(slab_apply, V, wgs, true, ACT, false);   // (past the caches 89.5 -> 94 us for [16, 64, 64, 320])
+    // Few samples' sums per channel are folded beside the second pass ([16, 64, 64, 320] 89.8 -> 87.3 us), many before it.
+    p.n0 = n;
+    p.folds = params && p.nc <= 512 ? (p.channels + 7) / 8 : 0;
+    if (params && !p.folds) AM_TRY((fold_samples<T, double>(p, p.chan, p.nc, n > 0)));
+    AM_GN_LAUNCH(slab_apply, V, wgs + p.folds, true, ACT, false);   // (past the caches 89.5 -> 94 us for [16, 64, 64, 320])
     AM_TRY(check_launch("slab_apply"));
   }
   return AM_OK;
