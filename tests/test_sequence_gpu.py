@@ -488,6 +488,32 @@ def test_group_norm_of_views(hip, shape, groups, dt):
             close(a.toCpu(), c.astype(np.float64), 2 * t, name)
 
 
+def test_group_norm_of_more_samples_than_its_scratch_holds(hip):
+    """2100 samples of 8192 channels in one group: their sums take more than 256 MB, so the slabs run in two launches and the second
+    adds to the parameters' gradients of the first."""
+    B, S, C = 2100, 2, 8192
+    rng = np.random.default_rng(91)
+    x, dy = rng.standard_normal((B, S, C), dtype=np.float32) * np.float32(2), rng.standard_normal((B, S, C), dtype=np.float32)
+    X, DY, w, b = hip.toHip(x), hip.toHip(dy), hip.toHip(np.ones(C, np.float32)), hip.toHip(np.zeros(C, np.float32))
+    y, mean, rstd = hip.group_norm_forward(X, w, b, 1)
+    dx, dw, db = (t.toCpu() for t in hip.group_norm_backward(DY, X, w, b, mean, rstd, 1))
+    sums, sizes = np.zeros((2, C)), np.zeros((2, C))
+    for n in range(0, B, 300):
+        d = dy[n:n + 300].astype(np.float64)
+        xhat = ref.norm(x[n:n + 300], None, None, 1, 1e-5)
+        for i, a in enumerate((d * xhat, d)):
+            sums[i] += a.sum((0, 1))
+        sizes[0] += (np.abs(d) * (np.abs(xhat) + 1)).sum((0, 1))
+        sizes[1] += np.abs(d).sum((0, 1))
+    # xhat: mean, rstd (2), difference, product; the product with dy, four rows in float, the result: 10 u of |dy| (|xhat| + 1)
+    close(dw, sums[0], 10 * 2.0 ** -24 * sizes[0], "dweight")
+    close(db, sums[1], 5 * 2.0 ** -24 * sizes[1], "dbias")
+    part = slice(2040, 2056)                                                 # on both sides of the seam
+    by, bdx, _, _ = norm_bounds(x[part], None, None, dy[part], 1, 1e-5, "f32")
+    close(y.toCpu()[part], ref.norm(x[part], None, None, 1, 1e-5), by, "y")
+    close(dx[part], ref.norm_backward(dy[part], x[part], None, None, 1, 1e-5)[0], bdx, "dx")
+
+
 @pytest.mark.parametrize("shape,groups", [((0, 8), 2), ((3, 0, 8), 4), ((0, 4, 4, 6), 1)], ids=str)
 def test_group_norm_of_nothing(hip, shape, groups):
     x = np.zeros(shape, np.float32)
