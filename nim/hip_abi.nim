@@ -171,14 +171,14 @@ proc am_hip_gru_gates_f32*(batch, H: int64, w3x: ptr cfloat, ldw: int64, u3h: pt
 proc am_hip_gru_gates_f64*(batch, H: int64, w3x: ptr cdouble, ldw: int64, u3h: ptr cdouble, ldu: int64, hidden: ptr cdouble, ldh: int64, r, z, n, uh: ptr cdouble, lds: int64): cint {.importc.}
 proc am_hip_gru_gates_backward_f32*(batch, H: int64, dnext, h, r, z, n, uh: ptr cfloat, ld_in: int64, dw3x: ptr cfloat, ldw: int64, du3h: ptr cfloat, ldu: int64): cint {.importc.}
 proc am_hip_gru_gates_backward_f64*(batch, H: int64, dnext, h, r, z, n, uh: ptr cdouble, ld_in: int64, dw3x: ptr cdouble, ldw: int64, du3h: ptr cdouble, ldu: int64): cint {.importc.}
-proc am_hip_rotary_f32*(batch, tokens, heads, dim, rot_dim: int64; layout, inverse: cint; scale: cfloat; positions: ptr int64; pos_b, pos_t: int64; frequencies: ptr cdouble; x: ptr cfloat; x_b, x_t, x_h: int64; out: ptr cfloat; out_b, out_t, out_h: int64): cint {.importc.}
-proc am_hip_rotary_f64*(batch, tokens, heads, dim, rot_dim: int64; layout, inverse: cint; scale: cdouble; positions: ptr int64; pos_b, pos_t: int64; frequencies, x: ptr cdouble; x_b, x_t, x_h: int64; out: ptr cdouble; out_b, out_t, out_h: int64): cint {.importc.}
-proc am_hip_decay_attention_f32*(batch, tokens, heads, kv_heads, dk, dv: int64; scale: cfloat; log_decay: ptr cfloat; lengths: ptr int64; q: ptr cfloat; q_b, q_t, q_h: int64; k: ptr cfloat; k_b, k_t, k_h: int64; v: ptr cfloat; v_b, v_t, v_h: int64; state_in: ptr cfloat; si_b, si_h: int64; out: ptr cfloat; o_b, o_t, o_h: int64; state_out: ptr cfloat; so_b, so_h: int64): cint {.importc.}
-proc am_hip_decay_attention_f64*(batch, tokens, heads, kv_heads, dk, dv: int64; scale: cdouble; log_decay: ptr cdouble; lengths: ptr int64; q: ptr cdouble; q_b, q_t, q_h: int64; k: ptr cdouble; k_b, k_t, k_h: int64; v: ptr cdouble; v_b, v_t, v_h: int64; state_in: ptr cdouble; si_b, si_h: int64; out: ptr cdouble; o_b, o_t, o_h: int64; state_out: ptr cdouble; so_b, so_h: int64): cint {.importc.}
+proc am_hip_rotary_f32*(batch, tokens, heads, dim, rot_dim: int64; layout, inverse: cint; scale: cfloat; positions: ptr int64; pos_b, pos_t: int64; frequencies: ptr cdouble; x: ptr cfloat; x_b, x_t, x_h: int64; res: ptr cfloat; out_b, out_t, out_h: int64): cint {.importc.}
+proc am_hip_rotary_f64*(batch, tokens, heads, dim, rot_dim: int64; layout, inverse: cint; scale: cdouble; positions: ptr int64; pos_b, pos_t: int64; frequencies, x: ptr cdouble; x_b, x_t, x_h: int64; res: ptr cdouble; out_b, out_t, out_h: int64): cint {.importc.}
+proc am_hip_decay_attention_f32*(batch, tokens, heads, kv_heads, dk, dv: int64; scale: cfloat; log_decay: ptr cfloat; lengths: ptr int64; q: ptr cfloat; q_b, q_t, q_h: int64; k: ptr cfloat; k_b, k_t, k_h: int64; v: ptr cfloat; v_b, v_t, v_h: int64; state_in: ptr cfloat; si_b, si_h: int64; res: ptr cfloat; o_b, o_t, o_h: int64; state_out: ptr cfloat; so_b, so_h: int64): cint {.importc.}
+proc am_hip_decay_attention_f64*(batch, tokens, heads, kv_heads, dk, dv: int64; scale: cdouble; log_decay: ptr cdouble; lengths: ptr int64; q: ptr cdouble; q_b, q_t, q_h: int64; k: ptr cdouble; k_b, k_t, k_h: int64; v: ptr cdouble; v_b, v_t, v_h: int64; state_in: ptr cdouble; si_b, si_h: int64; res: ptr cdouble; o_b, o_t, o_h: int64; state_out: ptr cdouble; so_b, so_h: int64): cint {.importc.}
 proc am_hip_decay_attention_backward_f32*(batch, tokens, heads, kv_heads, dk, dv: int64; scale: cfloat; log_decay: ptr cfloat; lengths: ptr int64; grad_out: ptr cfloat; g_b, g_t, g_h: int64; q: ptr cfloat; q_b, q_t, q_h: int64; k: ptr cfloat; k_b, k_t, k_h: int64; v: ptr cfloat; v_b, v_t, v_h: int64; state_in: ptr cfloat; si_b, si_h: int64; grad_state_out: ptr cfloat; gso_b, gso_h: int64; grad_q: ptr cfloat; gq_b, gq_t, gq_h: int64; grad_k: ptr cfloat; gk_b, gk_t, gk_h: int64; grad_v: ptr cfloat; gv_b, gv_t, gv_h: int64; grad_state_in: ptr cfloat; gsi_b, gsi_h: int64): cint {.importc.}
 proc am_hip_decay_attention_backward_f64*(batch, tokens, heads, kv_heads, dk, dv: int64; scale: cdouble; log_decay: ptr cdouble; lengths: ptr int64; grad_out: ptr cdouble; g_b, g_t, g_h: int64; q: ptr cdouble; q_b, q_t, q_h: int64; k: ptr cdouble; k_b, k_t, k_h: int64; v: ptr cdouble; v_b, v_t, v_h: int64; state_in: ptr cdouble; si_b, si_h: int64; grad_state_out: ptr cdouble; gso_b, gso_h: int64; grad_q: ptr cdouble; gq_b, gq_t, gq_h: int64; grad_k: ptr cdouble; gk_b, gk_t, gk_h: int64; grad_v: ptr cdouble; gv_b, gv_t, gv_h: int64; grad_state_in: ptr cdouble; gsi_b, gsi_h: int64): cint {.importc.}
-proc am_hip_decay_attention_step_f32*(batch, heads, kv_heads, dk, dv: int64; scale: cfloat; log_decay, q: ptr cfloat; q_b, q_h: int64; k: ptr cfloat; k_b, k_h: int64; v: ptr cfloat; v_b, v_h: int64; state: ptr cfloat; s_b, s_h: int64; out: ptr cfloat; o_b, o_h: int64): cint {.importc.}
-proc am_hip_decay_attention_step_f64*(batch, heads, kv_heads, dk, dv: int64; scale: cdouble; log_decay, q: ptr cdouble; q_b, q_h: int64; k: ptr cdouble; k_b, k_h: int64; v: ptr cdouble; v_b, v_h: int64; state: ptr cdouble; s_b, s_h: int64; out: ptr cdouble; o_b, o_h: int64): cint {.importc.}
+proc am_hip_decay_attention_step_f32*(batch, heads, kv_heads, dk, dv: int64; scale: cfloat; log_decay, q: ptr cfloat; q_b, q_h: int64; k: ptr cfloat; k_b, k_h: int64; v: ptr cfloat; v_b, v_h: int64; state: ptr cfloat; s_b, s_h: int64; res: ptr cfloat; o_b, o_h: int64): cint {.importc.}
+proc am_hip_decay_attention_step_f64*(batch, heads, kv_heads, dk, dv: int64; scale: cdouble; log_decay, q: ptr cdouble; q_b, q_h: int64; k: ptr cdouble; k_b, k_h: int64; v: ptr cdouble; v_b, v_h: int64; state: ptr cdouble; s_b, s_h: int64; res: ptr cdouble; o_b, o_h: int64): cint {.importc.}
 proc am_hip_group_norm_f32*(batch, spatial, channels, groups: int64; eps: cfloat; activation: cint; x: ptr cfloat; x_n, x_s: int64; weight, bias, y: ptr cfloat; y_n, y_s: int64; mean, rstd: ptr cfloat): cint {.importc.}
 proc am_hip_group_norm_f64*(batch, spatial, channels, groups: int64; eps: cdouble; activation: cint; x: ptr cdouble; x_n, x_s: int64; weight, bias, y: ptr cdouble; y_n, y_s: int64; mean, rstd: ptr cdouble): cint {.importc.}
 proc am_hip_group_norm_backward_f32*(batch, spatial, channels, groups: int64; activation: cint; dy: ptr cfloat; dy_n, dy_s: int64; x: ptr cfloat; x_n, x_s: int64; weight, bias, mean, rstd, dx: ptr cfloat; dx_n, dx_s: int64; dweight, dbias: ptr cfloat): cint {.importc.}
