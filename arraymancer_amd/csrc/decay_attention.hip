@@ -1117,8 +1117,13 @@ static int check_sizes(const char* fn, int64_t batch, int64_t tokens, int64_t he
 
 template <typename T> struct Strided { const T* p; int64_t b, t, h; };
 template <typename T> struct Result { T* p; int64_t b, t, h; };
-template <typename T> static bool broadcast_result(const Result<T>& r, int64_t batch, int64_t tokens, int64_t heads) {
-  return tokens > 0 && ((batch > 1 && r.b == 0) || (tokens > 1 && r.t == 0) || (heads > 1 && r.h == 0));
+template <typename T> static bool broadcast_result(const Result<T>& r, int64_t batch, int64_t tokens, int64_t heads, int64_t width) {
+  return tokens > 0 && ((batch > 1 && r.b == 0) || (tokens > 1 && r.t < width && -r.t < width) || (heads > 1 && r.h == 0));
+}
+// Any token stride will do for a single token, but the chunks write whole tiles of rows and leave it to the buffer's end to drop
+// those behind the last token: a row's width at least has to lie between them.
+template <typename T> static void one_token(Result<T>& r, int64_t tokens, int64_t width) {
+  if (tokens == 1) r.t = width;
 }
 
 template <typename T>
@@ -1128,8 +1133,9 @@ static int forward(const char* fn, int64_t batch, int64_t tokens, int64_t heads,
   AM_TRY(check_sizes(fn, batch, tokens, heads, kv_heads, dk, dv));
   if (batch == 0 || heads == 0) return AM_OK;
   if (!log_decay || (tokens && (!q.p || !k.p || !v.p || !out.p))) return fail(AM_E_ARG, "%s: null tensor pointer", fn);
-  if (broadcast_result(out, batch, tokens, heads) || (s1 && ((batch > 1 && s1_b == 0) || (heads > 1 && s1_h == 0))))
-    return fail(AM_E_SHAPE, "%s: a result is a broadcast view", fn);
+  if (broadcast_result(out, batch, tokens, heads, dv) || (s1 && ((batch > 1 && s1_b == 0) || (heads > 1 && s1_h == 0))))
+    return fail(AM_E_SHAPE, "%s: a result is a broadcast view, or its tokens overlap", fn);
+  one_token(out, tokens, dv);
   AM_TRY(ensure_init());
   const int group = (int)(heads / kv_heads);
   Role<T> p = {};
@@ -1184,9 +1190,13 @@ static int backward(const char* fn, int64_t batch, int64_t tokens, int64_t heads
   AM_TRY(check_sizes(fn, batch, tokens, heads, kv_heads, dk, dv));
   if (batch == 0 || heads == 0) return AM_OK;
   if (!log_decay || (tokens && (!go.p || !q.p || !k.p || !v.p || !dq.p || !dkey.p || !dval.p))) return fail(AM_E_ARG, "%s: null tensor pointer", fn);
-  if (broadcast_result(dq, batch, tokens, heads) || broadcast_result(dkey, batch, tokens, kv_heads) || broadcast_result(dval, batch, tokens, kv_heads) ||
+  if (broadcast_result(dq, batch, tokens, heads, dk) || broadcast_result(dkey, batch, tokens, kv_heads, dk) ||
+      broadcast_result(dval, batch, tokens, kv_heads, dv) ||
       (gs0 && ((batch > 1 && gs0_b == 0) || (heads > 1 && gs0_h == 0))))
-    return fail(AM_E_SHAPE, "%s: a result is a broadcast view", fn);
+    return fail(AM_E_SHAPE, "%s: a result is a broadcast view, or its tokens overlap", fn);
+  one_token(dq, tokens, dk);
+  one_token(dkey, tokens, dk);
+  one_token(dval, tokens, dv);
   AM_TRY(ensure_init());
   const int group = (int)(heads / kv_heads);
   const Operand<T> Q = {q.p, q.b, q.t, q.h, 1}, G = {go.p, go.b, go.t, go.h, 1};

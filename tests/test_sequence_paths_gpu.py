@@ -1,0 +1,44 @@
+"""The sequence operators at the C interface's edges and along every way that their dispatch can take, on the device.
+
+u = half a step of the element type. Attention is compared with its closed form (no recurrence) in float64; a result that is a
+sum of products may be off by the roundings that a term passes, counted as in tests/test_sequence_gpu.py, times u times the sum
+of the absolute terms."""
+import numpy as np
+import pytest
+
+import sequence_reference as ref
+from arraymancer_amd._lib import last_error
+from arraymancer_amd.sequence_hip import _rows
+from conftest import DTYPES, seed_of
+from test_sequence_gpu import attention_inputs, close, roundings, unit
+
+pytestmark = pytest.mark.gpu
+
+
+def strided(t, token_stride):
+    """Pointer and strides of `t` [batch, tokens, heads, dim], with another token stride than its own."""
+    p, b, _, h = _rows(t)
+    return p, b, token_stride, h
+
+
+@pytest.mark.parametrize("stride", [0, 1, 7, -3])
+@pytest.mark.parametrize("dt", ["f32", "f64"])
+@pytest.mark.parametrize("dk,dv", [(8, 12), (64, 128), (7, 5)])
+def test_a_single_tokens_stride_does_not_matter(hip, dk, dv, dt, stride):
+    """With one token the token stride of an operand or a result leads nowhere, whatever it is: the bits of the packed call,
+    forwards and backwards, and nothing beside the results."""
+    B, H, KH = 3, 4, 4
+    x = attention_inputs(hip, (B, 1, H, KH, dk, dv), dt, seed_of("one token", dk, dv, dt))
+    d = {n: hip.toHip(a) for n, a in x.items() if n not in ("scale", "lengths")}
+    want = hip.decay_attention(d["q"], d["k"], d["v"], d["g"], state=d["state"], scale=0.5)
+    want += hip.decay_attention_backward(d["go"], d["q"], d["k"], d["v"], d["g"], state=d["state"], scale=0.5, gradState=d["gs"])
+    got = [hip.toHip(np.full(t.shape, 7, DTYPES[dt])) for t in want]
+    sizes = (B, 1, H, KH, dk, dv, 0.5, d["g"].data_ptr(), None)
+    q, k, v, go = (strided(d[n], stride) for n in ("q", "k", "v", "go"))
+    L = hip.load_library()
+    s0 = _rows(d["state"])[:3]
+    assert getattr(L, f"am_hip_decay_attention_{dt}")(*sizes, *q, *k, *v, *s0, *strided(got[0], stride), *_rows(got[1])[:3]) == 0, last_error()
+    assert getattr(L, f"am_hip_decay_attention_backward_{dt}")(*sizes, *go, *q, *k, *v, *s0, *_rows(d["gs"])[:3], *(a for t in got[2:5] for a in strided(t, stride)),
+                                                               *_rows(got[5])[:3]) == 0, last_error()
+    for a, b in zip(got, want):
+        assert np.array_equal(a.toCpu(), b.toCpu())
