@@ -8,9 +8,8 @@
 //
 // The angle depends on the token and the pair alone, so a lane keeps one 16-byte vector of pairs of one token, makes its
 // sines and cosines once and walks over the heads with them. Positions of long texts reach 10^5 and more, where a float
-// angle is off by 10^-2: the angle is formed in double and divided by 2 pi (for double results into an unevaluated sum of two
-// doubles), the whole part of these turns is dropped exactly, and only the rest, at most half a turn, is rounded to the
-// result's type for sincospi.
+// angle is off by 10^-2: for results of either type the angle is the product in double and sine and cosine are made in double,
+// whose reduction loses nothing however far the angle, and rounded to the result's type once, scale included.
 #include "common.h"
 #include "fastdiv.h"
 
@@ -30,20 +29,6 @@ template <typename T> struct Args {
   T scale, sign;
   int copy_rest;
 };
-
-__device__ __forceinline__ void sincos_turns(double turns, float& s, float& c) { sincospif((float)(2.0 * (turns - rint(turns))), &s, &c); }
-
-// sine and cosine of p * f
-__device__ __forceinline__ void sincos_at(double p, double f, float& s, float& c) {
-  sincos_turns(p * (f * 0.15915494309189535), s, c);
-}
-__device__ __forceinline__ void sincos_at(double p, double f, double& s, double& c) {
-  // the angle p * f as a double, as everyone else forms it; its turns with 1 / (2 pi) as the sum of two doubles, the product
-  // with the first one exactly through fma
-  const double inv_hi = 0.15915494309189535, inv_lo = -9.839338337591243e-18;
-  const double a = p * f, t = a * inv_hi, rest = fma(a, inv_hi, -t) + a * inv_lo;
-  sincospi(2.0 * ((t - rint(t)) + rest), &s, &c);
-}
 
 template <bool NT, typename V> __device__ __forceinline__ V fetch(const V* p) {
   if constexpr (NT) return __builtin_nontemporal_load(p);
@@ -81,10 +66,10 @@ __global__ __launch_bounds__(256) void rotate(Args<T> p) {
   T sn[P], cs[P];
 #pragma unroll
   for (int e = 0; e < P; ++e) {
-    T s, c;
-    sincos_at(pos, p.freq[u * P + e], s, c);
-    sn[e] = s * p.scale * p.sign;
-    cs[e] = c * p.scale;
+    double s, c;
+    sincos(pos * p.freq[u * P + e], &s, &c);
+    sn[e] = (T)(s * (double)p.scale * (double)p.sign);
+    cs[e] = (T)(c * (double)p.scale);
   }
   const int at = (int)u * V;
 #pragma unroll 4

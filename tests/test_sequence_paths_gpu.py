@@ -42,3 +42,22 @@ def test_a_single_tokens_stride_does_not_matter(hip, dk, dv, dt, stride):
                                                                *_rows(got[5])[:3]) == 0, last_error()
     for a, b in zip(got, want):
         assert np.array_equal(a.toCpu(), b.toCpu())
+
+
+@pytest.mark.parametrize("dt", ["f32", "f64"])
+def test_rotary_rounds_its_sines_once(hip, dt):
+    """Pairs (0, 1) give back the sines and cosines themselves, those next to 0 among them: as good relatively as a double sine,
+    then rounded to the result's type. The device's sine and cosine are good to 2 steps (4 u of a double), the product with the
+    scale to 1 u, NumPy's to 1 step (2 u)."""
+    T, n = 4096, 8
+    rng = np.random.default_rng(31)
+    pos = rng.integers(-10 ** 6, 10 ** 6, (1, T))
+    freq = rng.uniform(0.01, 1.0, n)
+    angle = pos.astype(np.float64)[..., None] * freq
+    assert (np.abs(np.sin(angle)) < 1e-3).sum() > 5 and (np.abs(np.cos(angle)) < 1e-3).sum() > 5
+    allowed = 7 * 2.0 ** -53 + (2.0 ** -24 if dt == "f32" else 0)
+    x = np.concatenate([np.zeros((1, T, 1, n)), np.ones((1, T, 1, n))], -1).astype(DTYPES[dt])
+    got = hip.rotary(hip.toHip(x), hip.toHip(pos), hip.toHip(freq)).toCpu()[:, :, 0].astype(np.float64)
+    for a, b in ((got[..., :n], -np.sin(angle)), (got[..., n:], np.cos(angle))):
+        off = np.abs(a - b) / np.abs(b)
+        assert off.max() <= allowed, f"{off.max() / allowed:.2f} times what is allowed"
