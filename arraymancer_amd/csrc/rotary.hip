@@ -27,7 +27,6 @@ template <typename T> struct Args {
   uint32_t turning;                              // units that turn, the others are copied
   int heads, heads_per_lane, half;               // half = rot_dim / 2
   T scale, sign;
-  int copy_rest;
 };
 
 template <bool NT, typename V> __device__ __forceinline__ V fetch(const V* p) {
