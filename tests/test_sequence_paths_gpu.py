@@ -61,3 +61,31 @@ def test_rotary_rounds_its_sines_once(hip, dt):
     for a, b in ((got[..., :n], -np.sin(angle)), (got[..., n:], np.cos(angle))):
         off = np.abs(a - b) / np.abs(b)
         assert off.max() <= allowed, f"{off.max() / allowed:.2f} times what is allowed"
+
+
+def slow_decays(tokens, count):
+    """float32 log decays near -10^-6 whose e^{g tokens} lies nearly half a step from the next float: rounded once and used again
+    and again it would pull to one side by about u / 2 every time."""
+    g = (-1e-6 * (1 + np.arange(20000) / 20000)).astype(np.float32)
+    e = np.exp(g.astype(np.float64) * tokens)
+    off = np.abs(e.astype(np.float32).astype(np.float64) - e)
+    return np.sort(g[off > 0.8 * 2.0 ** -25][:count])
+
+
+def walk(n):
+    """What n roundings of half a step at most, with no side, come to: six times their standard deviation, and 4 u for what follows."""
+    return (6 * np.sqrt(n / 3) + 4) * 2.0 ** -24
+
+
+def test_slow_decays_keep_a_prompts_state(hip):
+    """A state that only decays, over 1024 chunks in one walk (512 heads fill the device: no segments)."""
+    H, T, D = 512, 32768, 4
+    g = slow_decays(32, H)
+    assert len(g) == H
+    rng = np.random.default_rng(41)
+    s = (rng.uniform(0.5, 1, (1, H, D, D)) * rng.choice([-1, 1], (1, H, D, D))).astype(np.float32)
+    nothing = hip.zeros((1, 1, 1, D), np.float32).broadcast((1, T, H, D))
+    out, end = hip.decay_attention(nothing, nothing, nothing, hip.toHip(g), state=hip.toHip(s))
+    del out
+    want = s.astype(np.float64) * np.exp(g.astype(np.float64) * T)[None, :, None, None]
+    close(end.toCpu(), want, walk(T // 32) * np.abs(want), "state")
