@@ -6,6 +6,7 @@ of the absolute terms."""
 import numpy as np
 import pytest
 
+import sequence_closed as closed
 import sequence_reference as ref
 from arraymancer_amd._lib import last_error
 from arraymancer_amd.sequence_hip import _rows
@@ -89,3 +90,32 @@ def test_slow_decays_keep_a_prompts_state(hip):
     del out
     want = s.astype(np.float64) * np.exp(g.astype(np.float64) * T)[None, :, None, None]
     close(end.toCpu(), want, walk(T // 32) * np.abs(want), "state")
+
+
+# Which kernel takes a walk goes by its rows (up to 32, 64, 96, 128, 192, 256), its columns, the heads and tokens there are, and by
+# whether rows are whole vectors of 16 bytes; a walk of dk rows and dv columns goes with one of dv rows and dk columns in the backward
+# pass. Many heads, for workgroups of 128 columns (more than 64 columns, and work for every CU):
+MANY = [(4, 130, 32, 16, dk, dv) for dk, dv in ((32, 96), (64, 128), (96, 128), (192, 256), (30, 66), (62, 90), (94, 126), (190, 254), (128, 72), (126, 70),
+                                               (256, 192), (254, 190), (96, 32), (128, 64), (66, 30), (90, 62))]
+# and few, for those of 64 columns (whose rows two wavefronts share from 128 on), all in segments
+FEW = [(2, 197, 2, 1, dk, dv) for dk, dv in ((32, 64), (96, 40), (128, 64), (192, 60), (256, 24), (30, 62), (94, 34), (126, 62), (190, 54), (254, 22), (64, 32),
+                                            (40, 96), (64, 192), (24, 256), (62, 30), (34, 94), (62, 126), (54, 190), (22, 254))]
+# float64 has one form, of 64 columns
+DOUBLE = [(2, 197, 2, 1, dk, dv) for dk, dv in ((32, 64), (96, 128), (192, 256), (31, 63), (95, 127), (191, 255), (64, 32), (128, 96), (256, 192), (63, 31),
+                                               (127, 95), (255, 191))]
+
+
+@pytest.mark.parametrize("size,dt", [(s, "f32") for s in MANY + FEW] + [(s, "f64") for s in DOUBLE], ids=str)
+def test_every_kernel_of_decay_attention(hip, size, dt):
+    """Prompt and gradients through every chunk kernel, from a state and with one, sequences of all lengths."""
+    x = attention_inputs(hip, size, dt, seed_of("paths", size, dt))
+    x["lengths"][0], x["lengths"][-1] = size[1], size[1] // 2
+    d = {n: hip.toHip(a) for n, a in x.items() if n != "scale"}
+    kw = dict(lengths=x["lengths"], scale=x["scale"])
+    ab = {n: np.abs(a) for n, a in x.items() if n not in ("lengths", "scale", "g")}
+    got = hip.decay_attention(d["q"], d["k"], d["v"], d["g"], state=d["state"], lengths=d["lengths"], scale=x["scale"])
+    got += hip.decay_attention_backward(d["go"], d["q"], d["k"], d["v"], d["g"], state=d["state"], lengths=d["lengths"], scale=x["scale"], gradState=d["gs"])
+    want, bound = (closed.attention(a["q"], a["k"], a["v"], x["g"], a["state"], **kw) +
+                   closed.attention_backward(a["go"], a["q"], a["k"], a["v"], x["g"], a["state"], gs=a["gs"], **kw) for a in (x, ab))
+    for name, a, b, m in zip(("out", "state", "dq", "dk", "dv", "dstate"), got, want, bound):
+        close(a.toCpu(), b, roundings(size) * unit(DTYPES[dt]) * m, name)
