@@ -15,9 +15,9 @@
 //  - slabs, for the rest: a workgroup takes a slab of rows of one sample and reads them whole, channels next to each other, whatever the
 //    group's width; a lane owns V channels and keeps two sums for each. The slabs' sums per channel go to scratch memory
 //    and a small kernel folds them in a fixed order, per group (mean, rstd, or the two averages of the backward pass) and,
-//    backwards, per channel; then a second pass over the slabs writes the result. The sums of the forward pass are of
-//    x - pivot, with the group's first element as pivot, in double: no cancellation where the mean is large against the
-//    deviation.
+//    backwards, per channel; then a second pass over the slabs writes the result. The forward pass keeps means and squared
+//    deviations from them, in double, never sums of squares about a fixed point: nothing cancels where the mean is large
+//    against the deviation, or where single elements (an image's empty border) lie far from the rest.
 #include "common.h"
 #include "fastdiv.h"
 #include "scratch.h"
@@ -32,7 +32,7 @@ template <typename T> struct Args {
   T* y; int64_t y_n, y_s;            // forward: the result; backward: dx
   T* mean; T* rstd;                  // [batch, groups]
   T* dweight; T* dbias;
-  double* part;                      // slabs: [n][slab][channel][2]
+  double* part;                      // slabs: [n][slab][channel][2]: forward mean and squared deviations, backward sums of dz xhat and dz
   double* chan;                      // slabs, backward: [n][channel][2], null when no parameter's gradient is wanted
   T* share;                          // teams, backward: [slot][group][row][channel of the group][2] (workgroups: rows summed), null likewise
   T* coef;                           // backward: [n][group][2], the two averages
@@ -467,35 +467,62 @@ template <typename T, int V> __device__ __forceinline__ Place place(const Args<T
   return w;
 }
 
-// Per slab and channel: the sums of x - pivot and of its square; BWD: the sums of dz * xhat and dz.
+// Rows of a slab.
+template <typename T> __device__ __forceinline__ int64_t rows_of_slab(const Args<T>& p, int64_t slab) {
+  const int64_t left = p.spatial - slab * p.rows_per_slab;
+  return left < p.rows_per_slab ? left : p.rows_per_slab;
+}
+
+// Per slab and channel: the mean of x and its squared deviations from it; BWD: the sums of dz * xhat and dz.
+// Forwards a lane takes its rows in runs of 64: the sums of d = x - m and of d * d, m being its mean so far (of the first run: its
+// first element), then m <- m + sum d / n and squares <- squares + sum d^2 - (sum d)^2 / n with n the rows up to there. The subtraction
+// loses at most a factor of 64 in the first run, and of 2 later, however far the first element lies from the others; for double
+// images of 40000 elements around 1000 behind a first 0, sums about that 0 were off by 10^-11.
 template <typename T, int V, bool BWD, int ACT>
 __global__ __launch_bounds__(256) void slab_sums(Args<T> p) {
   typedef typename Vec<T, V>::type vec_t;
   __shared__ double lds[256 * V * 2];
   const Place w = place<T, V>(p, blockIdx.x);
-  double a[V], b[V];
+  double a[V], b[V], m[V], sq[V];
 #pragma unroll
-  for (int e = 0; e < V; ++e) a[e] = b[e] = 0.0;
+  for (int e = 0; e < V; ++e) a[e] = b[e] = m[e] = sq[e] = 0.0;
   const int64_t lo = (int64_t)w.slab * p.rows_per_slab;
-  const int64_t hi = lo + p.rows_per_slab < p.spatial ? lo + p.rows_per_slab : p.spatial;
+  const int64_t hi = lo + rows_of_slab(p, w.slab);
   if (w.live) {
-    T pivot[V], mean[V], rstd[V], wt[V], bs[V];
+    T mean[V], rstd[V], wt[V], bs[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const int g = (int)p.per_div.div((uint32_t)(w.c + e));
       if constexpr (BWD) {
+        const int g = (int)p.per_div.div((uint32_t)(w.c + e));
         wt[e] = p.weight ? p.weight[w.c + e] : (T)1;
         bs[e] = p.bias ? p.bias[w.c + e] : (T)0;
         mean[e] = p.mean[w.n * p.groups + g];
         rstd[e] = p.rstd[w.n * p.groups + g];
-      } else {
-        pivot[e] = p.x[w.n * p.x_n + (int64_t)g * p.per];
       }
     }
     const T* x = p.x + w.n * p.x_n + w.c;
     const T* dy = BWD ? p.dy + w.n * p.dy_n + w.c : nullptr;
     constexpr int R = 4;                         // rows on their way at once
-    int64_t s = lo + w.row0;
+    int64_t s = lo + w.row0, taken = 0, seen = 0;   // forwards: rows in the sums, and in the mean
+    if constexpr (!BWD) {
+      if (s < hi) {
+        const vec_t first = *(const vec_t*)(x + s * p.x_s);
+#pragma unroll
+        for (int e = 0; e < V; ++e) m[e] = (double)first[e];
+      }
+    }
+    auto settle = [&]() {
+      seen += taken;
+      taken = 0;
+      const double share = 1.0 / (double)seen;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const double t = a[e] * share;
+        sq[e] += b[e] - a[e] * t;
+        m[e] += t;
+        a[e] = b[e] = 0.0;
+      }
+    };
     for (; s + (R - 1) * p.rows_at_once < hi; s += R * p.rows_at_once) {
       vec_t xv[R], dv[R];
 #pragma unroll
@@ -519,11 +546,15 @@ __global__ __launch_bounds__(256) void slab_sums(Args<T> p) {
         } else {
 #pragma unroll
           for (int r = 0; r < R; ++r) {
-            const double d = (double)xv[r][e] - (double)pivot[e];
+            const double d = (double)xv[r][e] - m[e];
             a[e] += d;
             b[e] += d * d;
           }
         }
+      }
+      if constexpr (!BWD) {
+        taken += R;
+        if (taken == 64) settle();
       }
     }
     for (; s < hi; s += p.rows_at_once) {
@@ -538,35 +569,70 @@ __global__ __launch_bounds__(256) void slab_sums(Args<T> p) {
           a[e] += (double)(dz * h);
           b[e] += (double)dz;
         } else {
-          const double d = (double)xv[e] - (double)pivot[e];
+          const double d = (double)xv[e] - m[e];
           a[e] += d;
           b[e] += d * d;
         }
       }
+      if constexpr (!BWD) ++taken;
+    }
+    if constexpr (!BWD) {
+      if (taken) settle();
     }
   }
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    lds[(threadIdx.x * V + e) * 2] = a[e];
-    lds[(threadIdx.x * V + e) * 2 + 1] = b[e];
+    lds[(threadIdx.x * V + e) * 2] = BWD ? a[e] : m[e];
+    lds[(threadIdx.x * V + e) * 2 + 1] = BWD ? b[e] : sq[e];
   }
   __syncthreads();
   if (!w.live || w.row0 != 0) return;
   double* out = p.part + ((w.n * p.slabs + w.slab) * (int64_t)p.channels + w.c) * 2;
+  const int64_t rows = hi - lo;
+  const int lanes = rows < p.rows_at_once ? (int)rows : p.rows_at_once;   // lanes that have rows of this slab
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    for (int r = 1; r < p.rows_at_once; ++r) {
-      a[e] += lds[((threadIdx.x + r * p.lanes) * V + e) * 2];
-      b[e] += lds[((threadIdx.x + r * p.lanes) * V + e) * 2 + 1];
+    auto at = [&](int r) { return (threadIdx.x + r * p.lanes) * V + e; };
+    if constexpr (BWD) {
+      for (int r = 1; r < p.rows_at_once; ++r) {
+        a[e] += lds[at(r) * 2];
+        b[e] += lds[at(r) * 2 + 1];
+      }
+      out[2 * e] = a[e];
+      out[2 * e + 1] = b[e];
+    } else {
+      // the lanes' means and squares: the first (rows % rows_at_once) lanes have a row more than the others
+      const double few = (double)(rows / p.rows_at_once);
+      const int more = (int)(rows % p.rows_at_once);
+      double shift = 0.0;
+      for (int r = 1; r < lanes; ++r) shift += (few + (r < more ? 1.0 : 0.0)) * (lds[at(r) * 2] - m[e]);
+      const double all = m[e] + shift / (double)rows;
+      double squares = 0.0;
+      for (int r = 0; r < lanes; ++r) {
+        const double d = lds[at(r) * 2] - all;
+        squares += lds[at(r) * 2 + 1] + (few + (r < more ? 1.0 : 0.0)) * (d * d);
+      }
+      out[2 * e] = all;
+      out[2 * e + 1] = squares;
     }
-    out[2 * e] = a[e];
-    out[2 * e + 1] = b[e];
   }
 }
 
-// The slabs' sums of one group, in a fixed order: mean and rstd, or (BWD) the two averages of the backward pass and, where
-// they are wanted, each channel's sums over the sample. A lane stays with one channel (of up to 256 at a time) and takes
-// every so many-th slab.
+// The sum of `v` over the workgroup of 256, in a fixed order, the same in every lane.
+__device__ __forceinline__ Vec<double, 2>::type fold_256(Vec<double, 2>::type v, Vec<double, 2>::type (&lds)[256]) {
+  __syncthreads();
+  lds[threadIdx.x] = v;
+  __syncthreads();
+  for (int d = 128; d >= 1; d >>= 1) {
+    if ((int)threadIdx.x < d) lds[threadIdx.x] += lds[threadIdx.x + d];
+    __syncthreads();
+  }
+  return lds[0];
+}
+
+// The slabs of one group, in a fixed order. Forwards mean and rstd from the slabs' means and squares, in two passes over them (the
+// second one's reading is still in the die's L2); BWD the two averages of the backward pass and, where they are wanted, each channel's
+// sums over the sample. A lane stays with one channel (of up to 256 at a time) and takes every so many-th slab.
 template <typename T, bool BWD>
 __global__ __launch_bounds__(256) void group_fold(Args<T> p) {
   typedef Vec<double, 2>::type pair_t;
@@ -576,54 +642,51 @@ __global__ __launch_bounds__(256) void group_fold(Args<T> p) {
   const pair_t* part = (const pair_t*)p.part + n * p.slabs * (int64_t)p.channels + (int64_t)g * p.per;
   const int wide = p.per < 256 ? p.per : 256, rows = 256 / wide;
   const int k = (int)threadIdx.x / wide, cl = (int)threadIdx.x - k * wide;
-  pair_t all = (pair_t)(0.0);                              // lanes of row 0: their channels' sums
-  for (int c0 = 0; c0 < p.per; c0 += wide) {
-    const int c = c0 + cl;
-    const bool live = k < rows && c < p.per;
-    pair_t s = (pair_t)(0.0);
-    if (live) {
-      int i = k;
-      for (; i + 7 * rows < p.slabs; i += 8 * rows) {
-        pair_t v[8];
+  // take(pair, slab) for every slab of the lane's row in channel c
+  auto each = [&](int c, auto take) {
+    int i = k;
+    for (; i + 7 * rows < p.slabs; i += 8 * rows) {
+      pair_t v[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) v[u] = part[(int64_t)(i + u * rows) * p.channels + c];
+      for (int u = 0; u < 8; ++u) v[u] = part[(int64_t)(i + u * rows) * p.channels + c];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) s += v[u];
-      }
-      for (; i < p.slabs; i += rows) s += part[(int64_t)i * p.channels + c];
+      for (int u = 0; u < 8; ++u) take(v[u], i + u * rows);
     }
-    __syncthreads();
-    lds[threadIdx.x] = s;
-    __syncthreads();
-    if (live && k == 0) {
-      for (int r = 1; r < rows; ++r) s += lds[threadIdx.x + r * wide];
-      if constexpr (BWD) {
-        if (p.chan) ((pair_t*)p.chan)[n * p.channels + (int64_t)g * p.per + c] = s;
-        all += s * (p.weight ? (double)p.weight[g * p.per + c] : 1.0);
-      } else {
-        all += s;
-      }
-    }
-  }
-  __syncthreads();
-  lds[threadIdx.x] = all;
-  __syncthreads();
-  for (int d = 128; d >= 1; d >>= 1) {
-    if ((int)threadIdx.x < d) lds[threadIdx.x] += lds[threadIdx.x + d];
-    __syncthreads();
-  }
-  if (threadIdx.x) return;
-  all = lds[0];
+    for (; i < p.slabs; i += rows) take(part[(int64_t)i * p.channels + c], i);
+  };
   const double count = (double)p.spatial * (double)p.per;
   const int64_t at = n * p.groups + g;
   if constexpr (BWD) {
+    pair_t all = (pair_t)(0.0);                            // lanes of row 0: their channels' sums
+    for (int c0 = 0; c0 < p.per; c0 += wide) {
+      const int c = c0 + cl;
+      const bool live = k < rows && c < p.per;
+      pair_t s = (pair_t)(0.0);
+      if (live) each(c, [&](pair_t v, int) { s += v; });
+      __syncthreads();
+      lds[threadIdx.x] = s;
+      __syncthreads();
+      if (live && k == 0) {
+        for (int r = 1; r < rows; ++r) s += lds[threadIdx.x + r * wide];
+        if (p.chan) ((pair_t*)p.chan)[n * p.channels + (int64_t)g * p.per + c] = s;
+        all += s * (p.weight ? (double)p.weight[g * p.per + c] : 1.0);
+      }
+    }
+    all = fold_256(all, lds);
+    if (threadIdx.x) return;
     p.coef[2 * at] = (T)(all[1] / count);
     p.coef[2 * at + 1] = (T)(all[0] / count);
   } else {
-    const double m = all[0] / count;
-    double var = all[1] / count - m * m;
-    if (var < 0.0) var = 0.0;
-    p.mean[at] = (T)((double)p.x[n * p.x_n + (int64_t)g * p.per] + m);
+    const double pivot = part[0][0];
+    pair_t s = (pair_t)(0.0);
+    for (int c = cl; c < p.per && k < rows; c += wide) each(c, [&](pair_t v, int i) { s[0] += (double)rows_of_slab(p, i) * (v[0] - pivot); });
+    const double mean = pivot + fold_256(s, lds)[0] / count;
+    s = (pair_t)(0.0);
+    for (int c = cl; c < p.per && k < rows; c += wide)
+      each(c, [&](pair_t v, int i) { s[1] += v[1] + (double)rows_of_slab(p, i) * ((v[0] - mean) * (v[0] - mean)); });
+    const double var = fold_256(s, lds)[1] / count;
+    if (threadIdx.x) return;
+    p.mean[at] = (T)mean;
     p.rstd[at] = (T)(1.0 / sqrt(var + (double)p.eps));
   }
 }

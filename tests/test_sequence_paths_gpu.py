@@ -11,7 +11,7 @@ import sequence_reference as ref
 from arraymancer_amd._lib import last_error
 from arraymancer_amd.sequence_hip import _rows
 from conftest import DTYPES, seed_of
-from test_sequence_gpu import attention_inputs, close, roundings, unit
+from test_sequence_gpu import attention_inputs, close, norm_bounds, norm_inputs, roundings, unit
 
 pytestmark = pytest.mark.gpu
 
@@ -119,3 +119,23 @@ def test_every_kernel_of_decay_attention(hip, size, dt):
                    closed.attention_backward(a["go"], a["q"], a["k"], a["v"], x["g"], a["state"], gs=a["gs"], **kw) for a in (x, ab))
     for name, a, b, m in zip(("out", "state", "dq", "dk", "dv", "dstate"), got, want, bound):
         close(a.toCpu(), b, roundings(size) * unit(DTYPES[dt]) * m, name)
+
+
+# ---------------------------------------------------------------------- group norm's slabs
+@pytest.mark.parametrize("shape,groups", [((1, 40000, 2), 2), ((2, 4225, 24), 2), ((1, 70000, 3), 3)], ids=str)
+def test_slabs_whose_first_elements_lie_far_from_the_rest(hip, shape, groups):
+    """Elements around 1000 behind zeros, in the first row and at a few other places: in float64 the variance is as good as two passes
+    make it. The sums pass up to 600 roundings (a run, 256 lanes, 256 slabs a lane of the fold, its 8 folds); the subtraction of a run of 64 rows takes up to 64 times the three roundings of its
+    operands: (600 + 3 * 64) u for the variance, half of it for rstd."""
+    rng = np.random.default_rng(seed_of("pivot", shape))
+    x = 1000 + rng.normal(size=shape)
+    x[:, 0] = 0
+    x[:, 64::9973] = 0
+    x[:, 1::8192] = 2000
+    _, mean, rstd = hip.group_norm_forward(hip.toHip(x), None, None, groups, eps=0.0)
+    v = ref._grouped(x, groups).astype(np.longdouble)
+    m = v.mean((1, 3), keepdims=True)
+    want = 1 / np.sqrt(((v - m) ** 2).mean((1, 3)))
+    u = 2.0 ** -53
+    close(rstd.toCpu(), want.astype(np.float64), (600 + 3 * 64) / 2 * u * want.astype(np.float64), "rstd")
+    close(mean.toCpu(), m[:, 0, :, 0].astype(np.float64), 600 * u * np.abs(v).mean((1, 3)).astype(np.float64), "mean")
