@@ -122,6 +122,79 @@ def test_every_kernel_of_decay_attention(hip, size, dt):
 
 
 # ---------------------------------------------------------------------- group norm's slabs
+# Runs of memory too short for an image held in registers, or groups too large: whole rows of a slab, in vectors and singly.
+SLABS = [((2, 3000, 4), 4), ((1, 4225, 24), 2), ((2, 2100, 7), 7)]
+
+
+def chain(dt):
+    """The roundings that a slab's sums pass. They run in double: of a lane's run of 64 rows, of up to 256 lanes, of up to 256 slabs
+    a lane of the fold and of its 8 folds, 600 at most; in float only what follows them counts."""
+    return 600 if dt == "f64" else 64
+
+
+@pytest.mark.parametrize("dt", ["f32", "f64"])
+@pytest.mark.parametrize("shape,groups", SLABS, ids=str)
+def test_slabs_without_parameters_and_of_a_large_mean(hip, shape, groups, dt):
+    x, _, _, dy = norm_inputs(shape, dt, seed_of("slab mean", shape, dt), mean=300.0)
+    by, bdx, _, _ = norm_bounds(x, None, None, dy, groups, 1e-3, dt, chain(dt))
+    y, mean, rstd = hip.group_norm_forward(hip.toHip(x), None, None, groups, eps=1e-3)
+    close(y.toCpu(), ref.norm(x, None, None, groups, 1e-3), by, "y")
+    dx, dw, db = hip.group_norm_backward(hip.toHip(dy), hip.toHip(x), None, None, mean, rstd, groups)
+    assert dw is None and db is None
+    close(dx.toCpu(), ref.norm_backward(dy, x, None, None, groups, 1e-3)[0], bdx, "dx")
+
+
+@pytest.mark.parametrize("dt", ["f32", "f64"])
+@pytest.mark.parametrize("shape,groups", SLABS, ids=str)
+def test_slabs_far_out(hip, shape, groups, dt):
+    """Weights that take silu far beyond the range of e^z on both sides; only one of the parameters' gradients wanted."""
+    x, w, b, dy = norm_inputs(shape, dt, seed_of("slab far", shape, dt))
+    w *= DTYPES[dt](300)
+    bounds = norm_bounds(x, w, b, dy, groups, 1e-5, dt, chain(dt))
+    X, W, B, DY = (hip.toHip(a) for a in (x, w, b, dy))
+    y, mean, rstd = hip.group_norm_forward(X, W, B, groups, activation="silu")
+    with np.errstate(over="ignore"):
+        want = (ref.norm(x, w, b, groups, 1e-5, "silu"),) + ref.norm_backward(dy, x, w, b, groups, 1e-5, "silu")
+    for name, a, r, bound in zip(("y", "dx", "dweight", "dbias"), (y,) + hip.group_norm_backward(DY, X, W, B, mean, rstd, groups, activation="silu"), want, bounds):
+        close(a.toCpu(), r, bound, name)
+    y, mean, rstd = hip.group_norm_forward(X, W, None, groups)
+    dx, dw, db = hip.group_norm_backward(DY, X, W, None, mean, rstd, groups)
+    bounds = norm_bounds(x, w, None, dy, groups, 1e-5, dt, chain(dt))
+    want = ref.norm_backward(dy, x, w, None, groups, 1e-5)
+    assert db is None
+    close(y.toCpu(), ref.norm(x, w, None, groups, 1e-5), bounds[0], "y")
+    close(dx.toCpu(), want[0], bounds[1], "dx")
+    close(dw.toCpu(), want[1], bounds[2], "dweight")
+
+
+@pytest.mark.parametrize("dt", ["f32", "f64"])
+@pytest.mark.parametrize("shape,groups", SLABS + [((3, 130, 48), 3), ((5, 7, 60), 4), ((4, 20, 512), 1)], ids=str)
+def test_group_norm_of_rows_with_gaps(hip, shape, groups, dt):
+    """Rows that lie apart, on 16-byte boundaries and off them, for x, for the gradient and for both, through slabs, images, teams and
+    workgroups: nothing is copied first, and the result is that of packed operands up to the roundings of another order."""
+    from arraymancer_amd.sequence_hip import _channels_last
+    C = shape[-1]
+    x, w, b, dy = norm_inputs(shape, dt, seed_of("gaps", shape, dt))
+    W, B = hip.toHip(w), hip.toHip(b)
+
+    def apart(a, front):
+        wide = np.full(shape[:-1] + (C + 8,), 99, a.dtype)
+        wide[..., front:front + C] = a
+        t = hip.toHip(wide)[:, :, front:front + C]
+        assert _channels_last(t)[0] is t and t.strides[1] == C + 8
+        return t
+
+    X, DY = hip.toHip(x), hip.toHip(dy)
+    y, mean, rstd = hip.group_norm_forward(X, W, B, groups, activation="silu")
+    want = [t.toCpu().astype(np.float64) for t in (y,) + hip.group_norm_backward(DY, X, W, B, mean, rstd, groups, activation="silu")]
+    bounds = norm_bounds(x, w, b, dy, groups, 1e-5, dt, chain(dt))
+    for front in (4, 1):
+        for xs, ds in ((apart(x, front), DY), (X, apart(dy, front)), (apart(x, front), apart(dy, front))):
+            y, m, r = hip.group_norm_forward(xs, W, B, groups, activation="silu")
+            for a, c, t in zip((y,) + hip.group_norm_backward(ds, xs, W, B, m, r, groups, activation="silu"), want, bounds):
+                close(a.toCpu(), c, 2 * t, f"front {front}")
+
+
 @pytest.mark.parametrize("shape,groups", [((1, 40000, 2), 2), ((2, 4225, 24), 2), ((1, 70000, 3), 3)], ids=str)
 def test_slabs_whose_first_elements_lie_far_from_the_rest(hip, shape, groups):
     """Elements around 1000 behind zeros, in the first row and at a few other places: in float64 the variance is as good as two passes
