@@ -198,8 +198,8 @@ def test_group_norm_of_rows_with_gaps(hip, shape, groups, dt):
 @pytest.mark.parametrize("shape,groups", [((1, 40000, 2), 2), ((2, 4225, 24), 2), ((1, 70000, 3), 3)], ids=str)
 def test_slabs_whose_first_elements_lie_far_from_the_rest(hip, shape, groups):
     """Elements around 1000 behind zeros, in the first row and at a few other places: in float64 the variance is as good as two passes
-    make it. The sums pass up to 600 roundings (a run, 256 lanes, 256 slabs a lane of the fold, its 8 folds); the subtraction of a run of 64 rows takes up to 64 times the three roundings of its
-    operands: (600 + 3 * 64) u for the variance, half of it for rstd."""
+    make it. The sums pass up to 600 roundings (see `chain`); the subtraction of a run of 64 rows takes up to 64 times the three
+    roundings of its operands: (600 + 3 * 64) u for the variance, half of it for rstd."""
     rng = np.random.default_rng(seed_of("pivot", shape))
     x = 1000 + rng.normal(size=shape)
     x[:, 0] = 0
@@ -212,3 +212,75 @@ def test_slabs_whose_first_elements_lie_far_from_the_rest(hip, shape, groups):
     u = 2.0 ** -53
     close(rstd.toCpu(), want.astype(np.float64), (600 + 3 * 64) / 2 * u * want.astype(np.float64), "rstd")
     close(mean.toCpu(), m[:, 0, :, 0].astype(np.float64), 600 * u * np.abs(v).mean((1, 3)).astype(np.float64), "mean")
+
+
+# ---------------------------------------------------------------------- tensors larger than the caches keep
+@pytest.mark.parametrize("dt", ["f32", "f64"])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_rotary_past_the_caches(hip, dt, layout):
+    """40 MB (80 in float64), read past the caches, give the bits of their parts, which are not."""
+    B, T, H, D = 5, 997, 16, 128
+    rng = np.random.default_rng(seed_of("far rotary", dt, layout))
+    x, pos, freq = rng.normal(size=(B, T, H, D)).astype(DTYPES[dt]), rng.integers(0, 10 ** 5, (B, T)), hip.rotary_frequencies(96)
+    whole = hip.rotary(hip.toHip(x), hip.toHip(pos), freq, layout=layout, scale=1.1).toCpu()
+    for t in range(0, T, 250):
+        part = hip.rotary(hip.toHip(np.ascontiguousarray(x[:, t:t + 250])), hip.toHip(np.ascontiguousarray(pos[:, t:t + 250])), freq, layout=layout, scale=1.1)
+        assert np.array_equal(whole[:, t:t + 250], part.toCpu())
+
+
+@pytest.mark.parametrize("dt", ["f32", "f64"])
+def test_steps_past_the_caches(hip, dt):
+    """States of 40 MB and more, one step of all against the steps of parts."""
+    B, H, KH, D = 40, 16, 4, 128
+    rng = np.random.default_rng(seed_of("far step", dt))
+    mk = lambda *s: rng.normal(size=s).astype(DTYPES[dt])
+    q, k, v, s, g = mk(B, H, D), mk(B, KH, D), mk(B, KH, D), mk(B, H, D, D), hip.toHip((-1 / 2.0 ** np.arange(H)).astype(DTYPES[dt]))
+    state = hip.toHip(s)
+    out = hip.decay_attention_step(hip.toHip(q), hip.toHip(k), hip.toHip(v), g, state, scale=0.1).toCpu()
+    after = state.toCpu()
+    for b in range(0, B, 10):
+        part = hip.toHip(s[b:b + 10])
+        # (fewer heads take narrower columns, and add up the rows in another order)
+        got = hip.decay_attention_step(*(hip.toHip(a[b:b + 10]) for a in (q, k, v)), g, part, scale=0.1).toCpu()
+        assert np.array_equal(after[b:b + 10], part.toCpu())
+        bound = 0.1 * np.einsum("bhi,bhij->bhj", np.abs(q[b:b + 10]), np.abs(part.toCpu())).astype(np.float64)
+        close(got, out[b:b + 10].astype(np.float64), 2 * (D + 2) * unit(DTYPES[dt]) * bound, "out")
+
+
+@pytest.mark.parametrize("dt", ["f32", "f64"])
+@pytest.mark.parametrize("shape,groups,parts", [((4200, 2048), 16, 4), ((2400, 3, 1280), 2, 4), ((6, 1000, 1000, 4), 4, 6)], ids=str)
+def test_group_norm_past_the_caches(hip, shape, groups, parts, dt):
+    """Teams, workgroups and slabs over more than 32 MB against the same samples in parts that fit; forwards without the statistics
+    (which is what reads past the caches) and backwards. The parameters' gradients are added up from the parts'.
+    Both sides' mean is off by chain u avg|x| (at most 1.04 deviations here) and rstd by chain u, xhat by their sum; dz moves with
+    xhat by at most |dy w| / 2 times that, and is |dy| * 1.1 at most itself; a lane adds up 64 samples or 4 rows in the type."""
+    shape = (shape[0] // (DTYPES[dt](0).itemsize // 4),) + shape[1:]
+    parts = parts * 4 // DTYPES[dt](0).itemsize
+    rng = np.random.default_rng(seed_of("far norm", shape, dt))
+    C, T, u, n = shape[-1], DTYPES[dt], unit(DTYPES[dt]), chain(dt)
+    x, dy = rng.standard_normal(shape, dtype=T) * T(2) + T(0.5), rng.standard_normal(shape, dtype=T)
+    w, b = rng.standard_normal(C, dtype=T), rng.standard_normal(C, dtype=T)
+    X, DY, W, B = (hip.toHip(a) for a in (x, dy, w, b))
+    assert x.nbytes > 32 * 2 ** 20 >= x.nbytes // parts
+    y = hip.group_norm(X, W, B, groups, activation="silu").toCpu()
+    y2, mean, rstd = hip.group_norm_forward(X, W, B, groups, activation="silu")
+    assert np.array_equal(y, y2.toCpu())
+    dx, dw, db = (t.toCpu() for t in hip.group_norm_backward(DY, X, W, B, mean, rstd, groups, activation="silu"))
+    sums, allowed = np.zeros((2, C)), np.zeros((2, C))
+    for at in np.array_split(np.arange(shape[0]), parts):
+        at = slice(at[0], at[-1] + 1)
+        xp, dp = hip.toHip(x[at]), hip.toHip(dy[at])
+        yp, m, r = hip.group_norm_forward(xp, W, B, groups, activation="silu")
+        dxp, *grads = hip.group_norm_backward(dp, xp, W, B, m, r, groups, activation="silu")
+        if at.stop == shape[0]:
+            by, bdx, _, _ = norm_bounds(x[at], w, b, dy[at], groups, 1e-5, dt, n)
+            close(yp.toCpu(), y[at].astype(np.float64), 2 * by, "y")
+            close(dxp.toCpu(), dx[at].astype(np.float64), 2 * bdx, "dx")
+        sums += [t.toCpu().astype(np.float64) for t in grads]
+        xhat = (x[at].reshape(x[at].shape[0], -1, groups, C // groups) - m.toCpu()[:, None, :, None]) * r.toCpu()[:, None, :, None]
+        h, d = np.abs(xhat).reshape(-1, C), np.abs(dy[at]).reshape(-1, C)
+        off, wa = 2 * n * u * (h + T(1.04)), np.abs(w)
+        allowed[0] += (d * (off * (1.1 + 0.5 * wa * h) + 128 * u * 1.1 * h)).sum(0, dtype=np.float64)
+        allowed[1] += (d * (off * 0.5 * wa + 128 * u * 1.1)).sum(0, dtype=np.float64)
+    close(dw, sums[0], allowed[0], "dweight")
+    close(db, sums[1], allowed[1], "dbias")
