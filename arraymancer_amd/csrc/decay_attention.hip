@@ -1197,10 +1197,10 @@ static int forward(const char* fn, int64_t batch, int64_t tokens, int64_t heads,
 
 // out[b, t, head, :] = the sum of the `group` heads' shares that follow each other, in the heads' order
 template <typename T, int V>
-__global__ __launch_bounds__(256) void fold(const T* shares, Result<T> out, int64_t rows, int tokens, int kv_heads, int group, int d) {
+__global__ __launch_bounds__(256) void fold(const T* shares, Result<T> out, int64_t first, int64_t rows, int tokens, int kv_heads, int group, int d) {
   typedef T vec_t __attribute__((ext_vector_type(V)));
   const int per = d / V;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t i = (first + blockIdx.x) * 256 + threadIdx.x;
   const int64_t row = i / per;                             // (batch, token, head)
   if (row >= rows) return;
   const int c = (int)(i - row * per) * V;
@@ -1218,10 +1218,15 @@ static int fold_heads(const T* shares, const Result<T>& out, int64_t batch, int6
   if (rows == 0) return AM_OK;
   const bool vec = d % W == 0 && (uintptr_t)out.p % 16 == 0 && out.b % W == 0 && out.t % W == 0 && out.h % W == 0;
   const int64_t wgs = (rows * (vec ? d / W : d) + 255) / 256;
-  if (wgs >= ((int64_t)1 << 31) || tokens >= ((int64_t)1 << 31)) return fail(AM_E_SHAPE, "decay attention: too many tokens for shared heads");
-  if (vec) hipLaunchKernelGGL((fold<T, W>), dim3((unsigned)wgs), dim3(256), 0, stream(), shares, out, rows, (int)tokens, (int)kv_heads, group, d);
-  else hipLaunchKernelGGL((fold<T, 1>), dim3((unsigned)wgs), dim3(256), 0, stream(), shares, out, rows, (int)tokens, (int)kv_heads, group, d);
-  return check_launch("fold");
+  if (tokens >= ((int64_t)1 << 31)) return fail(AM_E_SHAPE, "decay attention: too many tokens for shared heads");
+  constexpr int64_t kLaunch = (int64_t)1 << 16;             // workgroups: a launch has less than 2^32 threads
+  for (int64_t first = 0; first < wgs; first += kLaunch) {
+    const dim3 grid((unsigned)(wgs - first < kLaunch ? wgs - first : kLaunch)), block(256);
+    if (vec) hipLaunchKernelGGL((fold<T, W>), grid, block, 0, stream(), shares, out, first, rows, (int)tokens, (int)kv_heads, group, d);
+    else hipLaunchKernelGGL((fold<T, 1>), grid, block, 0, stream(), shares, out, first, rows, (int)tokens, (int)kv_heads, group, d);
+    AM_TRY(check_launch("fold"));
+  }
+  return AM_OK;
 }
 
 template <typename T>

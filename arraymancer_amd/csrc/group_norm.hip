@@ -852,6 +852,17 @@ static int fold_samples(const Args<T>& p, const P* part, int64_t samples, bool a
   } while (0)
 
 constexpr size_t kMostScratch = (size_t)256 << 20;
+constexpr int64_t kMostThreads = ((int64_t)1 << 32) - 1;     // of a launch
+
+// Samples of a slab launch: as many as the scratch memory and a launch hold (beside the workgroups that fold up to 2^24 channels).
+template <typename T> static int64_t samples_at_once(const Args<T>& p, size_t per_sample) {
+  const int64_t wgs = (int64_t)p.slabs * p.tiles > p.groups ? (int64_t)p.slabs * p.tiles : p.groups;
+  int64_t nc = (int64_t)(kMostScratch / per_sample);
+  const int64_t launch = (kMostThreads / 256 - ((int64_t)1 << 21)) / wgs;
+  if (nc > launch) nc = launch;
+  if (nc < 1) nc = 1;
+  return nc < p.batch ? nc : p.batch;
+}
 
 template <typename T> static bool fits(const void* base, int64_t sn, int64_t ss, int64_t batch, int64_t spatial) {
   constexpr int64_t W = 16 / (int64_t)sizeof(T);
@@ -898,7 +909,7 @@ static int team_pass(Args<T> p, int lanes, int units) {
   const int64_t each = (p.batch + slots - 1) / slots;
   slots = (p.batch + each - 1) / each;
   const int64_t wgs = (slots * p.groups + at_once - 1) / at_once;
-  if (wgs >= ((int64_t)1 << 31)) return fail(AM_E_SHAPE, "group norm: too many groups for one launch");
+  if (wgs > kMostThreads / 256) return fail(AM_E_SHAPE, "group norm: too many groups for one launch");
   const int64_t rows = lanes == 256 ? 1 : p.spatial;      // of a slot's shares
   Scratch share;
   if (BWD && (p.dweight || p.dbias)) {
@@ -952,11 +963,21 @@ static int image_pass(Args<T> p, int lanes) {
     AM_TRY(share.take((size_t)p.batch * p.channels * 2 * sizeof(T)));
     p.share = (T*)share.p;
   }
-  if (lanes == 256 && p.spatial <= (int64_t)p.rows_at_once * (U / 2)) launch_image<T, 256, V, U / 2, ACT, BWD>(p);
-  else if (lanes == 256) launch_image<T, 256, V, U, ACT, BWD>(p);
-  else if (lanes == 512) launch_image<T, 512, V, U, ACT, BWD>(p);
-  else launch_image<T, 1024, V, U, ACT, BWD>(p);
-  AM_TRY(check_launch("group norm of images"));
+  const int64_t most = (kMostThreads / lanes - 8) / p.groups;    // samples of a launch
+  for (int64_t n = 0; n < p.batch; n += most) {
+    Args<T> q = p;
+    q.batch = p.batch - n < most ? p.batch - n : most;
+    q.x += n * p.x_n;
+    q.y += n * p.y_n;
+    if (BWD) q.dy += n * p.dy_n;
+    if (p.mean) { q.mean += n * p.groups; q.rstd += n * p.groups; }
+    if (p.share) q.share += n * p.channels * 2;
+    if (lanes == 256 && p.spatial <= (int64_t)p.rows_at_once * (U / 2)) launch_image<T, 256, V, U / 2, ACT, BWD>(q);
+    else if (lanes == 256) launch_image<T, 256, V, U, ACT, BWD>(q);
+    else if (lanes == 512) launch_image<T, 512, V, U, ACT, BWD>(q);
+    else launch_image<T, 1024, V, U, ACT, BWD>(q);
+    AM_TRY(check_launch("group norm of images"));
+  }
   return p.share ? fold_samples<T, T>(p, p.share, p.batch, false) : AM_OK;
 }
 
@@ -979,7 +1000,6 @@ static int try_images(Args<T>& p, bool aligned, bool& taken) {
   if (p.spatial < 128 || run < 16) return AM_OK;
   const bool slabs = p.spatial * (p.per / (aligned && p.per % W == 0 ? W : 1)) > 256 * kUnits;
   if (slabs && run < 48 && (double)p.batch * (double)p.spatial * p.channels * sizeof(T) > 48e6) return AM_OK;
-  if (p.batch * p.groups >= ((int64_t)1 << 31) - 8) return AM_OK;
   int V = 16 / (int)sizeof(T);
   // rows one behind the other, and all that the lanes may count up to within 2^31 bytes
   constexpr int64_t most = ((int64_t)1 << 31) / ((kImageHeld<T> + 1) * kImage * (int)sizeof(T));
@@ -993,7 +1013,7 @@ static int try_images(Args<T>& p, bool aligned, bool& taken) {
   const int64_t upr = p.per / V;
   int lanes = 256;
   while (lanes <= kImage && (upr > lanes || (p.spatial + lanes / upr - 1) / (lanes / upr) * V > kImageHeld<T>)) lanes *= 2;
-  if (lanes > kImage) return AM_OK;
+  if (lanes > kImage || p.groups > kMostThreads / lanes - 8) return AM_OK;
   taken = true;
   p.units_div = FastDiv((uint32_t)upr);
   p.rows_at_once = (int)(lanes / upr);
@@ -1025,9 +1045,7 @@ static int forward(Args<T> p) {
   T* const rstd = p.rstd;
   set_slabs(p, V, p.spatial, p.batch);
   const size_t per_sample = (size_t)p.slabs * p.channels * 2 * sizeof(double);
-  int64_t nc = (int64_t)(kMostScratch / per_sample);
-  if (nc < 1) nc = 1;
-  if (nc > p.batch) nc = p.batch;
+  const int64_t nc = samples_at_once(p, per_sample);
   Scratch part;
   AM_TRY(part.take(per_sample * (size_t)nc));
   p.part = (double*)part.p;
@@ -1070,9 +1088,7 @@ static int backward(Args<T> p) {
   Scratch part;
   set_slabs(p, V, p.spatial, p.batch);
   const size_t per_sample = (size_t)p.slabs * p.channels * 2 * sizeof(double);
-  int64_t nc = (int64_t)(kMostScratch / per_sample);
-  if (nc < 1) nc = 1;
-  if (nc > p.batch) nc = p.batch;
+  const int64_t nc = samples_at_once(p, per_sample);
   const size_t coef_bytes = (size_t)nc * p.groups * 2 * sizeof(T);
   const size_t part_bytes = per_sample * (size_t)nc, chan_bytes = params ? (size_t)nc * p.channels * 2 * sizeof(double) : 0;
   AM_TRY(part.take(part_bytes + chan_bytes + coef_bytes));

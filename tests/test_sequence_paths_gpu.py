@@ -284,3 +284,43 @@ def test_group_norm_past_the_caches(hip, shape, groups, parts, dt):
         allowed[1] += (d * (off * 0.5 * wa + 128 * u * 1.1)).sum(0, dtype=np.float64)
     close(dw, sums[0], allowed[0], "dweight")
     close(db, sums[1], allowed[1], "dbias")
+
+
+# ---------------------------------------------------------------------- more than a launch holds
+def test_group_norm_of_more_images_than_a_launch_holds(hip):
+    """2^24 groups of 256 lanes each are 2^32 threads, which no launch may have: 2^18 samples of 64 groups, every one the same memory
+    (the result has 34 GB). Forwards and backwards the first and the last are those of a single sample."""
+    B, S, C, G = 2 ** 18, 128, 256, 64
+    rng = np.random.default_rng(61)
+    one = [hip.toHip(rng.standard_normal((1, S, C), dtype=np.float32)) for _ in range(2)]
+    w = hip.toHip(rng.standard_normal(C, dtype=np.float32))
+    x, dy = (t.broadcast((B, S, C)) for t in one)
+    want = hip.group_norm_forward(one[0], w, w, G, activation="silu")
+    y, mean, rstd = hip.group_norm_forward(x, w, w, G, activation="silu")
+    for at in (slice(0, 1), slice(B - 1, B), slice(B // 2, B // 2 + 1)):
+        assert np.array_equal(y[at].toCpu(), want[0].toCpu())
+    assert (mean.toCpu() == want[1].toCpu()).all() and (rstd.toCpu() == want[2].toCpu()).all()
+    del y
+    grads = hip.group_norm_backward(one[1], one[0], w, w, *want[1:], G, activation="silu")
+    dx, dw, db = hip.group_norm_backward(dy, x, w, w, mean, rstd, G, activation="silu")
+    for at in (slice(0, 1), slice(B - 1, B), slice(B // 2, B // 2 + 1)):
+        assert np.array_equal(dx[at].toCpu(), grads[0].toCpu())
+    # 2^18 equal numbers are added in double: only the results are rounded, and the one sample's
+    for a, b in ((dw, grads[1]), (db, grads[2])):
+        assert (np.abs(a.toCpu() - B * b.toCpu().astype(np.float64)) <= 2 * 2.0 ** -24 * B * np.abs(b.toCpu())).all()
+
+
+def test_shared_heads_are_added_up_over_several_launches(hip):
+    """More gradients of keys than 2^16 workgroups take: with every head's own copy of keys and values, added up afterwards in the
+    heads' order, the bits are the same."""
+    B, T, H, dk, dv = 2, 140_000, 2, 65, 4
+    assert B * T * dk > 2 ** 16 * 256
+    rng = np.random.default_rng(62)
+    mk = lambda *s: hip.toHip(rng.standard_normal(s, dtype=np.float32))
+    q, k, v, go = mk(B, T, H, dk), mk(B, T, 1, dk), mk(B, T, 1, dv), mk(B, T, H, dv)
+    g = hip.toHip(np.array([-0.5, -0.01], np.float32))
+    _, dkey, dval, _ = hip.decay_attention_backward(go, q, k, v, g)
+    _, keys, vals, _ = hip.decay_attention_backward(go, q, k.broadcast((B, T, H, dk)), v.broadcast((B, T, H, dv)), g)
+    for a, b in ((dkey, keys), (dval, vals)):
+        b = b.toCpu()
+        assert np.array_equal(a.toCpu()[:, :, 0], b[:, :, 0] + b[:, :, 1])
