@@ -694,16 +694,26 @@ proc decay_attention_backward*[T: float32 | float64](grad_output, q, k, v, log_d
   when T is float32: call am_hip_decay_attention_backward_f32
   else: call am_hip_decay_attention_backward_f64
 
-proc checkNorm[T](x, weight, bias: HipTensor[T]) =
+proc checkNorm[T](x, weight, bias: HipTensor[T], groups: int) =
   if x.rank < 2 or not x.is_C_contiguous: raise newException(ValueError, "group_norm: a contiguous [batch, ..., channels] is needed")
   let C = x.shape[x.rank - 1]
   if weight.size != C or bias.size != C or not weight.is_C_contiguous or not bias.is_C_contiguous:
     raise newException(ValueError, "group_norm: weight and bias must be [channels]")
+  if groups < 1 or C mod groups != 0:
+    raise newException(ValueError, "group_norm: " & $C & " channels cannot form " & $groups & " groups")
+
+proc checkNormGradients[T](grad_output, x, mean, rstd: HipTensor[T], groups: int) =
+  if grad_output.shape != x.shape or not grad_output.is_C_contiguous:
+    raise newException(ValueError, "group_norm_backward: the output's gradient must be contiguous and have x's shape")
+  if mean.rank != 2 or mean.shape[0] != x.shape[0] or mean.shape[1] != groups or not mean.is_C_contiguous:
+    raise newException(ValueError, "group_norm_backward: mean must be the contiguous [batch, groups] of group_norm")
+  if rstd.shape != mean.shape or not rstd.is_C_contiguous:
+    raise newException(ValueError, "group_norm_backward: rstd must be the contiguous [batch, groups] of group_norm")
 
 proc group_norm*[T: float32 | float64](x, weight, bias: HipTensor[T], groups: int, eps: T = 1e-5, activation = AM_ACT_NONE):
     tuple[y, mean, rstd: HipTensor[T]] =
   ## act((x - mean) / sqrt(variance + eps) * weight + bias) of a channels-last [batch, ..., channels], with what the backward pass needs.
-  checkNorm(x, weight, bias)
+  checkNorm(x, weight, bias, groups)
   let (N, C) = (x.shape[0], x.shape[x.rank - 1])
   let S = if N * C == 0: 0 else: x.size div (N * C)
   result = (newHipTensor[T](x.shape.toSeq), newHipTensor[T]([N, groups]), newHipTensor[T]([N, groups]))
@@ -716,8 +726,8 @@ proc group_norm*[T: float32 | float64](x, weight, bias: HipTensor[T], groups: in
 proc group_norm_backward*[T: float32 | float64](grad_output, x, weight, bias, mean, rstd: HipTensor[T], groups: int, activation = AM_ACT_NONE):
     tuple[dx, dweight, dbias: HipTensor[T]] =
   ## The gradients of `group_norm`.
-  checkNorm(x, weight, bias)
-  if grad_output.size != x.size or not grad_output.is_C_contiguous: raise newException(ValueError, "group_norm_backward: the output's gradient must be contiguous and have x's shape")
+  checkNorm(x, weight, bias, groups)
+  checkNormGradients(grad_output, x, mean, rstd, groups)
   let (N, C) = (x.shape[0], x.shape[x.rank - 1])
   let S = if N * C == 0: 0 else: x.size div (N * C)
   result = (newHipTensor[T](x.shape.toSeq), newHipTensor[T](weight.shape.toSeq), newHipTensor[T](bias.shape.toSeq))

@@ -53,3 +53,24 @@ def test_nothing_is_called_by_a_keyword(name):
 def test_the_check_sees_parameters_variables_and_fields():
     seen = declared("proc f*(a, out: ptr cfloat; b: int): tuple[x, end: int] = discard\nlet (of, c) = g()\nconst\n  mod* = 1\n# var is: int\n")
     assert {"f", "a", "out", "b", "x", "end", "of", "c", "mod"} <= set(seen) and "is" not in seen
+
+
+def body(name):
+    """The text of one proc of nim/tensor_hip.nim."""
+    with open(os.path.join(ROOT, "nim", "tensor_hip.nim")) as f:
+        text = f.read()
+    found = re.search(rf"^proc {name}\*?\[.*?(?=^(?:proc|template|type|#) ?)", text, flags=re.M | re.S)
+    assert found, name
+    return found.group(0)
+
+
+def test_the_statistics_of_group_norm_are_looked_at_before_they_are_read():
+    """mean, rstd and the gradient go to the device as bare pointers: their shapes and their order in memory are checked first."""
+    calls = body("group_norm_backward")
+    check = calls.index("checkNormGradients(grad_output, x, mean, rstd, groups)")
+    assert check < calls.index("mean.get_offset_ptr") and check < calls.index("newHipTensor")
+    checks = body("checkNormGradients")
+    for what in ("grad_output.shape != x.shape", "mean.rank != 2", "mean.shape[0] != x.shape[0]", "mean.shape[1] != groups", "rstd.shape != mean.shape"):
+        assert what in checks
+    for t in ("grad_output", "mean", "rstd"):
+        assert f"not {t}.is_C_contiguous" in checks
