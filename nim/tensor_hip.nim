@@ -601,27 +601,38 @@ proc gru_cell_forward*[T: float32 | float64](input, W3, U3, bW3, bU3: HipTensor[
   else: call am_hip_gru_gates_f64
 
 # ---------------------------------------------------------------- sequence mixing (no counterpart in the reference)
+# A tensor that may be left out is given as `default(HipTensor[T])`, whose rank is 0.
+proc given[T](t: HipTensor[T]): bool = t.rank > 0
+
+proc ptrOrNil[T](t: HipTensor[T]): ptr T =
+  if t.given: t.get_offset_ptr else: nil
+
+proc strideOr0[T](t: HipTensor[T], dim: int): int64 =
+  if t.given: int64 t.strides[dim] else: 0'i64
+
 proc hipRows[T](t: HipTensor[T]): HipTensor[T] =
   ## `t`, or a copy of it, with unit stride in the last dimension.
   if t.strides[t.rank - 1] == 1 or t.shape[t.rank - 1] == 1: t else: t.clone()
 
 proc rotate[T: float32 | float64](x: HipTensor[T], positions: HipTensor[int64], frequencies: HipTensor[float64], layout: cint, scale: T, inverse: cint): HipTensor[T] =
-  if x.rank != 4 or positions.rank != 2 or positions.shape[0] != x.shape[0] or positions.shape[1] != x.shape[1]:
-    raise newException(ValueError, "rotary: x must be [batch, tokens, heads, dim] and positions [batch, tokens]")
+  if x.rank != 4: raise newException(ValueError, "rotary: x must be [batch, tokens, heads, dim]")
+  if positions.given and (positions.rank != 2 or positions.shape[0] != x.shape[0] or positions.shape[1] != x.shape[1]):
+    raise newException(ValueError, "rotary: positions must be [batch, tokens]")
   if frequencies.rank != 1 or not frequencies.is_C_contiguous or 2 * frequencies.shape[0] > x.shape[3]:
     raise newException(ValueError, "rotary: frequencies must be a contiguous vector of at most dim / 2 values")
   let src = x.hipRows
   result = newHipTensor[T](x.shape.toSeq)
   template call(f: untyped) =
     check f(int64 x.shape[0], int64 x.shape[1], int64 x.shape[2], int64 x.shape[3], int64(2 * frequencies.shape[0]), layout, inverse, scale,
-            positions.get_offset_ptr, int64 positions.strides[0], int64 positions.strides[1], frequencies.get_offset_ptr,
+            positions.ptrOrNil, positions.strideOr0(0), positions.strideOr0(1), frequencies.get_offset_ptr,
             src.get_offset_ptr, int64 src.strides[0], int64 src.strides[1], int64 src.strides[2],
             result.get_offset_ptr, int64 result.strides[0], int64 result.strides[1], int64 result.strides[2])
   when T is float32: call am_hip_rotary_f32
   else: call am_hip_rotary_f64
 
 proc rotary*[T: float32 | float64](x: HipTensor[T], positions: HipTensor[int64], frequencies: HipTensor[float64], layout = AM_ROTARY_HALF, scale: T = 1): HipTensor[T] =
-  ## The pairs of every head of x [batch, tokens, heads, dim] turned by position * frequency.
+  ## The pairs of every head of x [batch, tokens, heads, dim] turned by position * frequency; positions may be left out for the
+  ## token's index.
   rotate(x, positions, frequencies, layout, scale, 0)
 
 proc rotary_backward*[T: float32 | float64](gradient: HipTensor[T], positions: HipTensor[int64], frequencies: HipTensor[float64], layout = AM_ROTARY_HALF, scale: T = 1): HipTensor[T] =
@@ -637,21 +648,31 @@ proc checkAttention[T](q, k, v, log_decay, state: HipTensor[T], lead: int) =
     raise newException(ValueError, "decay_attention: q and k must share dk, k and v their heads")
   if log_decay.rank != 1 or log_decay.shape[0] != q.shape[lead] or not log_decay.is_C_contiguous:
     raise newException(ValueError, "decay_attention: log_decay must be [heads]")
-  if state.rank != 4 or state.shape[0] != q.shape[0] or state.shape[1] != q.shape[lead] or state.shape[2] != q.shape[lead + 1] or
-     state.shape[3] != v.shape[lead + 1] or not state.is_C_contiguous:
+  if state.given and (state.rank != 4 or state.shape[0] != q.shape[0] or state.shape[1] != q.shape[lead] or state.shape[2] != q.shape[lead + 1] or
+     state.shape[3] != v.shape[lead + 1] or not state.is_C_contiguous):
     raise newException(ValueError, "decay_attention: the state must be a contiguous [batch, heads, dk, dv]")
 
-proc decay_attention*[T: float32 | float64](q, k, v, log_decay: HipTensor[T], state: var HipTensor[T], scale: T = 1): HipTensor[T] =
-  ## Linear attention with a decay for each head over whole sequences; `state` is carried on in place.
+proc checkLengths(lengths: HipTensor[int64], batch: int) =
+  if lengths.given and (lengths.rank != 1 or lengths.shape[0] != batch or not lengths.is_C_contiguous):
+    raise newException(ValueError, "decay_attention: lengths must be [batch]")
+
+proc decay_attention*[T: float32 | float64](q, k, v, log_decay: HipTensor[T], state: var HipTensor[T], scale: T = 1,
+                                            lengths = default(HipTensor[int64])): HipTensor[T] =
+  ## Linear attention with a decay for each head over whole sequences; `state` is carried on in place, or begins with zeros
+  ## where it is `default(HipTensor[T])` and receives the last state then. lengths [batch]: the tokens of each sequence, behind
+  ## which the result is 0; left out: all of them.
   checkAttention(q, k, v, log_decay, state, 2)
+  checkLengths(lengths, q.shape[0])
   let (qq, kk, vv) = (q.hipRows, k.hipRows, v.hipRows)
   result = newHipTensor[T]([q.shape[0], q.shape[1], q.shape[2], v.shape[3]])
+  let first = state
+  if not state.given: state = newHipTensor[T]([q.shape[0], q.shape[2], q.shape[3], v.shape[3]])
   template call(f: untyped) =
     check f(int64 q.shape[0], int64 q.shape[1], int64 q.shape[2], int64 k.shape[2], int64 q.shape[3], int64 v.shape[3], scale,
-            log_decay.get_offset_ptr, nil, qq.get_offset_ptr, int64 qq.strides[0], int64 qq.strides[1], int64 qq.strides[2],
+            log_decay.get_offset_ptr, lengths.ptrOrNil, qq.get_offset_ptr, int64 qq.strides[0], int64 qq.strides[1], int64 qq.strides[2],
             kk.get_offset_ptr, int64 kk.strides[0], int64 kk.strides[1], int64 kk.strides[2],
             vv.get_offset_ptr, int64 vv.strides[0], int64 vv.strides[1], int64 vv.strides[2],
-            state.get_offset_ptr, int64 state.strides[0], int64 state.strides[1],
+            first.ptrOrNil, first.strideOr0(0), first.strideOr0(1),
             result.get_offset_ptr, int64 result.strides[0], int64 result.strides[1], int64 result.strides[2],
             state.get_offset_ptr, int64 state.strides[0], int64 state.strides[1])
   when T is float32: call am_hip_decay_attention_f32
@@ -659,6 +680,7 @@ proc decay_attention*[T: float32 | float64](q, k, v, log_decay: HipTensor[T], st
 
 proc decay_attention_step*[T: float32 | float64](q, k, v, log_decay: HipTensor[T], state: var HipTensor[T], scale: T = 1): HipTensor[T] =
   ## One new token of every sequence: q [batch, heads, dk], k [batch, kv_heads, dk], v [batch, kv_heads, dv].
+  if not state.given: raise newException(ValueError, "decay_attention_step: a state is needed")
   checkAttention(q, k, v, log_decay, state, 1)
   let (qq, kk, vv) = (q.hipRows, k.hipRows, v.hipRows)
   result = newHipTensor[T]([q.shape[0], q.shape[1], v.shape[2]])
@@ -670,37 +692,43 @@ proc decay_attention_step*[T: float32 | float64](q, k, v, log_decay: HipTensor[T
   when T is float32: call am_hip_decay_attention_step_f32
   else: call am_hip_decay_attention_step_f64
 
-proc decay_attention_backward*[T: float32 | float64](grad_output, q, k, v, log_decay, state: HipTensor[T], grad_state: HipTensor[T], scale: T = 1):
-    tuple[dq, dk, dv, dstate: HipTensor[T]] =
-  ## The gradients of `decay_attention` from those of its output and of the state it left; `state` is the one it began with.
+proc decay_attention_backward*[T: float32 | float64](grad_output, q, k, v, log_decay, state: HipTensor[T], grad_state: HipTensor[T], scale: T = 1,
+                                                     lengths = default(HipTensor[int64])): tuple[dq, dk, dv, dstate: HipTensor[T]] =
+  ## The gradients of `decay_attention` from those of its output and of the state it left; `state` is the one it began with. Either
+  ## state may be left out for zeros; without `state`, dstate is `default(HipTensor[T])`.
   checkAttention(q, k, v, log_decay, state, 2)
   checkAttention(q, k, v, log_decay, grad_state, 2)
+  checkLengths(lengths, q.shape[0])
   if grad_output.rank != 4 or grad_output.shape[0] != q.shape[0] or grad_output.shape[1] != q.shape[1] or grad_output.shape[2] != q.shape[2] or
      grad_output.shape[3] != v.shape[3]: raise newException(ValueError, "decay_attention_backward: the output's gradient must be [batch, tokens, heads, dv]")
   let (go, qq, kk, vv) = (grad_output.hipRows, q.hipRows, k.hipRows, v.hipRows)
-  result = (newHipTensor[T](q.shape.toSeq), newHipTensor[T](k.shape.toSeq), newHipTensor[T](v.shape.toSeq), newHipTensor[T](state.shape.toSeq))
+  result = (newHipTensor[T](q.shape.toSeq), newHipTensor[T](k.shape.toSeq), newHipTensor[T](v.shape.toSeq), default(HipTensor[T]))
+  if state.given: result.dstate = newHipTensor[T](state.shape.toSeq)
   template call(f: untyped) =
     check f(int64 q.shape[0], int64 q.shape[1], int64 q.shape[2], int64 k.shape[2], int64 q.shape[3], int64 v.shape[3], scale,
-            log_decay.get_offset_ptr, nil, go.get_offset_ptr, int64 go.strides[0], int64 go.strides[1], int64 go.strides[2],
+            log_decay.get_offset_ptr, lengths.ptrOrNil, go.get_offset_ptr, int64 go.strides[0], int64 go.strides[1], int64 go.strides[2],
             qq.get_offset_ptr, int64 qq.strides[0], int64 qq.strides[1], int64 qq.strides[2],
             kk.get_offset_ptr, int64 kk.strides[0], int64 kk.strides[1], int64 kk.strides[2],
             vv.get_offset_ptr, int64 vv.strides[0], int64 vv.strides[1], int64 vv.strides[2],
-            state.get_offset_ptr, int64 state.strides[0], int64 state.strides[1],
-            grad_state.get_offset_ptr, int64 grad_state.strides[0], int64 grad_state.strides[1],
+            state.ptrOrNil, state.strideOr0(0), state.strideOr0(1), grad_state.ptrOrNil, grad_state.strideOr0(0), grad_state.strideOr0(1),
             result.dq.get_offset_ptr, int64 result.dq.strides[0], int64 result.dq.strides[1], int64 result.dq.strides[2],
             result.dk.get_offset_ptr, int64 result.dk.strides[0], int64 result.dk.strides[1], int64 result.dk.strides[2],
             result.dv.get_offset_ptr, int64 result.dv.strides[0], int64 result.dv.strides[1], int64 result.dv.strides[2],
-            result.dstate.get_offset_ptr, int64 result.dstate.strides[0], int64 result.dstate.strides[1])
+            result.dstate.ptrOrNil, result.dstate.strideOr0(0), result.dstate.strideOr0(1))
   when T is float32: call am_hip_decay_attention_backward_f32
   else: call am_hip_decay_attention_backward_f64
 
 proc checkNorm[T](x, weight, bias: HipTensor[T], groups: int) =
-  if x.rank < 2 or not x.is_C_contiguous: raise newException(ValueError, "group_norm: a contiguous [batch, ..., channels] is needed")
+  if x.rank < 2: raise newException(ValueError, "group_norm: a tensor [batch, ..., channels] is needed")
   let C = x.shape[x.rank - 1]
-  if weight.size != C or bias.size != C or not weight.is_C_contiguous or not bias.is_C_contiguous:
+  if (weight.given and (weight.size != C or not weight.is_C_contiguous)) or (bias.given and (bias.size != C or not bias.is_C_contiguous)):
     raise newException(ValueError, "group_norm: weight and bias must be [channels]")
   if groups < 1 or C mod groups != 0:
     raise newException(ValueError, "group_norm: " & $C & " channels cannot form " & $groups & " groups")
+
+proc hipPacked[T](t: HipTensor[T]): HipTensor[T] =
+  ## `t`, or a row-major copy of it (the output of a convolution, permuted).
+  if t.is_C_contiguous: t else: t.clone()
 
 proc checkNormGradients[T](grad_output, x, mean, rstd: HipTensor[T], groups: int) =
   if grad_output.shape != x.shape or not grad_output.is_C_contiguous:
@@ -713,28 +741,33 @@ proc checkNormGradients[T](grad_output, x, mean, rstd: HipTensor[T], groups: int
 proc group_norm*[T: float32 | float64](x, weight, bias: HipTensor[T], groups: int, eps: T = 1e-5, activation = AM_ACT_NONE):
     tuple[y, mean, rstd: HipTensor[T]] =
   ## act((x - mean) / sqrt(variance + eps) * weight + bias) of a channels-last [batch, ..., channels], with what the backward pass needs.
+  ## weight and bias may be left out (1 and 0); an x whose elements are not in row-major order is copied first.
   checkNorm(x, weight, bias, groups)
   let (N, C) = (x.shape[0], x.shape[x.rank - 1])
   let S = if N * C == 0: 0 else: x.size div (N * C)
+  let src = x.hipPacked
   result = (newHipTensor[T](x.shape.toSeq), newHipTensor[T]([N, groups]), newHipTensor[T]([N, groups]))
   template call(f: untyped) =
-    check f(int64 N, int64 S, int64 C, int64 groups, eps, activation, x.get_offset_ptr, int64(S * C), int64 C, weight.get_offset_ptr, bias.get_offset_ptr,
+    check f(int64 N, int64 S, int64 C, int64 groups, eps, activation, src.get_offset_ptr, int64(S * C), int64 C, weight.ptrOrNil, bias.ptrOrNil,
             result.y.get_offset_ptr, int64(S * C), int64 C, result.mean.get_offset_ptr, result.rstd.get_offset_ptr)
   when T is float32: call am_hip_group_norm_f32
   else: call am_hip_group_norm_f64
 
 proc group_norm_backward*[T: float32 | float64](grad_output, x, weight, bias, mean, rstd: HipTensor[T], groups: int, activation = AM_ACT_NONE):
     tuple[dx, dweight, dbias: HipTensor[T]] =
-  ## The gradients of `group_norm`.
+  ## The gradients of `group_norm`; dweight and dbias are `default(HipTensor[T])` without weight and bias.
   checkNorm(x, weight, bias, groups)
   checkNormGradients(grad_output, x, mean, rstd, groups)
   let (N, C) = (x.shape[0], x.shape[x.rank - 1])
   let S = if N * C == 0: 0 else: x.size div (N * C)
-  result = (newHipTensor[T](x.shape.toSeq), newHipTensor[T](weight.shape.toSeq), newHipTensor[T](bias.shape.toSeq))
+  let src = x.hipPacked
+  result = (newHipTensor[T](x.shape.toSeq), default(HipTensor[T]), default(HipTensor[T]))
+  if weight.given: result.dweight = newHipTensor[T](weight.shape.toSeq)
+  if bias.given: result.dbias = newHipTensor[T](bias.shape.toSeq)
   template call(f: untyped) =
-    check f(int64 N, int64 S, int64 C, int64 groups, activation, grad_output.get_offset_ptr, int64(S * C), int64 C, x.get_offset_ptr, int64(S * C), int64 C,
-            weight.get_offset_ptr, bias.get_offset_ptr, mean.get_offset_ptr, rstd.get_offset_ptr, result.dx.get_offset_ptr, int64(S * C), int64 C,
-            result.dweight.get_offset_ptr, result.dbias.get_offset_ptr)
+    check f(int64 N, int64 S, int64 C, int64 groups, activation, grad_output.get_offset_ptr, int64(S * C), int64 C, src.get_offset_ptr, int64(S * C), int64 C,
+            weight.ptrOrNil, bias.ptrOrNil, mean.get_offset_ptr, rstd.get_offset_ptr, result.dx.get_offset_ptr, int64(S * C), int64 C,
+            result.dweight.ptrOrNil, result.dbias.ptrOrNil)
   when T is float32: call am_hip_group_norm_backward_f32
   else: call am_hip_group_norm_backward_f64
 

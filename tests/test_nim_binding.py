@@ -74,3 +74,17 @@ def test_the_statistics_of_group_norm_are_looked_at_before_they_are_read():
         assert what in checks
     for t in ("grad_output", "mean", "rstd"):
         assert f"not {t}.is_C_contiguous" in checks
+
+
+@pytest.mark.parametrize("name", ["decay_attention", "decay_attention_backward"])
+def test_padded_batches_reach_the_device(name):
+    text = body(name)
+    assert "lengths = default(HipTensor[int64])" in text and "checkLengths(lengths" in text and "log_decay.get_offset_ptr, lengths.ptrOrNil" in text
+
+
+@pytest.mark.parametrize("name,optional", [("rotate", ["positions"]), ("decay_attention", ["first", "lengths"]), ("decay_attention_backward", ["state", "grad_state", "lengths"]),
+                                           ("group_norm", ["weight", "bias"]), ("group_norm_backward", ["weight", "bias"])])
+def test_what_may_be_left_out_is_handed_on_as_nil(name, optional):
+    text = body(name)
+    for t in optional:
+        assert f" {t}.ptrOrNil" in text and not re.search(rf"\b{t}\.get_offset_ptr", text)
