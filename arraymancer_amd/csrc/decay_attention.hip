@@ -62,9 +62,13 @@ __device__ __forceinline__ float next_factor(Rounded f, float& debt) {
 //     o_i = sum_{j <= i} A_ij c_j + e^{g (i + after)} a_i S      A_ij = e^{g (i - j)} (a_i . b_j)
 //     S <- e^{g N} S + sum_j e^{g (N - after - j)} b_j^T c_j
 // so a chunk is four products: a b^T (32 x 32), A c, a S and b^T c. A workgroup walks the chunks of one head, a wavefront
-// owning columns of S and of o for all da rows (or half of them, below), as accumulators that never leave its registers: the product
+// owning columns of S and of o for all da rows (or half of them, below), as accumulators in its registers: the product
 // instructions leave neighbouring rows of a result in a lane, and the sum over k may take its k in any order that both
 // operands share, so the rows of S a lane holds are k of the next product's right operand as they stand.
+// Registers run out, and a few to some hundred of them are spilled, where rows are no whole vectors of 16 bytes (an address of 64
+// bits for every element) and in float64 from 192 rows on; tests/test_sequence_resources.py holds the list. us of prompt +
+// gradients, 4 x 4096 tokens, 16 heads in float32: of 128 x 128 218 + 591, of 126 x 126 376 + 1049; 2 x 1024 tokens, 8 heads in
+// float64: of 128 x 128 68 + 170, of 192 x 192 154 + 416, of 256 x 256 240 + 623.
 //   - a b^T is computed transposed, so that a lane's four values lie next to each other in a row of A in LDS; the three
 //     tiles on and under the diagonal go to three wavefronts.
 //   - c is read straight into the layout of a right operand, which A c and b^T c share.
@@ -1104,7 +1108,8 @@ template <typename T> struct StepArgs {
 };
 
 // NT: the states go past the caches both ways, where they are larger than those keep (192 sequences, 16 heads of 128 x 128:
-// 83.8 -> 77.2 us, 4.8 -> 5.2 TB/s; with the loads alone 82.6).
+// 83.8 -> 77.2 us, 4.8 -> 5.2 TB/s; with the loads alone 82.6). Single elements (rows that are no whole vectors) go through them at
+// any size: past them is not measured; heads of 126 x 126 take 84.9 us, 4.6 TB/s, of 127 x 127 in float64 5.1 TB/s.
 template <typename T, int V, bool NT>
 __global__ __launch_bounds__(256) void step(StepArgs<T> p, int lanes, int tiles) {
   typedef T vec_t __attribute__((ext_vector_type(V)));

@@ -900,7 +900,9 @@ static void launch_team(const Args<T>& p, int lanes, int units, int64_t slots, i
 template <typename T, int V, int ACT, bool BWD>
 static int team_pass(Args<T> p, int lanes, int units) {
   // Samples per team: as many as leave eight workgroups for every CU (backwards two, as the shares of the parameters'
-  // gradients have to be written and read again: [16384, 2048] in 16 groups 88 us, against 96 with one and 100 with four), and at most 64, so that a lane's shares are short sums.
+  // gradients have to be written and read again: [16384, 2048] in 16 groups 88 us, against 96 with one and 100 with four), and at most 64: a lane's shares are sums of that many
+  // terms in the result's type, 64 roundings at most (in double they would take twice the registers, which hold the sample as well),
+  // and go on in double in `channel_fold`. They keep every row of a sample, with few samples a team up to twice x in memory.
   const int64_t at_once = 256 / lanes;
   int64_t slots = (int64_t)num_cus() * (BWD ? 2 : 8) * at_once / p.groups;
   if (slots < (p.batch + 63) / 64) slots = (p.batch + 63) / 64;

@@ -11,9 +11,10 @@ walks the tokens one after the other. A layer of them, with the framework's own 
               linear(y, Wo)
 
 `decay_attention` takes prompts and training batches, `decay_attention_step` one new token of every sequence; both carry the
-same state. Naming and conventions are those of tensor_hip: float32 / float64 tensors, `_into` for a result the caller owns,
-`_forward` for the form that also returns what the backward pass needs, gradients from `_backward` functions. Operands may be
-strided views; one whose last dimension has no unit stride is copied on the device first.
+same state. Naming and conventions are those of tensor_hip: float32 / float64 tensors, `_into` for a result the caller owns
+(rotary alone has one: the others return new tensors, through the C interface they write wherever they are told), `_forward` for
+the form that also returns what the backward pass needs, gradients from `_backward` functions. Operands may be strided views; one
+whose last dimension has no unit stride is copied on the device first.
 """
 from __future__ import annotations
 

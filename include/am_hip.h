@@ -666,7 +666,8 @@ int am_hip_gru_gates_backward_f64(int64_t batch, int64_t H, const double* dnext,
  * same use - a state of fixed size per sequence, one step per new token - whose training and whose prompts run over all
  * tokens at once: rotary positions on queries and keys, linear attention with a decay for each head, and a group norm of
  * every head's output (which serves channels-last images as well). No counterpart in the reference. Strides are in elements;
- * the last dimension of every operand has unit stride. Results must not overlap operands unless it is said.
+ * the last dimension of every operand has unit stride. Results must not overlap operands unless it is said, nor themselves; a
+ * dimension of extent 1 may have any stride.
  *
  * Rotary positions. x and out [batch, tokens, heads, dim] (strides _b, _t, _h): the first rot_dim elements of a head are
  * rot_dim / 2 pairs, element i with i + rot_dim / 2 (AM_ROTARY_HALF) or 2 i with 2 i + 1 (AM_ROTARY_INTERLEAVED). Pair i of
@@ -738,7 +739,8 @@ int am_hip_decay_attention_step_f64(int64_t batch, int64_t heads, int64_t kv_hea
  * `groups` equal groups, and each (sample, group) is normalised over its spatial * channels / groups elements:
  *   y = act((x - mean) / sqrt(variance + eps) * weight[c] + bias[c])
  * weight and bias [channels] may be NULL (1 and 0). mean and rstd [batch, groups] (both or NULL) receive what the backward
- * pass needs. Sums over a group run in double, or, where the group fits the registers of a workgroup, in two passes. */
+ * pass needs. Where a group fits the registers of a workgroup its mean and its deviations are summed in two passes in the
+ * type; where it does not, in double, as means and deviations of parts of it that are put together. */
 #define AM_ACT_NONE 0
 #define AM_ACT_RELU 1   /* (0 >= z) ? 0 : z            */
 #define AM_ACT_SILU 2   /* z / (1 + e^-z)              */
