@@ -9,7 +9,8 @@
 // The angle depends on the token and the pair alone, so a lane keeps one 16-byte vector of pairs of one token, makes its
 // sines and cosines once and walks over the heads with them. Positions of long texts reach 10^5 and more, where a float
 // angle is off by 10^-2: for results of either type the angle is the product in double and sine and cosine are made in double,
-// whose reduction loses nothing however far the angle, and rounded to the result's type once, scale included.
+// whose reduction loses nothing however far the angle, and rounded to the result's type once, scale included. (Against a float sine
+// of an angle that double had reduced: [4, 2048, 32, 128] 44.6 -> 45.1 us; with one head to a token [16, 4096, 1, 64] 8.8 -> 10.7.)
 #include "common.h"
 #include "fastdiv.h"
 
