@@ -840,9 +840,10 @@ template <typename T> HipTensor<T> channels_last_(const HipTensor<T>& t, int64_t
   ss = ok && extent ? step : r.shape.back();
   return r;
 }
+inline void groups_(int64_t channels, int64_t groups) { need_(groups >= 1 && channels % groups == 0, "group_norm: the channels cannot form that many groups"); }
 template <typename T> HipTensor<T> vector_(const HipTensor<T>* t, int64_t channels) {
   if (!t) return HipTensor<T>();
-  need_(t->size() == channels && t->shape.back() == channels, "group_norm: weight and bias must be [channels]");
+  need_(t->rank() > 0 && t->size() == channels && t->shape.back() == channels, "group_norm: weight and bias must be [channels]");
   return t->is_C_contiguous() ? *t : t->clone();
 }
 }  // namespace detail
@@ -914,6 +915,8 @@ template <typename T>
 HipTensor<T> group_norm(const HipTensor<T>& x, const HipTensor<T>* weight, const HipTensor<T>* bias, int64_t groups, T eps = T(1e-5), int activation = AM_ACT_NONE,
                         std::vector<HipTensor<T>>* kept = nullptr) {
   static_assert(std::is_floating_point<T>::value, "group_norm is defined for float tensors");
+  detail::need_(x.rank() >= 2, "group_norm: a tensor [batch, ..., channels] is needed");
+  detail::groups_(x.shape.back(), groups);
   int64_t sn, ss;
   const HipTensor<T> src = detail::channels_last_(x, sn, ss);
   const int64_t N = x.shape[0], C = x.shape.back(), S = N && C ? x.size() / (N * C) : 0;
@@ -929,7 +932,9 @@ HipTensor<T> group_norm(const HipTensor<T>& x, const HipTensor<T>* weight, const
 template <typename T>
 std::vector<HipTensor<T>> group_norm_backward(const HipTensor<T>& grad_output, const HipTensor<T>& x, const HipTensor<T>* weight, const HipTensor<T>* bias,
                                               const std::vector<HipTensor<T>>& kept, int64_t groups, int activation = AM_ACT_NONE) {
+  detail::need_(x.rank() >= 2, "group_norm_backward: a tensor [batch, ..., channels] is needed");
   detail::need_(grad_output.shape == x.shape, "group_norm_backward: the output's gradient must have x's shape");
+  detail::groups_(x.shape.back(), groups);
   int64_t sn, ss, gn, gs;
   const HipTensor<T> src = detail::channels_last_(x, sn, ss), go = detail::channels_last_(grad_output, gn, gs);
   const int64_t N = x.shape[0], C = x.shape.back(), S = N && C ? x.size() / (N * C) : 0;
